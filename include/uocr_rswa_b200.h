@@ -423,6 +423,82 @@ UOCR_B200_API int uocr_b200_rswa_gather_heads_paged(
     int n, int capacity_rows, float* out_k, float* out_v, uocr_b200_workspace* ws,
     uocr_b200_stream_t stream);
 
+/* ================================================================================================
+ * Rotary positions: both layouts, part of the head, scaled for long contexts.
+ * The reference rotates whole heads in the half layout without scaling (src/kernels/cuda/rope_fused.cu:
+ * 12-40), which uocr_b200_rswa_decode_step_rope_paged folds into the fused step with that kernel's own
+ * fp32 angles.  The calls below turn pair i of every head by angle = d_positions[row] * freq_i and
+ * scale it by `amplitude`: (x0, x1) -> amplitude * (x0 cos - x1 sin, x0 sin + x1 cos).  Angles are exact
+ * to 2^-33 turns for every 32-bit position (the fused step's fp32 angles are off by up to
+ * position * 2^-24 radians); the rotation is done in fp32 and rounded once.
+ *   layout HALF: pair i is (i, i + rotary_dim/2); INTERLEAVED: (2i, 2i + 1).  Dims at and beyond
+ *     rotary_dim are copied.
+ *   freq_i = theta^(-2i/rotary_dim), and by `scaling`:
+ *     LINEAR  freq_i / factor;
+ *     BASE    theta replaced by theta * factor^(rotary_dim / (rotary_dim - 2));
+ *     RAMP    freq_i / factor * m + freq_i * (1 - m), m = clamp((i - a) / (b - a), 0, 1), where
+ *             a = max(floor(x(high)), 0), b = min(ceil(x(low)), rotary_dim - 1) (b + 0.001 where a == b), and
+ *             x(turns) = rotary_dim ln(orig_context / (2 pi turns)) / (2 ln theta) is the pair that makes
+ *             `turns` turns over the original context: pairs faster than `high` turns keep their frequency,
+ *             pairs slower than `low` are divided;
+ *     BANDS   freq_i / factor * (1 - m) + freq_i * m, m = clamp((turns_i - low) / (high - low), 0, 1) with
+ *             turns_i = orig_context freq_i / (2 pi).
+ * ============================================================================================= */
+enum { UOCR_B200_ROPE_HALF = 0, UOCR_B200_ROPE_INTERLEAVED = 1 };
+enum { UOCR_B200_ROPE_NONE = 0, UOCR_B200_ROPE_LINEAR = 1, UOCR_B200_ROPE_BASE = 2, UOCR_B200_ROPE_RAMP = 3, UOCR_B200_ROPE_BANDS = 4 };
+typedef struct {
+    int32_t layout;      /* UOCR_B200_ROPE_HALF or _INTERLEAVED                                        */
+    int32_t rotary_dim;  /* even, 2..256, at most head_dim                                             */
+    int32_t scaling;     /* UOCR_B200_ROPE_NONE ...                                                    */
+    float theta;         /* > 0 (> 1 for RAMP)                                                         */
+    float factor;        /* > 0, how many times longer the context is (not for NONE)                   */
+    float orig_context;  /* RAMP, BANDS: context length before scaling                                 */
+    float low, high;     /* RAMP, BANDS: 0 < low < high, in turns over the original context            */
+    float amplitude;     /* > 0, factor on the rotated dims (1: none)                                  */
+} uocr_b200_rope_desc;
+/* Host-side table of one model's frequencies.  Create it once; no device memory is involved and any
+ * number of streams and devices may use it at a time. */
+typedef struct uocr_b200_rope uocr_b200_rope;
+UOCR_B200_API int uocr_b200_rope_create(const uocr_b200_rope_desc* desc, uocr_b200_rope** out);
+UOCR_B200_API int uocr_b200_rope_destroy(uocr_b200_rope* rope);
+
+/* Packed projection rows.  Each of q, k, v may sit inside a wider row (one projection holding all
+ * three): row t starts `stride` elements after row t - 1.  q may be null with heads == 0.  q_out may be
+ * q itself with the same stride (in place); it must not overlap the inputs in any other way.  Rows that
+ * are 16-byte aligned, with strides to match, head_dim % 8 == 0 and (HALF) rotary_dim % 16 == 0 move in
+ * 16-byte accesses; others element by element. */
+typedef struct {
+    const void* q;
+    const void* k;
+    const void* v;
+    void* q_out; /* rotated queries, same type                                                         */
+    int64_t q_stride, k_stride, v_stride, q_out_stride; /* elements                                    */
+    int32_t dtype; /* of all four: UOCR_B200_F32 or UOCR_B200_BF16                                     */
+    int32_t heads; /* query heads                                                                      */
+} uocr_b200_qkv_rows;
+
+/* Rotates `total` rows of q and k (k_out may be k with the same stride; v is not read).  kv_heads may be
+ * 0, head_dim 2..1024.  For rows that reach the cache by another call, e.g. the text scatter. */
+UOCR_B200_API int uocr_b200_rswa_rope_rows(const uocr_b200_rope* rope, const uocr_b200_qkv_rows* rows, void* k_out,
+                                           int64_t k_out_stride, const int* d_positions, int total, int kv_heads,
+                                           int head_dim, uocr_b200_stream_t stream);
+
+/* uocr_b200_rswa_write_prefill_ragged_paged with the rotation in the same pass: q rows are rotated to
+ * q_out, k rows are rotated, rounded to the pool dtype and written with v to token d_pos[t] of the fixed
+ * region of slot d_slots[t].  Rows whose token is outside the table (status bit 4) or whose block is
+ * bad (bit 1) only have their q rotated.  No two rows may name the same token. */
+UOCR_B200_API int uocr_b200_rswa_rope_write_prefill_paged(
+    const uocr_b200_paged_kv* kv, const uocr_b200_rope* rope, const uocr_b200_qkv_rows* rows, const int* d_positions,
+    const int* d_slots, const int* d_pos, int total, uocr_b200_workspace* ws, uocr_b200_stream_t stream);
+
+/* uocr_b200_rswa_append_decode_batch_paged with the rotation in the same pass: the single-token form.
+ * Cursors advance as in that call.  A slot named twice in a batch is appended to once, for its first row;
+ * its other rows only have their q rotated and status bit 4 is set. */
+UOCR_B200_API int uocr_b200_rswa_rope_append_decode_batch_paged(
+    const uocr_b200_paged_kv* kv, const uocr_b200_rope* rope, const uocr_b200_qkv_rows* rows, const int* d_positions,
+    int* d_len, int* d_ring_pos, const int* d_prefill_len, const int* d_slots, int batch, int window,
+    uocr_b200_workspace* ws, uocr_b200_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

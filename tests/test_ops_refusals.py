@@ -1,0 +1,83 @@
+"""Arguments the cache operators refuse, as far as they are checked before the device is looked at (no GPU here)."""
+import ctypes as C
+
+import pytest
+
+from paged_fixture import load_b200
+
+
+@pytest.fixture(scope="module")
+def b():
+    import os
+    m = load_b200()
+    if not os.path.exists(m.LIB_PATH):
+        m.build()
+    return m
+
+
+GOOD = dict(layout="half", rotary_dim=64, theta=10000.0)
+
+
+@pytest.mark.parametrize("change", [
+    dict(rotary_dim=0), dict(rotary_dim=63), dict(rotary_dim=258), dict(rotary_dim=-2), dict(theta=0.0), dict(theta=-1.0), dict(theta=float("nan")),
+    dict(theta=float("inf")), dict(amplitude=0.0), dict(amplitude=float("nan")), dict(scaling="linear", factor=0.0),
+    dict(scaling="base", factor=float("inf")), dict(scaling="ramp", factor=4.0, orig_context=0.0, low=1.0, high=32.0),
+    dict(scaling="ramp", factor=4.0, orig_context=4096.0, low=32.0, high=1.0), dict(scaling="ramp", factor=4.0, orig_context=4096.0, low=0.0, high=1.0),
+    dict(scaling="ramp", factor=4.0, orig_context=4096.0, low=1.0, high=32.0, theta=1.0),
+    dict(scaling="bands", factor=4.0, orig_context=4096.0, low=4.0, high=4.0),
+])
+def test_rope_create_refuses(b, change):
+    with pytest.raises(b.Error):
+        b.Rope(**{**GOOD, **change})
+
+
+def test_rope_create_unknown_enums(b):
+    h = C.c_void_p()
+    for layout, scaling in ((2, 0), (-1, 0), (0, 5), (0, -1)):
+        desc = b.RopeDesc(layout, 64, scaling, 10000.0, 2.0, 4096.0, 1.0, 4.0, 1.0)
+        assert b.lib().uocr_b200_rope_create(C.byref(desc), C.byref(h)) != 0
+    assert b.lib().uocr_b200_rope_create(None, C.byref(h)) != 0
+    assert b.lib().uocr_b200_rope_create(C.byref(b.RopeDesc(0, 64, 0, 10000.0, 1.0, 0.0, 0.0, 0.0, 1.0)), None) != 0
+    assert b.lib().uocr_b200_rope_destroy(None) == 0
+
+
+def test_rope_calls_refuse(b):
+    rope = b.Rope(**GOOD)
+    L = b.lib()
+    fake = 0x1000  # never dereferenced: every call below is refused first
+    ok = dict(q=fake, k=fake, v=fake, q_out=fake, q_stride=128, k_stride=128, v_stride=128, q_out_stride=128, dtype=0, heads=1)
+    rows = lambda **kw: C.byref(b.QkvRows(**{**ok, **kw}))
+    call = lambda r, kv_heads=1, head_dim=128, k_out=fake, k_out_stride=128, pos=fake, total=4, h=None: L.uocr_b200_rswa_rope_rows(
+        rope.h if h is None else h, r, k_out, k_out_stride, pos, total, kv_heads, head_dim, None)
+    assert call(rows(), total=0) == 0
+    assert call(rows(), pos=None) == 1
+    assert call(None) == 1
+    assert call(rows(), h=0) == 1
+    assert call(rows(dtype=2)) == 2
+    assert call(rows(heads=-1)) == 1
+    assert call(rows(heads=0), kv_heads=0) == 1
+    assert call(rows(heads=5000)) == 1
+    assert call(rows(q=None)) == 1
+    assert call(rows(q_out=None)) == 1
+    assert call(rows(), k_out=None) == 1
+    assert call(rows(), head_dim=32) == 1          # smaller than the rotated dims
+    assert call(rows(), head_dim=2048) == 1
+    assert call(rows(q_stride=127)) == 1
+    assert call(rows(q_out_stride=64)) == 1
+    assert call(rows(k_stride=0)) == 1
+    assert call(rows(), k_out_stride=1) == 1
+    assert call(rows(q_stride=256)) == 1           # in place with two strides
+    kv = b.PagedKV(fake, fake, fake, 4, 8, 1, 128, b.BF16)
+    write = lambda v=kv, r=None, slots=fake, pos=fake: L.uocr_b200_rswa_rope_write_prefill_paged(
+        C.byref(v) if v else None, rope.h, r or rows(), fake, slots, pos, 4, None, None)
+    assert write(v=None) == 1
+    assert write(slots=None) == 1
+    assert write(pos=None) == 1
+    assert write(r=rows(v=None)) == 1
+    assert write(r=rows(v_stride=3)) == 1
+    assert write(v=b.PagedKV(fake, fake, fake, 4, 8, 1, 96, b.BF16)) == 2
+    assert write(v=b.PagedKV(fake + 8, fake, fake, 4, 8, 1, 128, b.BF16)) == 1
+    app = lambda window=8, ln=fake: L.uocr_b200_rswa_rope_append_decode_batch_paged(
+        C.byref(kv), rope.h, rows(), fake, ln, fake, fake, fake, 4, window, None, None)
+    assert app(window=0) == 1
+    assert app(ln=None) == 1

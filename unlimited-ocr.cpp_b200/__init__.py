@@ -25,7 +25,7 @@ BLOCK_TOKENS = 16
 STATUS_BAD_BLOCK, STATUS_WAIT_TIMEOUT, STATUS_BAD_SLOT = 1, 2, 4
 
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
-              "-Xcompiler", "-fPIC,-fvisibility=hidden", "-shared"]
+              "-Xcompiler", "-fPIC,-fvisibility=hidden", "-shared", "-t", "0"]
 
 
 def sources():
@@ -48,6 +48,20 @@ class PagedKV(C.Structure):
     _fields_ = [("k_pool", C.c_void_p), ("v_pool", C.c_void_p), ("block_table", C.c_void_p),
                 ("table_stride", C.c_int32), ("num_blocks", C.c_int32), ("kv_heads", C.c_int32),
                 ("head_dim", C.c_int32), ("dtype", C.c_int32)]
+
+
+class RopeDesc(C.Structure):
+    """uocr_b200_rope_desc"""
+    _fields_ = [("layout", C.c_int32), ("rotary_dim", C.c_int32), ("scaling", C.c_int32), ("theta", C.c_float),
+                ("factor", C.c_float), ("orig_context", C.c_float), ("low", C.c_float), ("high", C.c_float),
+                ("amplitude", C.c_float)]
+
+
+class QkvRows(C.Structure):
+    """uocr_b200_qkv_rows"""
+    _fields_ = [("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p), ("q_out", C.c_void_p), ("q_stride", C.c_int64),
+                ("k_stride", C.c_int64), ("v_stride", C.c_int64), ("q_out_stride", C.c_int64), ("dtype", C.c_int32),
+                ("heads", C.c_int32)]
 
 
 class Error(RuntimeError):
@@ -103,6 +117,11 @@ _SIGS = {
     "uocr_b200_rswa_attention_paged": (_i, [C.POINTER(PagedKV), _i, _vp, _i, _vp, _i, _vp] + [_i] * 4 + [_vp, _vp, _vp]),
     "uocr_b200_rswa_gather_paged": (_i, [C.POINTER(PagedKV)] + [_vp] * 3 + [_i, _i, _vp, _vp, _i, _vp, _vp]),
     "uocr_b200_rswa_gather_heads_paged": (_i, [C.POINTER(PagedKV)] + [_vp] * 3 + [_i, _i, _vp, _vp, _vp, _vp]),
+    "uocr_b200_rope_create": (_i, [C.POINTER(RopeDesc), C.POINTER(_vp)]),
+    "uocr_b200_rope_destroy": (_i, [_vp]),
+    "uocr_b200_rswa_rope_rows": (_i, [_vp, C.POINTER(QkvRows), _vp, _i64, _vp, _i, _i, _i, _vp]),
+    "uocr_b200_rswa_rope_write_prefill_paged": (_i, [C.POINTER(PagedKV), _vp, C.POINTER(QkvRows)] + [_vp] * 3 + [_i, _vp, _vp]),
+    "uocr_b200_rswa_rope_append_decode_batch_paged": (_i, [C.POINTER(PagedKV), _vp, C.POINTER(QkvRows)] + [_vp] * 5 + [_i, _i, _vp, _vp]),
 }
 
 
@@ -239,15 +258,20 @@ def launch_count() -> int:
 
 
 class PagedLayer:
-    """Device storage of one layer's paged KV plus the descriptor the C ABI takes."""
+    """Device storage of one layer's paged KV plus the descriptor the C ABI takes.  `pools`: K and V
+    tensors the caller already holds, [num_blocks, kv_heads, 16, head_dim]; otherwise zero-filled ones are made."""
 
-    def __init__(self, num_blocks, kv_heads, head_dim, dtype, table, device="cuda"):
+    def __init__(self, num_blocks, kv_heads, head_dim, dtype, table, device="cuda", pools=None):
         import torch
         self.dtype = dtype
         tdt = torch.bfloat16 if dtype == BF16 else torch.float32
         shape = (num_blocks, kv_heads, BLOCK_TOKENS, head_dim)
-        self.k = torch.zeros(shape, dtype=tdt, device=device)
-        self.v = torch.zeros(shape, dtype=tdt, device=device)
+        if pools is None:
+            pools = tuple(torch.zeros(shape, dtype=tdt, device=device) for _ in range(2))
+        for t in pools:
+            if tuple(t.shape) != shape or t.dtype != tdt or not t.is_contiguous():
+                raise ValueError(f"a pool must be a contiguous {tdt} tensor of shape {shape}")
+        self.k, self.v = pools
         self.table = table  # int32 [slots, stride], shared between layers
         self.desc = PagedKV(self.k.data_ptr(), self.v.data_ptr(), table.data_ptr(), table.shape[1],
                             num_blocks, kv_heads, head_dim, dtype)
@@ -443,3 +467,70 @@ def attention_f32(q, kcache, vcache, kv_len, d_len, seq, q_start, heads, kv_head
     check(lib().uocr_b200_rswa_attention_f32(_p(q), _p(kcache), _p(vcache), kv_len, _p(d_len), seq, q_start, heads,
                                               kv_heads, head_dim, 1 if causal else 0, _p(out), ws.h,
                                               stream_handle(stream)))
+
+
+# ---- rotary positions --------------------------------------------------------------------------------
+
+_ROPE_LAYOUTS = {"half": 0, "interleaved": 1}
+_ROPE_SCALINGS = {"none": 0, "linear": 1, "base": 2, "ramp": 3, "bands": 4}
+
+
+class Rope:
+    """Frequencies of one model (uocr_b200_rope): see the header for the layouts and scalings."""
+
+    def __init__(self, layout="half", rotary_dim=128, theta=10000.0, scaling="none", factor=1.0, orig_context=0.0, low=0.0, high=0.0,
+                 amplitude=1.0):
+        desc = RopeDesc(_ROPE_LAYOUTS[layout], rotary_dim, _ROPE_SCALINGS[scaling], theta, factor, orig_context, low, high, amplitude)
+        h = _vp()
+        check(lib().uocr_b200_rope_create(C.byref(desc), C.byref(h)))
+        self.h = h
+
+    def __del__(self):
+        try:
+            lib().uocr_b200_rope_destroy(self.h)
+        except Exception:
+            pass
+
+
+def _dtype_of(t):
+    import torch
+    if t.dtype == torch.float32:
+        return F32
+    if t.dtype == torch.bfloat16:
+        return BF16
+    raise ValueError(f"rows must be float32 or bfloat16, got {t.dtype}")
+
+
+def _qkv_rows(q, k, v, q_out, heads):
+    """Packed rows, [rows, width] each with its own row stride and contiguous elements."""
+    ref = q if q is not None else k
+    for t in (q, k, v, q_out):
+        if t is not None and (t.dtype != ref.dtype or t.shape[0] != ref.shape[0] or t.stride(1) != 1 or t.device != ref.device):
+            raise ValueError("q, k, v and q_out must have one type, row count and device, and contiguous rows")
+    s = lambda t: 0 if t is None else (t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1]))
+    return QkvRows(_p(q), _p(k), _p(v), _p(q_out), s(q), s(k), s(v), s(q_out), _dtype_of(ref), heads)
+
+
+def rope_rows(rope, q, k, q_out, k_out, d_positions, heads, kv_heads, head_dim, stream=None):
+    """Rotates the packed rows of q and k (either may be None with 0 heads; outputs may be the inputs)."""
+    rows = _qkv_rows(q, k, None, q_out, heads)
+    if k_out is not None and (k_out.dtype != k.dtype or k_out.stride(1) != 1 or k_out.shape != k.shape):
+        raise ValueError("k_out must have k's type and shape, and contiguous rows")
+    check(lib().uocr_b200_rswa_rope_rows(rope.h, C.byref(rows), _p(k_out), k_out.stride(0) if k_out is not None else 0, _p(d_positions),
+                                         (q if q is not None else k).shape[0], kv_heads, head_dim, stream_handle(stream)))
+
+
+def rope_write_prefill_paged(layer, rope, q, k, v, q_out, d_positions, d_slots, d_pos, heads, ws=None, stream=None):
+    """rope + write_prefill_ragged_paged in one pass."""
+    rows = _qkv_rows(q, k, v, q_out, heads)
+    check(lib().uocr_b200_rswa_rope_write_prefill_paged(layer.ref(), rope.h, C.byref(rows), _p(d_positions), _p(d_slots), _p(d_pos),
+                                                        k.shape[0], ws.h if ws else None, stream_handle(stream)))
+
+
+def rope_append_decode_batch_paged(layer, rope, q, k, v, q_out, d_positions, d_len, d_ring, d_prefill, d_slots, window, heads, ws=None,
+                                   stream=None):
+    """rope + append_decode_batch_paged in one pass."""
+    rows = _qkv_rows(q, k, v, q_out, heads)
+    check(lib().uocr_b200_rswa_rope_append_decode_batch_paged(layer.ref(), rope.h, C.byref(rows), _p(d_positions), _p(d_len), _p(d_ring),
+                                                              _p(d_prefill), _p(d_slots), k.shape[0], window, ws.h if ws else None,
+                                                              stream_handle(stream)))

@@ -16,6 +16,7 @@
 #include "rswa_copy.cuh"
 #include "rswa_prefill_tc.cuh"
 #include "rswa_stream_read.cuh"
+#include "rswa_workspace.cuh"
 #include "uocr_rswa_b200.h"
 
 using namespace uocr_b200;
@@ -24,6 +25,13 @@ namespace {
 
 thread_local std::string g_last_error;
 std::atomic<uint64_t> g_launches{0};
+DeviceInfo g_dev[64];
+
+constexpr int kMaxWarpsPerCta = UOCR_ATTN_THREADS / 32;
+
+}  // namespace
+
+namespace uocr_b200 {
 
 int fail(int code, const std::string& msg) {
     g_last_error = msg;
@@ -34,26 +42,12 @@ int cuda_fail(cudaError_t e, const char* what) {
     return fail(UOCR_B200_ERR_CUDA, std::string(what) + ": " + cudaGetErrorString(e));
 }
 
-#define CHECK_CUDA(expr, what)                             \
-    do {                                                   \
-        cudaError_t e_ = (expr);                           \
-        if (e_ != cudaSuccess) return cuda_fail(e_, what); \
-    } while (0)
-
 int after_launch(const char* what) {
     g_launches.fetch_add(1, std::memory_order_relaxed);
     cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return cuda_fail(e, what);
     return UOCR_B200_OK;
 }
-
-struct DeviceInfo {
-    bool known = false;
-    int sms = 0;
-    int smem_optin = 0;
-    int cc_major = 0;
-};
-DeviceInfo g_dev[64];
 
 int device_info(const DeviceInfo** out) {
     int dev = 0;
@@ -73,49 +67,11 @@ int device_info(const DeviceInfo** out) {
     return UOCR_B200_OK;
 }
 
-constexpr int kMaxWarpsPerCta = UOCR_ATTN_THREADS / 32;
-constexpr int kMaxHeadDim = 256;
-
-bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
-
-bool head_dim_ok(int hd, int dtype) {
-    if (hd < (dtype == UOCR_B200_BF16 ? 8 : 4) || hd > kMaxHeadDim) return false;
-    return (hd & (hd - 1)) == 0;
-}
-
-}  // namespace
+}  // namespace uocr_b200
 
 // =================================================================================================
 // workspace
 // =================================================================================================
-struct uocr_b200_workspace {
-    int device = 0;
-    int max_rows = 0;
-    int total_warps_max = 0;
-    uint8_t* base = nullptr;
-    size_t bytes = 0;
-    int* status = nullptr;
-    int* rs = nullptr;
-    RowInfo* info = nullptr;
-    float* part_acc = nullptr;
-    float* part_ml = nullptr;
-    int* counters = nullptr;   // [pieces_max] arrival counters, zero between launches
-    int* planned_ctas = nullptr;  // fused step: ticket counter of CTAs that have planned; wraps to zero by itself
-    int pieces_max = 0;
-    uint32_t wait_limit = kWaitLimit;  // polls a tile wait may take (uocr_b200_workspace_set_wait_limit)
-    PrefillTile* tiles = nullptr;  // [max_rows] query-tile descriptors of the tensor-core prefill
-    TcWork* tile_work = nullptr;   // [max_rows] the same tiles, most key tiles first, with their key-tile counts
-    int* item_counter = nullptr;   // items the persistent prefill grid has handed out beyond every CTA's first
-    int plan_tiles = 0;            // tiles of the plan in tile_work (0: none)
-    int plan_window = 0;
-    bool plan_any_text = false;
-    unsigned plan_serial = 0;      // plans made on this workspace so far
-    int tiles_cap = 0;
-    bool out_bf16 = false;  // attention results are written as bf16 instead of fp32
-    bool timing = false;
-    bool overlap = false;  // fused decode step may start its prologue before the preceding kernel ends
-    cudaEvent_t ev0 = nullptr, ev1 = nullptr;
-};
 
 extern "C" {
 
@@ -151,12 +107,15 @@ int uocr_b200_workspace_create(int max_rows, uocr_b200_workspace** out) {
     const size_t o_info = o_rs + up(sizeof(int) * (size_t)(max_rows + 1));
     ws->pieces_max = ws->total_warps_max;
     const size_t o_acc = o_info + up(sizeof(RowInfo) * (size_t)max_rows);
-    const size_t o_ml = o_acc + up(sizeof(float) * 2 * (size_t)ws->pieces_max * kMaxHeadDim);
-    const size_t o_cnt = o_ml + up(sizeof(float) * 4 * (size_t)ws->pieces_max);
+    const size_t o_ml = o_acc + up(sizeof(float) * 2 * (size_t)ws->pieces_max * kPartElems);
+    const size_t o_cnt = o_ml + up(sizeof(float) * 4 * kScoreMaxGroup * (size_t)ws->pieces_max);
     const size_t o_tiles = o_cnt + up(sizeof(int) * ((size_t)ws->pieces_max + 64));
     ws->tiles_cap = max_rows;
     const size_t o_order = o_tiles + up(sizeof(PrefillTile) * (size_t)ws->tiles_cap);
-    ws->bytes = o_order + up(sizeof(TcWork) * (size_t)ws->tiles_cap) + 256;
+    const size_t o_count = o_order + up(sizeof(TcWork) * (size_t)ws->tiles_cap);
+    const size_t o_srow = o_count + 256;
+    const size_t o_srs = o_srow + up(kScoreRowBytes * (size_t)max_rows);
+    ws->bytes = o_srs + up(sizeof(long long) * (size_t)(max_rows + 1));
     cudaError_t e = cudaMalloc(&ws->base, ws->bytes);
     if (e != cudaSuccess) {
         delete ws;
@@ -177,7 +136,9 @@ int uocr_b200_workspace_create(int max_rows, uocr_b200_workspace** out) {
     ws->planned_ctas = ws->counters + ws->pieces_max;
     ws->tiles = reinterpret_cast<PrefillTile*>(ws->base + o_tiles);
     ws->tile_work = reinterpret_cast<TcWork*>(ws->base + o_order);
-    ws->item_counter = reinterpret_cast<int*>(ws->base + o_order + up(sizeof(TcWork) * (size_t)ws->tiles_cap));
+    ws->item_counter = reinterpret_cast<int*>(ws->base + o_count);
+    ws->score_rows = reinterpret_cast<ScoreRow*>(ws->base + o_srow);
+    ws->score_rs = reinterpret_cast<long long*>(ws->base + o_srs);
     *out = ws;
     return UOCR_B200_OK;
 }
@@ -497,6 +458,11 @@ int fill_paged(AttnCall& c, const uocr_b200_paged_kv* kv) {
     return UOCR_B200_OK;
 }
 
+
+}  // namespace
+
+namespace uocr_b200 {
+
 int paged_view(const uocr_b200_paged_kv* kv, PagedView* pv) {
     if (!kv || !kv->k_pool || !kv->v_pool || !kv->block_table) return fail(UOCR_B200_ERR_INVALID, "paged view: null pointer");
     if (kv->dtype != UOCR_B200_BF16 && kv->dtype != UOCR_B200_F32) return fail(UOCR_B200_ERR_UNSUPPORTED, "paged dtype must be bf16 or fp32");
@@ -512,7 +478,7 @@ int paged_view(const uocr_b200_paged_kv* kv, PagedView* pv) {
     return UOCR_B200_OK;
 }
 
-}  // namespace
+}  // namespace uocr_b200
 
 extern "C" {
 

@@ -3,28 +3,9 @@
 // All are pure HBM traffic: 16-byte vector accesses, one cache row (or row chunk) per thread group.
 #pragma once
 
-#include "rswa_device.cuh"
+#include "rswa_paged.cuh"
 
 namespace uocr_b200 {
-
-// The ring state machine of RSWACache::append_decode (src/scheduler/kv_cache.cpp:54-82) on device
-// cursors, as in rswa_append_batch_kernel (src/kernels/cuda/rswa_attention.cu:309-338) -- except
-// that exactly one thread reads and updates the cursors (the reference lets every thread of the
-// CTA do both without a barrier in between).  Returns the logical slot to write.
-__device__ __forceinline__ int ring_advance(int* len_p, int* ring_p, int prefill_len, int window) {
-    const int len = *len_p;
-    int row;
-    if (len < prefill_len + window) {
-        row = len;
-        *len_p = len + 1;
-        if (len + 1 >= prefill_len + window) *ring_p = 0;
-    } else {
-        const int rp = *ring_p;
-        row = prefill_len + rp;
-        *ring_p = (rp + 1) % window;
-    }
-    return row;
-}
 
 // ---- contiguous fp32 caches (the reference's own layout) ----------------------------------------
 __global__ void __launch_bounds__(256) rswa_append_f32_kernel(
@@ -89,14 +70,6 @@ __global__ void __launch_bounds__(256) rswa_scatter_f32_kernel(
     }
 }
 
-// ---- paged pool: [block][kv_head][16][head_dim] ---------------------------------------------------
-struct PagedView {
-    uint8_t* k_pool;
-    uint8_t* v_pool;
-    const int32_t* table;
-    int table_stride, num_blocks, kv_heads, head_dim;
-};
-
 // Writes one fp32 row (kv_heads*head_dim) into (block, offset) of the pool, rounding to KV.
 // One thread per 16-byte destination chunk.
 template <typename KV>
@@ -127,13 +100,6 @@ __device__ __forceinline__ void store_row_paged(const PagedView& pv, int blk, in
         }
     }
 }
-
-// Pools of several layers for the kernels that serve all layers of a step in one launch (blockIdx.z = layer).
-constexpr int kMaxLayersPerLaunch = 32;
-struct LayerPools {
-    uint8_t* k[kMaxLayersPerLaunch];
-    uint8_t* v[kMaxLayersPerLaunch];
-};
 
 template <typename KV>
 __device__ __forceinline__ void append_paged_row(const PagedView& pv, const float* __restrict__ k, const float* __restrict__ v,
