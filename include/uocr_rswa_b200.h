@@ -499,6 +499,72 @@ UOCR_B200_API int uocr_b200_rswa_rope_append_decode_batch_paged(
     int* d_len, int* d_ring_pos, const int* d_prefill_len, const int* d_slots, int batch, int window,
     uocr_b200_workspace* ws, uocr_b200_stream_t stream);
 
+/* ================================================================================================
+ * Attention with modified scores (no reference counterpart; the reference's attention is the plain
+ * softmax of src/scheduler/kv_cache.cpp:84-130, to which these reduce with an all-default descriptor):
+ *
+ *   x = scale * q.k;  x <- softcap * tanh(x / softcap);  x <- x - slopes[head] * |pos_q - pos_k|;
+ *   out = sum over the visible keys of softmax(x) v,  0 for a row that sees no key.
+ *
+ * Of the fixed region row r sees tokens [d_lo[r], d_hi[r]) -- a page of a document, a whole prefix in
+ * both directions, a document up to the row itself -- cut to the region; an empty range hides it.
+ * Ring and text-window tokens are all visible, as in the plain calls.  Keys and values a row does not
+ * see are never multiplied: they may hold anything, NaN included (the tensor-core call below states its
+ * own rule).  Everything is computed in fp32; `out` is fp32 or bf16 as the workspace says.
+ * ============================================================================================= */
+typedef struct {
+    float scale;         /* 0: 1/sqrt(head_dim)                                                        */
+    float softcap;       /* 0: none                                                                    */
+    const float* slopes; /* device [heads], or null: no bias                                           */
+    const int* d_q_pos;  /* device [rows], position of each query row; needed with slopes (ragged vision
+                            rows default to d_pos)                                                     */
+    const int* d_key_pos; /* device [slots][key_pos_stride], positions of the fixed region's tokens, e.g.
+                            after an eviction; null (and tokens beyond the stride): their own index.   */
+    int32_t key_pos_stride;
+    const int* d_lo;     /* device [rows], or null: 0                                                  */
+    const int* d_hi;     /* device [rows], or null: the whole region (decode and text rows), d_pos + 1
+                            (ragged vision rows)                                                       */
+} uocr_b200_score;
+
+/* Attention weights of a decode step, summed over heads and rows into one number per token of the fixed
+ * region: mass_out[slot][s] = decay * mass_in[slot][s] + sum of the weights, for every token s of the fixed
+ * region of every slot in the batch.  Sums are made in a fixed order: the same call gives the same bits.  Tokens a
+ * row does not see get no weight from it.  Entries beyond the region and slots outside the batch are
+ * left alone; a region longer than `stride` sets status bit 4 and its further tokens are not recorded. */
+typedef struct {
+    const float* mass_in; /* device [slots][stride]; null or decay == 0: not read                      */
+    float* mass_out;      /* device [slots][stride]; may be mass_in                                    */
+    int32_t stride;
+    float decay;          /* >= 0                                                                      */
+    void* scratch;        /* device, uocr_b200_rswa_mass_scratch_bytes(batch, heads, stride), 16-byte aligned */
+    size_t scratch_bytes;
+} uocr_b200_mass;
+UOCR_B200_API size_t uocr_b200_rswa_mass_scratch_bytes(int batch, int heads, int stride);
+
+/* One new token per row over prefix + ring, split over the cache's length and joined: what
+ * uocr_b200_rswa_attention_batch_paged is to the plain softmax.  d_len / d_ring_pos are the cursors the append
+ * left (the newest ring token is the row's own, at distance 0).  `mass` may be null. */
+UOCR_B200_API int uocr_b200_rswa_attention_scored_batch_paged(
+    const uocr_b200_paged_kv* kv, const uocr_b200_score* score, const void* q, int q_dtype, const int* d_len,
+    const int* d_ring_pos, const int* d_prefill_len, const int* d_slots, int batch, int window, int heads, void* out,
+    const uocr_b200_mass* mass, uocr_b200_workspace* ws, uocr_b200_stream_t stream);
+
+/* Packed vision rows over the fixed region, any geometry: uocr_b200_rswa_attention_ragged_paged with
+ * modified scores.  Row t is token d_pos[t] of slot d_slots[t] (causal unless d_hi says otherwise). */
+UOCR_B200_API int uocr_b200_rswa_attention_scored_ragged_paged(
+    const uocr_b200_paged_kv* kv, const uocr_b200_score* score, const void* q, int q_dtype, const int* d_prefill_len,
+    const int* d_slots, const int* d_pos, int total, int heads, void* out, uocr_b200_workspace* ws,
+    uocr_b200_stream_t stream);
+
+/* Packed text rows over the fixed region and the text window (pos - window, pos], any geometry: the
+ * attention half of uocr_b200_rswa_prefill_text_paged with modified scores.  The rows' K and V must already be
+ * in the text pool (uocr_b200_rswa_text_scatter_paged or its ring-filling form). */
+UOCR_B200_API int uocr_b200_rswa_prefill_text_scored_paged(
+    const uocr_b200_paged_kv* kv, const void* text_k_pool, const void* text_v_pool, int text_blocks,
+    const uocr_b200_score* score, const void* q, int q_dtype, const int* d_prefill_len, const int* d_slots,
+    const int* d_pos, const int* d_text_block0, int total, int window, int heads, void* out, uocr_b200_workspace* ws,
+    uocr_b200_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -81,3 +81,26 @@ def test_rope_calls_refuse(b):
         C.byref(kv), rope.h, rows(), fake, ln, fake, fake, fake, 4, window, None, None)
     assert app(window=0) == 1
     assert app(ln=None) == 1
+
+
+def test_scored_calls_refuse(b):
+    L, fake = b.lib(), 0x1000
+    kv = b.PagedKV(fake, fake, fake, 4, 8, 2, 128, b.BF16)
+    ok = dict(scale=0.0, softcap=0.0, slopes=None, d_q_pos=None, d_key_pos=None, key_pos_stride=0, d_lo=None, d_hi=None)
+    sc = lambda **kw: C.byref(b.ScoreDesc(**{**ok, **kw}))
+    inf, nan = float("inf"), float("nan")
+
+    def decode(score=None, v=kv, q=fake, q_dtype=0, ln=fake, ring=fake, pre=fake, slots=fake, batch=4, window=16, heads=4, out=fake, mass=None, ws=None):
+        return L.uocr_b200_rswa_attention_scored_batch_paged(C.byref(v) if v else None, sc() if score is None else score, q, q_dtype, ln, ring, pre, slots,
+                                                             batch, window, heads, out, mass, ws, None)
+    assert decode(batch=0) == 0
+    assert decode() == 1 and b"null" in L.uocr_b200_last_error()  # no workspace
+    assert decode(ln=None) == 1 and decode(ring=None) == 1 and decode(window=0) == 1 and decode(v=None) == 1
+    assert decode(v=b.PagedKV(fake, fake, fake, 4, 8, 2, 96, b.BF16)) == 2
+    assert L.uocr_b200_rswa_attention_scored_ragged_paged(C.byref(kv), sc(), fake, 0, fake, fake, None, 4, 4, fake, None, None) == 1
+    text = lambda kt=fake, blocks=4, window=4, b0=fake: L.uocr_b200_rswa_prefill_text_scored_paged(
+        C.byref(kv), kt, fake, blocks, sc(), fake, 0, fake, fake, fake, b0, 4, window, 4, fake, None, None)
+    assert text(kt=None) == 1 and text(kt=fake + 8) == 1 and text(blocks=0) == 1 and text(window=0) == 1 and text(b0=None) == 1
+    assert L.uocr_b200_rswa_mass_scratch_bytes(0, 4, 4) == 0
+    assert L.uocr_b200_rswa_mass_scratch_bytes(3, 2, 5) == 128 + 48
+    assert L.uocr_b200_rswa_mass_scratch_bytes(60000, 100, 100000) == 4 * 60000 * 100 * 100000 + 8 * 60000 * 100

@@ -64,6 +64,18 @@ class QkvRows(C.Structure):
                 ("heads", C.c_int32)]
 
 
+class ScoreDesc(C.Structure):
+    """uocr_b200_score"""
+    _fields_ = [("scale", C.c_float), ("softcap", C.c_float), ("slopes", C.c_void_p), ("d_q_pos", C.c_void_p), ("d_key_pos", C.c_void_p),
+                ("key_pos_stride", C.c_int32), ("d_lo", C.c_void_p), ("d_hi", C.c_void_p)]
+
+
+class MassDesc(C.Structure):
+    """uocr_b200_mass"""
+    _fields_ = [("mass_in", C.c_void_p), ("mass_out", C.c_void_p), ("stride", C.c_int32), ("decay", C.c_float), ("scratch", C.c_void_p),
+                ("scratch_bytes", C.c_size_t)]
+
+
 class Error(RuntimeError):
     def __init__(self, status, msg):
         super().__init__(f"uocr_b200 status {status}: {msg}")
@@ -117,6 +129,11 @@ _SIGS = {
     "uocr_b200_rswa_attention_paged": (_i, [C.POINTER(PagedKV), _i, _vp, _i, _vp, _i, _vp] + [_i] * 4 + [_vp, _vp, _vp]),
     "uocr_b200_rswa_gather_paged": (_i, [C.POINTER(PagedKV)] + [_vp] * 3 + [_i, _i, _vp, _vp, _i, _vp, _vp]),
     "uocr_b200_rswa_gather_heads_paged": (_i, [C.POINTER(PagedKV)] + [_vp] * 3 + [_i, _i, _vp, _vp, _vp, _vp]),
+    "uocr_b200_rswa_mass_scratch_bytes": (C.c_size_t, [_i, _i, _i]),
+    "uocr_b200_rswa_attention_scored_batch_paged": (_i, [C.POINTER(PagedKV), C.POINTER(ScoreDesc), _vp, _i] + [_vp] * 4 + [_i, _i, _i, _vp, _vp, _vp, _vp]),
+    "uocr_b200_rswa_attention_scored_ragged_paged": (_i, [C.POINTER(PagedKV), C.POINTER(ScoreDesc), _vp, _i] + [_vp] * 3 + [_i, _i, _vp, _vp, _vp]),
+    "uocr_b200_rswa_prefill_text_scored_paged": (_i, [C.POINTER(PagedKV), _vp, _vp, _i, C.POINTER(ScoreDesc), _vp, _i] + [_vp] * 4 +
+                                                 [_i, _i, _i, _vp, _vp, _vp]),
     "uocr_b200_rope_create": (_i, [C.POINTER(RopeDesc), C.POINTER(_vp)]),
     "uocr_b200_rope_destroy": (_i, [_vp]),
     "uocr_b200_rswa_rope_rows": (_i, [_vp, C.POINTER(QkvRows), _vp, _i64, _vp, _i, _i, _i, _vp]),
@@ -534,3 +551,54 @@ def rope_append_decode_batch_paged(layer, rope, q, k, v, q_out, d_positions, d_l
     check(lib().uocr_b200_rswa_rope_append_decode_batch_paged(layer.ref(), rope.h, C.byref(rows), _p(d_positions), _p(d_len), _p(d_ring),
                                                               _p(d_prefill), _p(d_slots), k.shape[0], window, ws.h if ws else None,
                                                               stream_handle(stream)))
+
+
+# ---- attention with modified scores --------------------------------------------------------------------
+
+class Score:
+    """Scale, cap, distance bias and visible ranges of one call (uocr_b200_score); keeps its tensors alive."""
+
+    def __init__(self, scale=0.0, softcap=0.0, slopes=None, d_q_pos=None, d_key_pos=None, d_lo=None, d_hi=None):
+        import torch
+        for t, dt in ((slopes, torch.float32), (d_q_pos, torch.int32), (d_key_pos, torch.int32), (d_lo, torch.int32), (d_hi, torch.int32)):
+            if t is not None and (t.dtype != dt or not t.is_contiguous()):
+                raise ValueError(f"expected a contiguous {dt} tensor")
+        self.keep = (slopes, d_q_pos, d_key_pos, d_lo, d_hi)
+        self.desc = ScoreDesc(scale, softcap, _p(slopes), _p(d_q_pos), _p(d_key_pos), d_key_pos.shape[1] if d_key_pos is not None else 0,
+                              _p(d_lo), _p(d_hi))
+
+
+class Mass:
+    """Accumulated attention weights of the fixed region, [slots, stride] (uocr_b200_mass), with scratch for `batch` rows."""
+
+    def __init__(self, mass_in, mass_out, batch, heads, decay=1.0):
+        import torch
+        for t in (mass_in, mass_out):
+            if t is not None and (t.dtype != torch.float32 or not t.is_contiguous() or t.shape != mass_out.shape):
+                raise ValueError("the mass must be contiguous float32, [slots, stride]")
+        stride = mass_out.shape[1]
+        n = lib().uocr_b200_rswa_mass_scratch_bytes(batch, heads, stride)
+        self.scratch = torch.empty(n, dtype=torch.uint8, device=mass_out.device)
+        self.keep = (mass_in, mass_out)
+        self.desc = MassDesc(_p(mass_in), _p(mass_out), stride, decay, _p(self.scratch), n)
+
+
+def attention_scored_batch_paged(layer, score, q, d_len, d_ring, d_prefill, d_slots, batch, window, heads, out, ws, mass=None, stream=None):
+    """Decode attention with modified scores; `mass` also accumulates the attention weights."""
+    check(lib().uocr_b200_rswa_attention_scored_batch_paged(
+        layer.ref(), C.byref(score.desc), _p(q), _dtype_of(q), _p(d_len), _p(d_ring), _p(d_prefill), _p(d_slots), batch, window, heads,
+        _p(out), C.byref(mass.desc) if mass is not None else None, ws.h, stream_handle(stream)))
+
+
+def attention_scored_ragged_paged(layer, score, q, d_prefill, d_slots, d_pos, total, heads, out, ws, stream=None):
+    """Packed vision rows with modified scores, any geometry."""
+    check(lib().uocr_b200_rswa_attention_scored_ragged_paged(layer.ref(), C.byref(score.desc), _p(q), _dtype_of(q), _p(d_prefill), _p(d_slots),
+                                                             _p(d_pos), total, heads, _p(out), ws.h, stream_handle(stream)))
+
+
+def prefill_text_scored_paged(layer, text_k, text_v, text_blocks, score, q, d_prefill, d_slots, d_pos, d_block0, total, window, heads, out, ws,
+                              stream=None):
+    """Packed text rows over prefix + text window with modified scores, any geometry (K and V already in the text pool)."""
+    check(lib().uocr_b200_rswa_prefill_text_scored_paged(layer.ref(), _p(text_k), _p(text_v), text_blocks, C.byref(score.desc), _p(q),
+                                                         _dtype_of(q), _p(d_prefill), _p(d_slots), _p(d_pos), _p(d_block0), total, window,
+                                                         heads, _p(out), ws.h, stream_handle(stream)))

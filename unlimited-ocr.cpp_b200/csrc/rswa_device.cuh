@@ -2,6 +2,7 @@
 // bf16 conversion on raw bits, and the per-geometry lane mapping used by the attention kernels.
 #pragma once
 
+#include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
 
@@ -107,6 +108,12 @@ __device__ __forceinline__ uint32_t f32_to_bf16_bits(float f) {
 
 __device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
     return f32_to_bf16_bits(lo) | (f32_to_bf16_bits(hi) << 16);
+}
+
+// The same rounding by the conversion instruction, which keeps a NaN a NaN.
+__device__ __forceinline__ uint32_t rn_bf16x2(float lo, float hi) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
 }
 
 // Widening a bf16 pair held in one 32-bit word: one byte permute per element (the low half needs its

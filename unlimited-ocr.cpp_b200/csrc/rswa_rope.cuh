@@ -15,8 +15,6 @@
 // every element is read and written by one thread, so a call may work in place.
 #pragma once
 
-#include <cuda_bf16.h>
-
 #include "rswa_paged.cuh"
 
 namespace uocr_b200 {
@@ -86,11 +84,6 @@ __device__ __forceinline__ void load8(const void* base, long long at, float (&f)
         f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w;
         f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
     }
-}
-
-__device__ __forceinline__ uint32_t rn_bf16x2(float lo, float hi) {
-    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&v);
 }
 
 template <typename T>

@@ -1,0 +1,674 @@
+// Split-KV attention with modified scores over the paged R-SWA cache: a tanh cap, a bias that grows with
+// the distance, and a visible range of the fixed region per row (pages, documents, prefixes).
+//
+//   x = scale * q.k;   x <- cap * tanh(x / cap);   x <- x - slope_h * |pos_q - pos_k|;   softmax over the
+//   visible keys;   out = sum of the weights times v, 0 for a row that sees nothing.
+//
+// The work model is that of the plain attention kernel: the 16-token tiles a row's heads can see are laid
+// out on one line and cut into equal pieces, one per warp of a persistent grid, so a batch of one long
+// sequence and a batch of many short ones load the SMs alike; a warp streams its piece's K and V tiles
+// through a private ring of shared memory with bulk copies, and the last warp to finish an item that
+// straddles pieces joins the partial results (maximum, sum, accumulator).  What differs:
+//   - an item is a row and up to four query heads of one KV head (G), so grouped heads read a tile once;
+//   - only tiles that hold a visible token are on the line: the cost of a page is the page;
+//   - the line is planned by every CTA in its own shared memory when the rows fit (one launch), else by
+//     rswa_scored_plan_kernel;
+//   - scores are modified one token per lane pair, after the reduction of the dot products, so the cap's
+//     tanh costs one call per token and head, not per element;
+//   - with attention weights asked for, the modified scores of the fixed region go to scratch (4 bytes per
+//     token and head, against 2 * head_dim * 2 bytes of K and V) and rswa_mass_kernel turns them into
+//     weights once the row's maximum and sum are known -- in a fixed order, without atomics.
+// Statistics, scores and accumulators are fp32; keys and values outside the visible range are never
+// multiplied, whatever they hold.  Bound by HBM.
+#pragma once
+
+#include "rswa_paged.cuh"
+#include "rswa_split.cuh"
+
+namespace uocr_b200 {
+
+enum ScoreMode : int { kScoreDecode = 0, kScoreRagged = 1, kScoreText = 2 };
+
+// What one row attends: tokens [lo, hi) of the fixed region, then `ring` tokens of its ring (table entries
+// from ring_entry) or of the text pool (from block text >> 4, the first text & 15 tokens of it skipped).
+struct ScoreRow {
+    int slot, lo, hi;
+    int ring_entry;
+    int ring;
+    int text;  // -1: ring
+    int age0;  // distance of token 0 of the first ring / text block; the distance of token t is age0 - t (+ window if negative)
+    int q_pos;
+};
+static_assert(sizeof(ScoreRow) == 32, "the workspace reserves 32 bytes a row");
+
+struct ScorePlan {
+    int mode, rows, items_per_row, window;
+    const int* d_slots;
+    const int* d_len;
+    const int* d_ring_pos;
+    const int* d_prefill_len;
+    const int* d_pos;
+    const int* d_text_block0;
+    const int* d_lo;
+    const int* d_hi;
+    const int* d_q_pos;
+    uint32_t* out;  // rows without a visible key are zero-filled here
+    int out_row_words;
+};
+
+struct ScoreParams {
+    ScorePlan plan;
+    const void* q;
+    int q_bf16;
+    void* out;
+    int out_bf16;
+    const uint8_t* k_base;
+    const uint8_t* v_base;
+    const uint8_t* k_text;
+    const uint8_t* v_text;
+    int text_blocks;
+    const int32_t* table;
+    int table_stride, num_blocks;
+    int rows, heads, kv_heads, group;
+    float q_scale;   // what q is multiplied by: scale / cap with a cap, scale * log2(e) without
+    float cap_log2;  // cap * log2(e); 0: none
+    const float* slopes;
+    const int* d_key_pos;
+    int key_pos_stride;
+    float* scores;  // attention weights asked for: [rows * heads][score_stride] modified scores (log2 domain), then [rows * heads][2] (max, 1 / sum)
+    float* score_ml;
+    int score_stride;
+    ScoreRow* info;  // plan in global memory (rows beyond kScoreSharedRows)
+    long long* rs;
+    float* part_acc;  // [2 * pieces][G * head_dim]
+    float* part_ml;   // [2 * pieces][2 G]
+    int* counters;
+    int* status;
+    uint32_t wait_limit;
+    int total_warps;
+};
+
+constexpr int kScoreSharedRows = 512;  // rows a CTA plans in its own shared memory
+
+// Clamped visible range of row r in a fixed region whose first `fixed` tokens are in the cache.
+__device__ __forceinline__ void score_range(const int* d_lo, const int* d_hi, int r, int fixed, int def_hi, int& lo, int& hi) {
+    hi = min(d_hi ? __ldg(d_hi + r) : def_hi, fixed);
+    lo = max(d_lo ? __ldg(d_lo + r) : 0, 0);
+    if (hi <= lo) lo = hi = 0;
+}
+
+__device__ __forceinline__ int score_plan_row(const ScorePlan& p, int r, ScoreRow& o) {
+    const int slot = __ldg(p.d_slots + r);
+    const int pfx = max(__ldg(p.d_prefill_len + slot), 0);
+    o.slot = slot;
+    o.ring_entry = (pfx + kBlockTokens - 1) / kBlockTokens;
+    o.ring = 0;
+    o.text = -1;
+    o.age0 = 0;
+    o.q_pos = 0;
+    int skip = 0;
+    if (p.mode == kScoreDecode) {
+        const int len = max(__ldg(p.d_len + slot), 0);
+        score_range(p.d_lo, p.d_hi, r, min(len, pfx), pfx, o.lo, o.hi);
+        o.ring = min(max(len - pfx, 0), p.window);
+        if (p.d_q_pos) o.q_pos = __ldg(p.d_q_pos + r);
+        // the newest ring token: the last one written before the window filled, the one behind the cursor after
+        const int cursor = __ldg(p.d_ring_pos + slot);
+        o.age0 = o.ring < p.window ? o.ring - 1 : (cursor > 0 ? cursor : p.window) - 1;
+    } else if (p.mode == kScoreRagged) {
+        const int pos = __ldg(p.d_pos + r);
+        score_range(p.d_lo, p.d_hi, r, pfx, pos + 1, o.lo, o.hi);
+        o.q_pos = p.d_q_pos ? __ldg(p.d_q_pos + r) : pos;
+    } else {
+        const int pos = __ldg(p.d_pos + r);
+        score_range(p.d_lo, p.d_hi, r, pfx, pfx, o.lo, o.hi);
+        const int first = max(0, pos - p.window + 1);
+        skip = first & (kBlockTokens - 1);
+        o.ring = max(pos - first + 1, 0);
+        o.text = ((__ldg(p.d_text_block0 + r) + first / kBlockTokens) << 4) | skip;
+        o.age0 = pos - (first - skip);
+        if (p.d_q_pos) o.q_pos = __ldg(p.d_q_pos + r);
+    }
+    const int fixed_tiles = o.hi > o.lo ? (o.hi + kBlockTokens - 1) / kBlockTokens - o.lo / kBlockTokens : 0;
+    const int ring_tiles = o.ring > 0 ? (skip + o.ring + kBlockTokens - 1) / kBlockTokens : 0;
+    return fixed_tiles + ring_tiles;
+}
+
+// Block-wide: info[0..rows) and the prefix sum of the rows' units (rs[0..rows]).  `scratch`: 33 long longs of shared memory.
+__device__ __forceinline__ void score_plan_rows(const ScorePlan& p, ScoreRow* info, long long* rs, long long* scratch, bool zero_rows) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nthreads = blockDim.x;
+    long long carry = 0;
+    for (int base = 0; base < p.rows; base += nthreads) {
+        const int r = base + tid;
+        long long units = 0;
+        if (r < p.rows) {
+            ScoreRow o;
+            units = (long long)score_plan_row(p, r, o) * p.items_per_row;
+            info[r] = o;
+            if (units == 0 && zero_rows)
+                for (int i = 0; i < p.out_row_words; ++i) p.out[(size_t)r * p.out_row_words + i] = 0u;
+        }
+        long long incl = units;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const long long t = __shfl_up_sync(0xffffffffu, incl, d);
+            if (lane >= d) incl += t;
+        }
+        if (lane == 31) scratch[warp] = incl;
+        __syncthreads();
+        long long before = carry;
+        for (int w = 0; w < warp; ++w) before += scratch[w];
+        if (r < p.rows) rs[r] = before + incl - units;
+        long long all = 0;
+        for (int w = 0; w < (nthreads >> 5); ++w) all += scratch[w];
+        carry += all;
+        __syncthreads();
+    }
+    if (tid == 0) rs[p.rows] = carry;
+}
+
+__global__ void __launch_bounds__(1024) rswa_scored_plan_kernel(ScorePlan p, ScoreRow* info, long long* rs) {
+    __shared__ long long scratch[33];
+    score_plan_rows(p, info, rs, scratch, true);
+}
+
+// Descriptor bits of a unit (one 16-token tile of an item).
+constexpr uint32_t kSuValid = 0x1f;        // bits 0-4: tokens [skip, valid) are visible
+constexpr int kSuSkipShift = 5;            // bits 5-8
+constexpr uint32_t kSuLast = 1u << 9;
+constexpr uint32_t kSuFirst = 1u << 10;
+constexpr uint32_t kSuFixed = 1u << 11;    // tile of the fixed region
+constexpr uint32_t kSuText = 1u << 12;     // tile of the text pool
+
+constexpr int kScoreRing = 2;              // tile slots per warp
+constexpr int kScoreThreads = 512;
+
+template <typename KV, int HD, int G>
+__global__ void __launch_bounds__(kScoreThreads, 1) rswa_scored_kernel(const __grid_constant__ ScoreParams p) {
+    using M = TileMap<KV, HD>;
+    constexpr int LPR = M::kLanesPerRow, CPL = M::kChunksPerLane, RPW = M::kRowsPerLoad;
+    constexpr int ITER = M::kIters, EPC = KV::kPerChunk, EPL = M::kElemsPerLane;
+    constexpr int PPC = EPC / 2, PPL = EPL / 2;
+    constexpr int ROWB = M::kRowBytes, TILE = M::kTileBytes;
+    constexpr unsigned FULL = 0xffffffffu;
+
+    extern __shared__ __align__(128) uint8_t smem[];
+    const int warps = blockDim.x >> 5;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int bar_bytes = (warps * kScoreRing * 8 + 127) & ~127;
+    uint8_t* my_tiles = smem + bar_bytes + (size_t)warp * (kScoreRing * TILE);
+    const uint32_t bar0 = smem_addr(smem) + warp * (kScoreRing * 8);
+    const uint32_t tile0 = smem_addr(my_tiles);
+    if (lane == 0) {
+#pragma unroll
+        for (int s = 0; s < kScoreRing; ++s) mbar_init(bar0 + 8 * s, 1);
+        mbar_init_fence();
+    }
+    __syncwarp();
+
+    // ---- the plan -------------------------------------------------------------------------------------
+    const ScoreRow* info = p.info;
+    const long long* rs = p.rs;
+    if (p.rows <= kScoreSharedRows) {
+        uint8_t* plan_base = smem + bar_bytes + (size_t)warps * (kScoreRing * TILE);
+        ScoreRow* info_s = reinterpret_cast<ScoreRow*>(plan_base);
+        long long* rs_s = reinterpret_cast<long long*>(plan_base + sizeof(ScoreRow) * p.rows);
+        score_plan_rows(p.plan, info_s, rs_s, rs_s + p.rows + 1, blockIdx.x == 0);
+        __syncthreads();
+        info = info_s;
+        rs = rs_s;
+    }
+    const int items_per_row = p.plan.items_per_row;
+    const long long total = rs[p.rows];
+    if (total == 0) return;
+    const PieceMap pm = make_piece_map(total, p.total_warps, warps);
+    // fewer pieces than warps are spread over the SMs
+    const int gw = (int)blockIdx.x * warps + warp;
+    const int gw_spread = warp * (int)gridDim.x + (int)blockIdx.x;
+    const int piece = pm.ns == p.total_warps ? gw : (gw_spread < pm.ns ? gw_spread : -1);
+    if (piece < 0) return;
+    const long long u0 = pm.start(piece);
+    const long long n_units = pm.end(piece) - u0;
+
+    const int g = lane % LPR;   // chunk position inside the row
+    const int rg = lane / LPR;  // which of the RPW rows of a warp-wide load
+    const int my_tok = (LPR >= 2 ? (g >> 1) * RPW : 0) + rg;  // the token whose score this lane ends up with
+    const bool one_of_pair = LPR < 2 || (g & 1) == 0;
+
+    // ---- unit descriptors: lane l describes unit desc_base + l of this piece ----------------------------
+    uint32_t d_tile = 0, d_meta = 0, d_item = 0;
+    int d_tok = 0;  // fixed region: index of the tile's token 0; ring / text: its distance from the query
+    long long desc_base = 0;
+    auto build_desc = [&](long long base) {
+        desc_base = base;
+        d_tile = d_meta = d_item = 0;
+        d_tok = 0;
+        if (base + lane < n_units) {
+            const long long u = u0 + base + lane;
+            int lo = 0, hi = p.rows;  // rs[lo] <= u < rs[hi]
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) >> 1;
+                if (rs[mid] <= u) lo = mid; else hi = mid;
+            }
+            const ScoreRow o = info[lo];
+            const int per_item = (int)((rs[lo + 1] - rs[lo]) / items_per_row);
+            const long long rem = u - rs[lo];
+            const int it = (int)(rem / per_item), j = (int)(rem - (long long)it * per_item);
+            const int kvh = it * G / p.group;
+            const int first = o.lo / kBlockTokens;
+            const int fixed_tiles = o.hi > o.lo ? (o.hi + kBlockTokens - 1) / kBlockTokens - first : 0;
+            uint32_t m = 0;
+            int valid, skip = 0, blk = -1;
+            if (j < fixed_tiles) {
+                const int s0 = (first + j) * kBlockTokens;
+                valid = min(kBlockTokens, o.hi - s0);
+                skip = max(o.lo - s0, 0);
+                d_tok = s0;
+                m |= kSuFixed;
+                if (first + j < p.table_stride) blk = __ldg(p.table + (size_t)o.slot * p.table_stride + first + j);
+                else atomicOr(p.status, kStatusBadSlot);
+            } else {
+                const int jr = j - fixed_tiles;
+                const int lead = o.text >= 0 ? o.text & 15 : 0;
+                valid = min(kBlockTokens, lead + o.ring - jr * kBlockTokens);
+                skip = jr == 0 ? lead : 0;
+                d_tok = o.age0 - jr * kBlockTokens;
+                if (o.text >= 0) {
+                    blk = (o.text >> 4) + jr;
+                    m |= kSuText;
+                } else if (o.ring_entry + jr < p.table_stride) {
+                    blk = __ldg(p.table + (size_t)o.slot * p.table_stride + o.ring_entry + jr);
+                } else {
+                    atomicOr(p.status, kStatusBadSlot);
+                }
+            }
+            if (blk < 0 || blk >= ((m & kSuText) ? p.text_blocks : p.num_blocks)) {
+                atomicOr(p.status, kStatusBadBlock);
+                blk = 0;
+            }
+            d_tile = (uint32_t)blk * p.kv_heads + kvh;
+            if (j == per_item - 1) m |= kSuLast;
+            if (j == 0) m |= kSuFirst;
+            d_meta = m | (uint32_t)valid | ((uint32_t)skip << kSuSkipShift);
+            d_item = (uint32_t)lo * (uint32_t)items_per_row + (uint32_t)it;
+        }
+    };
+
+    // ---- producer: tiles K(0) V(0) K(1) V(1) ... rotate through the slots ------------------------------
+    const uint64_t pol_stream = l2_policy_evict_first(), pol_keep = l2_policy_evict_last();
+    int issue_slot = 0, use_slot = 0;
+    long long issue_seq = 0, consumed = 0;
+    uint32_t phases = 0;
+    auto issue_next = [&]() {
+        if (issue_seq >= 2 * n_units) return;
+        const int src = (int)((issue_seq >> 1) - desc_base);
+        const bool is_v = (issue_seq & 1) != 0;
+        const uint32_t tile = __shfl_sync(FULL, d_tile, src);
+        const uint32_t meta = __shfl_sync(FULL, d_meta, src);
+        if (lane == 0) {
+            const uint32_t bar = bar0 + 8 * issue_slot;
+            const uint8_t* base = (meta & kSuText) ? (is_v ? p.v_text : p.k_text) : (is_v ? p.v_base : p.k_base);
+            mbar_arrive_expect_tx(bar, TILE);
+            // ring tiles are read once per launch; tiles of the fixed region again by whoever shares the prefix
+            bulk_copy_g2s_hint(tile0 + issue_slot * TILE, base + (size_t)tile * TILE, TILE, bar, (meta & kSuFixed) ? pol_keep : pol_stream);
+        }
+        issue_slot = issue_slot == kScoreRing - 1 ? 0 : issue_slot + 1;
+        ++issue_seq;
+    };
+    auto wait_tile = [&]() -> uint8_t* {
+        if (!mbar_wait_bounded(bar0 + 8 * use_slot, (phases >> use_slot) & 1u, p.status, p.wait_limit)) return nullptr;
+        uint8_t* t = my_tiles + use_slot * TILE;
+        phases ^= 1u << use_slot;
+        use_slot = use_slot == kScoreRing - 1 ? 0 : use_slot + 1;
+        ++consumed;
+        return t;
+    };
+
+    // ---- the item under way ------------------------------------------------------------------------------
+    float2 q2[G][PPL], acc2[G][PPL];
+    float m_run[G], l_run[G], slope[G];
+    int cur_slot = 0, cur_q_pos = 0;
+    auto load_item = [&](uint32_t item) {
+        const size_t at = (size_t)item * (G * HD);  // items_per_row * G == heads
+#pragma unroll
+        for (int i = 0; i < G; ++i) {
+#pragma unroll
+            for (int cp = 0; cp < CPL; ++cp) {
+                const int d0 = (g + 32 * cp) * EPC;
+#pragma unroll
+                for (int e = 0; e < EPC; e += 4) {
+                    float4 t;
+                    if (p.q_bf16) {
+                        const uint2 w = __ldg(reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p.q) + at + i * HD + d0 + e));
+                        t = make_float4(bf16_lo(w.x), bf16_hi(w.x), bf16_lo(w.y), bf16_hi(w.y));
+                    } else {
+                        t = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(p.q) + at + i * HD + d0 + e));
+                    }
+                    q2[i][(cp * EPC + e) / 2] = make_float2(t.x * p.q_scale, t.y * p.q_scale);
+                    q2[i][(cp * EPC + e) / 2 + 1] = make_float2(t.z * p.q_scale, t.w * p.q_scale);
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < PPL; ++e) acc2[i][e] = make_float2(0.f, 0.f);
+            m_run[i] = -INFINITY;
+            l_run[i] = 0.f;
+        }
+        const int r = (int)(item / (uint32_t)items_per_row);
+        if (p.slopes) {
+            const int h0 = (int)(item - (uint32_t)r * (uint32_t)items_per_row) * G;
+#pragma unroll
+            for (int i = 0; i < G; ++i) slope[i] = __ldg(p.slopes + h0 + i) * 1.4426950408889634f;
+            cur_slot = info[r].slot;
+            cur_q_pos = info[r].q_pos;
+        }
+    };
+    auto store_out = [&](size_t at, float a, float b, float c, float d) {
+        if (p.out_bf16) *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + at) = make_uint2(rn_bf16x2(a, b), rn_bf16x2(c, d));
+        else *reinterpret_cast<float4*>(static_cast<float*>(p.out) + at) = make_float4(a, b, c, d);
+    };
+
+    uint32_t pend[2];  // items this piece left a partial of: the first and the last
+    int pend_n = 0;
+
+    build_desc(0);
+#pragma unroll
+    for (int s = 0; s < kScoreRing; ++s) issue_next();
+    uint32_t cur_item = __shfl_sync(FULL, d_item, 0);
+    load_item(cur_item);
+    bool first_segment = true, gave_up = false;
+    bool from_start = (__shfl_sync(FULL, d_meta, 0) & kSuFirst) != 0;
+
+    for (long long it = 0; it < n_units; ++it) {
+        if (it - desc_base >= 32 - 2) build_desc(it);  // the producer looks two units ahead
+        const uint32_t meta = __shfl_sync(FULL, d_meta, (int)(it - desc_base));
+        const int tok0 = __shfl_sync(FULL, d_tok, (int)(it - desc_base));
+        const int nvalid = (int)(meta & kSuValid), nskip = (int)((meta >> kSuSkipShift) & 15);
+
+        // ---- scores of the tile's 16 tokens -------------------------------------------------------------
+        const uint8_t* ktile = wait_tile();
+        if (!ktile) { gave_up = true; break; }
+        float sc[G][ITER];
+#pragma unroll
+        for (int i = 0; i < ITER; ++i) {
+            const int t = (i * RPW + rg) & (kBlockTokens - 1);
+            float2 d2[G];
+#pragma unroll
+            for (int h = 0; h < G; ++h) d2[h] = make_float2(0.f, 0.f);
+#pragma unroll
+            for (int cp = 0; cp < CPL; ++cp) {
+                const uint4 w = *reinterpret_cast<const uint4*>(ktile + t * ROWB + (g + 32 * cp) * 16);
+                float2 f[PPC];
+                unpack2<KV>(w, f);
+#pragma unroll
+                for (int h = 0; h < G; ++h)
+#pragma unroll
+                    for (int e = 0; e < PPC; ++e) d2[h] = fma2(q2[h][cp * PPC + e], f[e], d2[h]);
+            }
+#pragma unroll
+            for (int h = 0; h < G; ++h) sc[h][i] = d2[h].x + d2[h].y;
+        }
+        __syncwarp();
+        issue_next();  // the K slot is free
+
+        const bool visible = my_tok >= nskip && my_tok < nvalid;
+        float dist = 0.f;
+        if (p.slopes) {
+            int a;
+            if (meta & kSuFixed) {
+                int at = tok0 + my_tok;
+                if (p.d_key_pos && visible && at < p.key_pos_stride) at = __ldg(p.d_key_pos + (size_t)cur_slot * p.key_pos_stride + at);
+                dist = __uint2float_rn((uint32_t)max(cur_q_pos, at) - (uint32_t)min(cur_q_pos, at));
+            } else {
+                a = tok0 - my_tok;
+                if (a < 0) a += p.plan.window;
+                dist = (float)a;
+            }
+        }
+        float pr[G];
+#pragma unroll
+        for (int h = 0; h < G; ++h) {
+            RowReduce<ITER, LPR / 2>::run(sc[h], lane);
+            float x = sc[h][0];
+            if (p.cap_log2 > 0.f) x = p.cap_log2 * tanhf(x);
+            if (p.slopes) x = fmaf(-slope[h], dist, x);
+            if (p.scores && (meta & kSuFixed) && visible && one_of_pair && tok0 + my_tok < p.score_stride)
+                __stcs(p.scores + ((size_t)cur_item * G + h) * p.score_stride + tok0 + my_tok, x);
+            x = visible ? x : -INFINITY;
+            // ---- online softmax, one running maximum per row group -----------------------------------------
+            float mt = x;
+#pragma unroll
+            for (int d = LPR / 2; d >= 2; d >>= 1) mt = fmaxf(mt, __shfl_xor_sync(FULL, mt, d));
+            const float m_new = fmaxf(m_run[h], mt);
+            const float m_safe = (m_new == -INFINITY) ? 0.f : m_new;
+            const float alpha = fast_exp2(m_run[h] - m_safe);
+            pr[h] = fast_exp2(x - m_safe);
+            l_run[h] = l_run[h] * alpha + pr[h];
+            m_run[h] = m_new;
+            const float2 alpha2 = make_float2(alpha, alpha);
+#pragma unroll
+            for (int e = 0; e < PPL; ++e) acc2[h][e] = mul2(acc2[h][e], alpha2);
+        }
+
+        // ---- acc += p . v ------------------------------------------------------------------------------------
+        const uint8_t* vtile = wait_tile();
+        if (!vtile) { gave_up = true; break; }
+        const bool all = nvalid == kBlockTokens && nskip == 0;
+#pragma unroll
+        for (int i = 0; i < ITER; ++i) {
+            const int t = i * RPW + rg;
+            float2 pi2[G];
+#pragma unroll
+            for (int h = 0; h < G; ++h) {
+                const float pi = (LPR >= 2) ? __shfl_sync(FULL, pr[h], rg * LPR + 2 * i) : pr[h];
+                pi2[h] = make_float2(pi, pi);
+            }
+            if (all ? (RPW <= kBlockTokens || t < kBlockTokens) : (t >= nskip && t < nvalid)) {  // rows outside may hold anything
+#pragma unroll
+                for (int cp = 0; cp < CPL; ++cp) {
+                    const uint4 w = *reinterpret_cast<const uint4*>(vtile + t * ROWB + (g + 32 * cp) * 16);
+                    float2 f[PPC];
+                    unpack2<KV>(w, f);
+#pragma unroll
+                    for (int h = 0; h < G; ++h)
+#pragma unroll
+                        for (int e = 0; e < PPC; ++e) acc2[h][cp * PPC + e] = fma2(pi2[h], f[e], acc2[h][cp * PPC + e]);
+                }
+            }
+        }
+        __syncwarp();
+        issue_next();  // the V slot is free
+
+        // ---- end of an item or of the piece ---------------------------------------------------------------
+        const bool item_done = (meta & kSuLast) != 0, piece_done = it == n_units - 1;
+        if (item_done || piece_done) {
+            const bool whole = item_done && from_start;
+            const int my_slot = 2 * piece + (first_segment ? 0 : 1);
+#pragma unroll
+            for (int h = 0; h < G; ++h) {
+                float mx = m_run[h];
+#pragma unroll
+                for (int d = LPR; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(FULL, mx, d));
+                const float mx_safe = (mx == -INFINITY) ? 0.f : mx;
+                const float wgt = fast_exp2(m_run[h] - mx_safe);
+                float lsum = l_run[h] * wgt;
+#pragma unroll
+                for (int d = 16; d >= 1; d >>= 1) lsum += __shfl_xor_sync(FULL, lsum, d);
+                if (LPR >= 2) lsum *= 0.5f;  // the two lanes of a pair carry the same token
+                float acc[EPL];
+#pragma unroll
+                for (int e = 0; e < PPL; ++e) {
+                    acc[2 * e] = acc2[h][e].x * wgt;
+                    acc[2 * e + 1] = acc2[h][e].y * wgt;
+                }
+#pragma unroll
+                for (int e = 0; e < EPL; ++e)
+#pragma unroll
+                    for (int d = LPR; d < 32; d <<= 1) acc[e] += __shfl_xor_sync(FULL, acc[e], d);
+                const float inv = lsum == 0.f ? 0.f : 1.f / lsum;
+                if (lane < LPR) {
+                    float* dst = p.part_acc + (size_t)my_slot * (G * HD) + h * HD;
+#pragma unroll
+                    for (int cp = 0; cp < CPL; ++cp)
+#pragma unroll
+                        for (int e = 0; e < EPC; e += 4) {
+                            const int d0 = (g + 32 * cp) * EPC + e;
+                            const float* a = acc + cp * EPC + e;
+                            if (whole) store_out((size_t)cur_item * (G * HD) + h * HD + d0, a[0] * inv, a[1] * inv, a[2] * inv, a[3] * inv);
+                            else __stcg(reinterpret_cast<float4*>(dst + d0), make_float4(a[0], a[1], a[2], a[3]));
+                        }
+                }
+                if (lane == 0) {
+                    if (whole) {
+                        if (p.scores) *reinterpret_cast<float2*>(p.score_ml + 2 * ((size_t)cur_item * G + h)) = make_float2(mx_safe, inv);
+                    } else {
+                        __stcg(reinterpret_cast<float2*>(p.part_ml + (size_t)my_slot * (2 * G) + 2 * h), make_float2(mx, lsum));
+                    }
+                }
+            }
+            if (!whole) pend[pend_n++ & 1] = cur_item;
+            first_segment = false;
+            if (!piece_done) {
+                cur_item = __shfl_sync(FULL, d_item, (int)(it + 1 - desc_base));
+                from_start = true;
+                load_item(cur_item);
+            }
+        }
+    }
+    if (gave_up) {
+        // A wait ran out (the status word says so and the launch's results are void).  Tiles issued and not yet consumed
+        // may still be on their way into this warp's slots: see them land before the CTA exits.  Full limit.
+        for (; consumed < issue_seq; ++consumed) {
+            mbar_wait_bounded(bar0 + 8 * use_slot, (phases >> use_slot) & 1u, nullptr);
+            phases ^= 1u << use_slot;
+            use_slot = use_slot == kScoreRing - 1 ? 0 : use_slot + 1;
+        }
+        return;
+    }
+
+    // ---- arrivals: whoever completes an item's set of partials joins them ------------------------------------
+    __syncwarp();  // the partial stores of every lane come before the arriving lane's release
+    for (int k = 0; k < pend_n; ++k) {
+        const uint32_t item = pend[k];
+        const int r = (int)(item / (uint32_t)items_per_row);
+        const int n = (int)((rs[r + 1] - rs[r]) / items_per_row);
+        const long long s0 = rs[r] + (long long)(item - (uint32_t)r * (uint32_t)items_per_row) * n;
+        const int wf = pm.of(s0), wl = pm.of(s0 + n - 1);
+        int old = 0;
+        if (lane == 0)  // release: this warp's partials (ordered before by the barrier above); acquire: the others'
+            asm volatile("atom.add.acq_rel.gpu.global.s32 %0, [%1], 1;" : "=r"(old) : "l"(p.counters + wf) : "memory");
+        old = __shfl_sync(FULL, old, 0);
+        if (old != wl - wf) continue;
+        const int n_part = wl - wf + 1;
+        const bool wf_second = pm.start(wf) < s0;  // the item is piece wf's second segment
+        auto slot_of = [&](int i) { return (size_t)(2 * (wf + i) + ((i == 0 && wf_second) ? 1 : 0)); };
+        constexpr int NK = (HD + 31) / 32, kBatch = NK > 4 ? 4 : 8;
+#pragma unroll 1
+        for (int h = 0; h < G; ++h) {
+            // The accumulators come in batches whose loads are all issued before any is used, the first together with
+            // the (max, sum) loads: a join costs about one round trip to L2 per batch.
+            float tmp[kBatch][NK], o[NK];
+            auto load_batch = [&](int b0) {
+#pragma unroll
+                for (int i = 0; i < kBatch; ++i) {
+                    const float* pa = p.part_acc + slot_of(b0 + i) * (G * HD) + h * HD;
+#pragma unroll
+                    for (int kk = 0; kk < NK; ++kk) {
+                        const int d = lane + 32 * kk;
+                        tmp[i][kk] = (b0 + i < n_part && d < HD) ? __ldcg(pa + d) : 0.f;
+                    }
+                }
+            };
+            load_batch(0);
+            float mall = -INFINITY, lall = 0.f;
+            for (int w0 = lane; w0 < n_part; w0 += 32) mall = fmaxf(mall, __ldcg(p.part_ml + slot_of(w0) * (2 * G) + 2 * h));
+#pragma unroll
+            for (int d = 16; d >= 1; d >>= 1) mall = fmaxf(mall, __shfl_xor_sync(FULL, mall, d));
+            const float m_safe = (mall == -INFINITY) ? 0.f : mall;
+#pragma unroll
+            for (int kk = 0; kk < NK; ++kk) o[kk] = 0.f;
+            float wg = 0.f;
+            for (int b0 = 0; b0 < n_part; b0 += kBatch) {
+                if ((b0 & 31) == 0) {
+                    wg = 0.f;
+                    if (b0 + lane < n_part) {
+                        const float2 ml = __ldcg(reinterpret_cast<const float2*>(p.part_ml + slot_of(b0 + lane) * (2 * G) + 2 * h));
+                        wg = fast_exp2(ml.x - m_safe);
+                        lall += ml.y * wg;
+                    }
+                }
+                if (b0) load_batch(b0);
+#pragma unroll
+                for (int i = 0; i < kBatch; ++i) {
+                    const float wi = __shfl_sync(FULL, wg, (b0 + i) & 31);
+#pragma unroll
+                    for (int kk = 0; kk < NK; ++kk) o[kk] = fmaf(tmp[i][kk], wi, o[kk]);
+                }
+            }
+#pragma unroll
+            for (int d = 16; d >= 1; d >>= 1) lall += __shfl_xor_sync(FULL, lall, d);
+            const float inv = lall == 0.f ? 0.f : 1.f / lall;
+#pragma unroll
+            for (int kk = 0; kk < NK; ++kk) {
+                const int d = lane + 32 * kk;
+                if (d < HD) {
+                    const size_t at = (size_t)item * (G * HD) + h * HD + d;
+                    if (p.out_bf16) static_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(o[kk] * inv);
+                    else static_cast<float*>(p.out)[at] = o[kk] * inv;
+                }
+            }
+            if (p.scores && lane == 0) *reinterpret_cast<float2*>(p.score_ml + 2 * ((size_t)item * G + h)) = make_float2(m_safe, inv);
+        }
+        if (lane == 0) p.counters[wf] = 0;  // for the next launch
+    }
+}
+
+// -------------------------------------------------------------------------------------------------
+// attention weights: mass_out[slot][s] = decay * mass_in[slot][s] + sum over the slot's rows and heads of the weight of
+// token s of the fixed region.  One thread per token adds its rows and heads in order; a slot named by several rows is
+// handled by its first row's CTAs.
+// -------------------------------------------------------------------------------------------------
+struct MassParams {
+    ScorePlan plan;
+    int heads;
+    const float* scores;
+    const float* score_ml;
+    const float* mass_in;
+    float* mass_out;
+    int stride;
+    float decay;
+    int* status;
+};
+
+constexpr int kMassThreads = 256;
+
+__global__ void __launch_bounds__(kMassThreads) rswa_mass_kernel(const __grid_constant__ MassParams p) {
+    const int b = blockIdx.y, tid = threadIdx.x;
+    const int slot = __ldg(p.plan.d_slots + b);
+    bool earlier = false;
+    for (int j = tid; j < b; j += kMassThreads) earlier |= __ldg(p.plan.d_slots + j) == slot;
+    if (__syncthreads_or(earlier)) return;
+    const int pfx = max(__ldg(p.plan.d_prefill_len + slot), 0);
+    const int n = min(pfx, p.stride);
+    if (pfx > p.stride && tid == 0 && blockIdx.x == 0) atomicOr(p.status, kStatusBadSlot);
+    const int s = blockIdx.x * kMassThreads + tid;
+    if ((int)blockIdx.x * kMassThreads >= n) return;
+    const size_t at = (size_t)slot * p.stride + s;
+    float sum = (s < n && p.mass_in && p.decay != 0.f) ? p.decay * p.mass_in[at] : 0.f;
+    const int fixed = min(max(__ldg(p.plan.d_len + slot), 0), pfx);
+    for (int r = b; r < p.plan.rows; ++r) {
+        if (__ldg(p.plan.d_slots + r) != slot) continue;
+        int lo, hi;
+        score_range(p.plan.d_lo, p.plan.d_hi, r, fixed, pfx, lo, hi);
+        if (s < lo || s >= hi || s >= n) continue;
+        const float* sc = p.scores + (size_t)r * p.heads * p.stride + s;
+        const float2* ml = reinterpret_cast<const float2*>(p.score_ml) + (size_t)r * p.heads;
+#pragma unroll 4
+        for (int h = 0; h < p.heads; ++h) {
+            const float2 w = __ldg(ml + h);
+            sum += fast_exp2(__ldcs(sc + (size_t)h * p.stride) - w.x) * w.y;
+        }
+    }
+    if (s < n) p.mass_out[at] = sum;
+}
+
+}  // namespace uocr_b200
