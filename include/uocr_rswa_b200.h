@@ -565,6 +565,48 @@ UOCR_B200_API int uocr_b200_rswa_prefill_text_scored_paged(
     const int* d_pos, const int* d_text_block0, int total, int window, int heads, void* out, uocr_b200_workspace* ws,
     uocr_b200_stream_t stream);
 
+/* ================================================================================================
+ * Eviction from the fixed region by accumulated attention weight (no reference counterpart; the
+ * reference keeps every vision token for good).  A step of an evicting engine: choose with
+ * uocr_b200_rswa_evict_select what uocr_b200_mass has accumulated, move the rows of all layers, publish.
+ * The ring is not touched: it drops its tokens by age.  The three calls are ordinary launches on one
+ * stream and need no synchronisation in between.
+ * ============================================================================================= */
+
+/* For each of the n slots the `keep` tokens of its fixed region with the largest mass, as an ascending
+ * list in d_keep[i][0 .. count), -1 up to `keep`; count = min(keep, region) goes to d_keep_len[i].  The first
+ * `sinks` and the last `recent` tokens count as infinitely heavy; NaN counts as lighter than
+ * everything; ties go to the lowest index.  A region longer than mass_stride sets status bit 4 and is
+ * treated as mass_stride tokens long.  `ws` may be null. */
+UOCR_B200_API int uocr_b200_rswa_evict_select(const float* mass, int mass_stride, const int* d_prefill_len, const int* d_slots, int n,
+                                              int keep, int sinks, int recent, int* d_keep, int* d_keep_len,
+                                              uocr_b200_workspace* ws, uocr_b200_stream_t stream);
+
+/* Token d_keep[i][j] of slot d_slots[i] becomes token j of its new region, j < d_keep_len[i], for K and V of
+ * every layer (1..32 views of one geometry behind one table, as in the all-layer append).  d_new_blocks
+ * [n][new_stride] names the new region's blocks -- needed where the old ones are shared with another
+ * sequence; they must not be in use by any slot.  With d_new_blocks == null the region is compacted in place, into
+ * its own first blocks; then the slot must be the only owner of its region.  Rows of the last block
+ * beyond the count are left as they are.  A list must ascend, as evict_select leaves it; tokens outside the
+ * region set status bit 4 and are skipped, bad blocks bit 1.  In place, a slot named twice is moved once. */
+UOCR_B200_API int uocr_b200_rswa_evict_compact_paged_layers(const uocr_b200_paged_kv* kv_layers, int layers, const int* d_prefill_len,
+                                                            const int* d_slots, int n, const int* d_keep, int keep_stride,
+                                                            const int* d_keep_len, const int32_t* d_new_blocks, int new_stride,
+                                                            uocr_b200_workspace* ws, uocr_b200_stream_t stream);
+
+/* Makes the new region of the n slots the one in force, after the rows of all layers have moved: the
+ * block-table row becomes the new blocks (the region's own first ones when d_new_blocks is null), then the
+ * ring's blocks, then -1; d_prefill_len[slot] = count; d_len[l][slot] falls by the evicted tokens in
+ * every layer (ring cursors stay); mass and d_key_pos (either may be null) are compacted along with the tokens,
+ * zero behind them.  d_key_pos starts out as 0, 1, 2, ... for a region that was never evicted from, and is what
+ * uocr_b200_score wants afterwards.  The region must be complete (d_len >= region) in every layer.  The blocks
+ * the slot no longer uses are the caller's to release.  A slot named twice is published once. */
+UOCR_B200_API int uocr_b200_rswa_evict_publish(int32_t* block_table, int table_stride, const int* d_slots, int n, const int* d_keep,
+                                               int keep_stride, const int* d_keep_len, const int32_t* d_new_blocks, int new_stride,
+                                               int* d_len, long long cursor_layer_stride, int layers, int* d_prefill_len, int window,
+                                               float* mass, int mass_stride, int* d_key_pos, int key_pos_stride,
+                                               uocr_b200_workspace* ws, uocr_b200_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

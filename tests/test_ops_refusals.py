@@ -104,3 +104,22 @@ def test_scored_calls_refuse(b):
     assert L.uocr_b200_rswa_mass_scratch_bytes(0, 4, 4) == 0
     assert L.uocr_b200_rswa_mass_scratch_bytes(3, 2, 5) == 128 + 48
     assert L.uocr_b200_rswa_mass_scratch_bytes(60000, 100, 100000) == 4 * 60000 * 100 * 100000 + 8 * 60000 * 100
+
+
+def test_evict_calls_refuse(b):
+    L, fake = b.lib(), 0x1000
+    select = lambda mass=fake, stride=8, pre=fake, n=2, keep=4, sinks=0, recent=0, out=fake, ln=fake: L.uocr_b200_rswa_evict_select(
+        mass, stride, pre, fake, n, keep, sinks, recent, out, ln, None, None)
+    assert select(n=0) == 0
+    for kw in (dict(mass=None), dict(stride=0), dict(pre=None), dict(keep=0), dict(keep=-1), dict(sinks=-1), dict(recent=-1), dict(out=None), dict(ln=None)):
+        assert select(**kw) == 1, kw
+    views = (b.PagedKV * 2)(b.PagedKV(fake, fake, fake, 4, 8, 2, 128, b.BF16), b.PagedKV(fake, fake, fake, 4, 8, 2, 64, b.BF16))
+    compact = lambda layers=1, keep=fake, stride=4, new=fake, new_stride=1, n=2: L.uocr_b200_rswa_evict_compact_paged_layers(
+        views, layers, fake, fake, n, keep, stride, fake, new, new_stride, None, None)
+    assert compact(n=0) == 0
+    assert compact(layers=2) == 1 and compact(layers=0) == 1 and compact(layers=33) == 1  # two geometries; layer counts
+    assert compact(keep=None) == 1 and compact(stride=0) == 1 and compact(new_stride=0) == 1 and compact(n=70000) == 2
+    publish = lambda table=fake, keep=fake, ln=fake, window=4, layers=1, mass=None, ms=0, kp=None, ks=0, new=None, ns=0: L.uocr_b200_rswa_evict_publish(
+        table, 4, fake, 2, keep, 4, fake, new, ns, ln, 8, layers, fake, window, mass, ms, kp, ks, None, None)
+    for kw in (dict(table=None), dict(keep=None), dict(ln=None), dict(window=0), dict(layers=0), dict(mass=fake), dict(kp=fake), dict(new=fake)):
+        assert publish(**kw) == 1, kw

@@ -134,6 +134,9 @@ _SIGS = {
     "uocr_b200_rswa_attention_scored_ragged_paged": (_i, [C.POINTER(PagedKV), C.POINTER(ScoreDesc), _vp, _i] + [_vp] * 3 + [_i, _i, _vp, _vp, _vp]),
     "uocr_b200_rswa_prefill_text_scored_paged": (_i, [C.POINTER(PagedKV), _vp, _vp, _i, C.POINTER(ScoreDesc), _vp, _i] + [_vp] * 4 +
                                                  [_i, _i, _i, _vp, _vp, _vp]),
+    "uocr_b200_rswa_evict_select": (_i, [_vp, _i, _vp, _vp, _i, _i, _i, _i, _vp, _vp, _vp, _vp]),
+    "uocr_b200_rswa_evict_compact_paged_layers": (_i, [_vp, _i, _vp, _vp, _i, _vp, _i, _vp, _vp, _i, _vp, _vp]),
+    "uocr_b200_rswa_evict_publish": (_i, [_vp, _i, _vp, _i, _vp, _i, _vp, _vp, _i, _vp, C.c_longlong, _i, _vp, _i, _vp, _i, _vp, _i, _vp, _vp]),
     "uocr_b200_rope_create": (_i, [C.POINTER(RopeDesc), C.POINTER(_vp)]),
     "uocr_b200_rope_destroy": (_i, [_vp]),
     "uocr_b200_rswa_rope_rows": (_i, [_vp, C.POINTER(QkvRows), _vp, _i64, _vp, _i, _i, _i, _vp]),
@@ -602,3 +605,29 @@ def prefill_text_scored_paged(layer, text_k, text_v, text_blocks, score, q, d_pr
     check(lib().uocr_b200_rswa_prefill_text_scored_paged(layer.ref(), _p(text_k), _p(text_v), text_blocks, C.byref(score.desc), _p(q),
                                                          _dtype_of(q), _p(d_prefill), _p(d_slots), _p(d_pos), _p(d_block0), total, window,
                                                          heads, _p(out), ws.h, stream_handle(stream)))
+
+
+# ---- eviction from the fixed region ----------------------------------------------------------------------
+
+def evict_select(mass, d_prefill, d_slots, n, keep, sinks, recent, d_keep, d_keep_len, ws=None, stream=None):
+    """The `keep` heaviest tokens of each slot's fixed region, ascending: d_keep int32 [n, keep], d_keep_len int32 [n]."""
+    check(lib().uocr_b200_rswa_evict_select(_p(mass), mass.shape[1], _p(d_prefill), _p(d_slots), n, keep, sinks, recent, _p(d_keep),
+                                            _p(d_keep_len), ws.h if ws else None, stream_handle(stream)))
+
+
+def evict_compact_paged_layers(layers, d_prefill, d_slots, n, d_keep, d_keep_len, d_new_blocks=None, ws=None, stream=None):
+    """Moves the kept rows of every layer to the new blocks (None: in place).  layers: PagedLayers, or their layer_array."""
+    arr = layers if isinstance(layers, C.Array) else layer_array(layers)
+    check(lib().uocr_b200_rswa_evict_compact_paged_layers(
+        arr, len(arr), _p(d_prefill), _p(d_slots), n, _p(d_keep), d_keep.shape[1], _p(d_keep_len), _p(d_new_blocks),
+        d_new_blocks.shape[1] if d_new_blocks is not None else 0, ws.h if ws else None, stream_handle(stream)))
+
+
+def evict_publish(table, d_slots, n, d_keep, d_keep_len, d_len, d_prefill, window, d_new_blocks=None, mass=None, d_key_pos=None, ws=None,
+                  stream=None):
+    """Puts the new regions in force: table rows, d_len [layers, slots], d_prefill, and the per-token arrays."""
+    width = lambda t: t.shape[1] if t is not None else 0
+    check(lib().uocr_b200_rswa_evict_publish(
+        _p(table), table.shape[1], _p(d_slots), n, _p(d_keep), d_keep.shape[1], _p(d_keep_len), _p(d_new_blocks), width(d_new_blocks), _p(d_len),
+        d_len.stride(0), d_len.shape[0], _p(d_prefill), window, _p(mass), width(mass), _p(d_key_pos), width(d_key_pos),
+        ws.h if ws else None, stream_handle(stream)))

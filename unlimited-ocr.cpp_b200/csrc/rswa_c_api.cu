@@ -478,6 +478,23 @@ int paged_view(const uocr_b200_paged_kv* kv, PagedView* pv) {
     return UOCR_B200_OK;
 }
 
+// Checks that `layers` views describe pools of one geometry behind one block table and collects the pools.
+int collect_layers(const uocr_b200_paged_kv* kv, int layers, PagedView* pv, LayerPools* pools, const char* who) {
+    if (!kv || layers <= 0 || layers > kMaxLayersPerLaunch)
+        return fail(UOCR_B200_ERR_INVALID, std::string(who) + ": 1..32 layers per call");
+    if (int rc = paged_view(&kv[0], pv)) return rc;
+    for (int l = 0; l < layers; ++l) {
+        PagedView one;
+        if (int rc = paged_view(&kv[l], &one)) return rc;
+        if (kv[l].dtype != kv[0].dtype || one.table != pv->table || one.table_stride != pv->table_stride ||
+            one.num_blocks != pv->num_blocks || one.kv_heads != pv->kv_heads || one.head_dim != pv->head_dim)
+            return fail(UOCR_B200_ERR_INVALID, std::string(who) + ": the layers must share block table, geometry and dtype");
+        pools->k[l] = one.k_pool;
+        pools->v[l] = one.v_pool;
+    }
+    return UOCR_B200_OK;
+}
+
 }  // namespace uocr_b200
 
 extern "C" {
@@ -529,23 +546,6 @@ int uocr_b200_rswa_append_decode_batch_paged(const uocr_b200_paged_kv* kv, const
     else
         rswa_append_paged_kernel<F32><<<batch, 256, 0, st>>>(pv, k, v, d_len, d_ring_pos, d_prefill_len, d_slots, window, status);
     return after_launch("append (paged)");
-}
-
-// Checks that `layers` views describe pools of one geometry behind one block table and collects the pools.
-static int collect_layers(const uocr_b200_paged_kv* kv, int layers, PagedView* pv, LayerPools* pools, const char* who) {
-    if (!kv || layers <= 0 || layers > kMaxLayersPerLaunch)
-        return fail(UOCR_B200_ERR_INVALID, std::string(who) + ": 1..32 layers per call");
-    if (int rc = paged_view(&kv[0], pv)) return rc;
-    for (int l = 0; l < layers; ++l) {
-        PagedView one;
-        if (int rc = paged_view(&kv[l], &one)) return rc;
-        if (kv[l].dtype != kv[0].dtype || one.table != pv->table || one.table_stride != pv->table_stride ||
-            one.num_blocks != pv->num_blocks || one.kv_heads != pv->kv_heads || one.head_dim != pv->head_dim)
-            return fail(UOCR_B200_ERR_INVALID, std::string(who) + ": the layers must share block table, geometry and dtype");
-        pools->k[l] = one.k_pool;
-        pools->v[l] = one.v_pool;
-    }
-    return UOCR_B200_OK;
 }
 
 int uocr_b200_rswa_append_decode_batch_paged_layers(const uocr_b200_paged_kv* kv_layers, int layers, const float* k,

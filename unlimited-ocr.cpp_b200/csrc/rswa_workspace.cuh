@@ -52,7 +52,10 @@ inline bool head_dim_ok(int hd, int dtype) {
 }
 
 struct PagedView;
+struct LayerPools;
+// Checked views of one layer, and of several layers of one geometry behind one block table.
 int paged_view(const uocr_b200_paged_kv* kv, PagedView* pv);
+int collect_layers(const uocr_b200_paged_kv* kv, int layers, PagedView* pv, LayerPools* pools, const char* who);
 
 }  // namespace uocr_b200
 
