@@ -565,6 +565,25 @@ UOCR_B200_API int uocr_b200_rswa_prefill_text_scored_paged(
     const int* d_pos, const int* d_text_block0, int total, int window, int heads, void* out, uocr_b200_workspace* ws,
     uocr_b200_stream_t stream);
 
+/* Packed vision and text rows on the tcgen05 tensor cores (bf16 KV, head_dim 128):
+ * uocr_b200_rswa_prefill_attention_tc with modified scores, tiles and plans as there.  d_lo / d_hi / d_q_pos are
+ * per packed row.  A plan (made by the plan call, or by the attention call when h_tiles is given) covers the
+ * keys that some row of a tile sees and so belongs to the ranges it was made with: it is reused by calls whose d_lo,
+ * d_hi and prefix lengths still hold the same values, and never by the call without modified scores.  fp32
+ * queries and fp32 results go through the tensor cores as bf16 pairs; bf16 queries are taken as they are and, for bf16
+ * results, the probabilities are rounded to bf16 (half a step, as the result itself).  K and V outside
+ * the span of keys that the rows of a query tile see -- from the first to the last -- may hold anything; inside it
+ * they must be finite, since the rows that do not see a key multiply its value by zero.  d_key_pos is not supported (UNSUPPORTED): keys
+ * stand at their own index. */
+UOCR_B200_API int uocr_b200_rswa_prefill_attention_scored_tc(
+    const uocr_b200_paged_kv* kv, const void* text_k_pool, const void* text_v_pool, int text_blocks,
+    const uocr_b200_score* score, const void* q, int q_dtype, const int* d_prefill_len,
+    const uocr_b200_prefill_tile* h_tiles, int n_tiles, int window, int heads, void* out, uocr_b200_workspace* ws,
+    uocr_b200_stream_t stream);
+UOCR_B200_API int uocr_b200_rswa_prefill_plan_scored_tc(const uocr_b200_score* score, const uocr_b200_prefill_tile* h_tiles, int n_tiles,
+                                                        const int* d_prefill_len, int window, uocr_b200_workspace* ws,
+                                                        uocr_b200_stream_t stream);
+
 /* ================================================================================================
  * Eviction from the fixed region by accumulated attention weight (no reference counterpart; the
  * reference keeps every vision token for good).  A step of an evicting engine: choose with

@@ -134,6 +134,8 @@ _SIGS = {
     "uocr_b200_rswa_attention_scored_ragged_paged": (_i, [C.POINTER(PagedKV), C.POINTER(ScoreDesc), _vp, _i] + [_vp] * 3 + [_i, _i, _vp, _vp, _vp]),
     "uocr_b200_rswa_prefill_text_scored_paged": (_i, [C.POINTER(PagedKV), _vp, _vp, _i, C.POINTER(ScoreDesc), _vp, _i] + [_vp] * 4 +
                                                  [_i, _i, _i, _vp, _vp, _vp]),
+    "uocr_b200_rswa_prefill_attention_scored_tc": (_i, [C.POINTER(PagedKV), _vp, _vp, _i, C.POINTER(ScoreDesc), _vp, _i, _vp, _vp, _i, _i, _i, _vp, _vp, _vp]),
+    "uocr_b200_rswa_prefill_plan_scored_tc": (_i, [C.POINTER(ScoreDesc), _vp, _i, _vp, _i, _vp, _vp]),
     "uocr_b200_rswa_evict_select": (_i, [_vp, _i, _vp, _vp, _i, _i, _i, _i, _vp, _vp, _vp, _vp]),
     "uocr_b200_rswa_evict_compact_paged_layers": (_i, [_vp, _i, _vp, _vp, _i, _vp, _i, _vp, _vp, _i, _vp, _vp]),
     "uocr_b200_rswa_evict_publish": (_i, [_vp, _i, _vp, _i, _vp, _i, _vp, _vp, _i, _vp, C.c_longlong, _i, _vp, _i, _vp, _i, _vp, _i, _vp, _vp]),
@@ -605,6 +607,22 @@ def prefill_text_scored_paged(layer, text_k, text_v, text_blocks, score, q, d_pr
     check(lib().uocr_b200_rswa_prefill_text_scored_paged(layer.ref(), _p(text_k), _p(text_v), text_blocks, C.byref(score.desc), _p(q),
                                                          _dtype_of(q), _p(d_prefill), _p(d_slots), _p(d_pos), _p(d_block0), total, window,
                                                          heads, _p(out), ws.h, stream_handle(stream)))
+
+
+def prefill_plan_scored_tc(score, tiles, d_prefill, window, ws, stream=None):
+    """Uploads and orders the query tiles for the score's visible ranges; later calls with reuse_plan=True share the plan."""
+    import numpy as np
+    t = np.ascontiguousarray(tiles, dtype=np.int32)
+    check(lib().uocr_b200_rswa_prefill_plan_scored_tc(C.byref(score.desc), t.ctypes.data, t.shape[0], _p(d_prefill), window, ws.h, stream_handle(stream)))
+
+
+def prefill_attention_scored_tc(layer, text_k, text_v, text_blocks, score, q, d_prefill, tiles, window, heads, out, ws, stream=None, reuse_plan=False):
+    """prefill_attention_tc with modified scores; q fp32 or bf16."""
+    import numpy as np
+    t = np.ascontiguousarray(tiles, dtype=np.int32)
+    check(lib().uocr_b200_rswa_prefill_attention_scored_tc(
+        layer.ref(), _p(text_k), _p(text_v), text_blocks, C.byref(score.desc), _p(q), _dtype_of(q), _p(d_prefill),
+        None if reuse_plan else t.ctypes.data, t.shape[0], window, heads, _p(out), ws.h, stream_handle(stream)))
 
 
 # ---- eviction from the fixed region ----------------------------------------------------------------------

@@ -495,6 +495,74 @@ int collect_layers(const uocr_b200_paged_kv* kv, int layers, PagedView* pv, Laye
     return UOCR_B200_OK;
 }
 
+// Tensor map of a K or V pool seen as a [rows][128] bf16 matrix, fetched in boxes of 16 rows x 64
+// elements (one 16-token block of one head, one 128-byte half of each row) with the 128-byte swizzle
+// the tensor-core operand layout uses.  Rows at or beyond `rows` read as zeros.
+int make_kv_map(CUtensorMap* map, const void* pool, long rows) {
+    using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                     const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                     CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+    static EncodeTiled encode = [] {
+        void* fn = nullptr;
+        cudaDriverEntryPointQueryResult found;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &found) != cudaSuccess ||
+            found != cudaDriverEntryPointSuccess)
+            fn = nullptr;
+        return reinterpret_cast<EncodeTiled>(fn);
+    }();
+    if (!encode) return fail(UOCR_B200_ERR_CUDA, "prefill_attention_tc: the driver does not export the tensor-map encoder");
+    if (!aligned16(pool) || rows <= 0 || rows >= (1L << 31))
+        return fail(UOCR_B200_ERR_INVALID, "prefill_attention_tc: pool must be 16-byte aligned and hold fewer than 2^31 token rows");
+    const cuuint64_t dims[2] = {(cuuint64_t)kTcTile, (cuuint64_t)rows};
+    const cuuint64_t strides[1] = {(cuuint64_t)kTcTile * 2};
+    const cuuint32_t box[2] = {64, (cuuint32_t)kBlockTokens};
+    const cuuint32_t elem_strides[2] = {1, 1};
+    const CUresult rc = encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(pool), dims, strides, box, elem_strides,
+                               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (rc != CUDA_SUCCESS) return fail(UOCR_B200_ERR_CUDA, "prefill_attention_tc: tensor-map encoding failed");
+    return UOCR_B200_OK;
+}
+
+// Uploads the tile descriptors and orders them on the device (the prefix lengths live there).
+int prefill_plan(const uocr_b200_prefill_tile* h_tiles, int n_tiles, const int* d_prefill_len, int window, const uocr_b200_score* score,
+                 uocr_b200_workspace* ws, cudaStream_t st, const char* who) {
+    if (!h_tiles || !d_prefill_len || !ws) return fail(UOCR_B200_ERR_INVALID, std::string(who) + ": null pointer");
+    if (n_tiles <= 0 || window <= 0) return fail(UOCR_B200_ERR_INVALID, std::string(who) + ": tile count and window must be positive");
+    if (n_tiles > ws->tiles_cap) return fail(UOCR_B200_ERR_WORKSPACE, std::string(who) + ": more tiles than the workspace holds");
+    bool any_text = false;
+    for (int i = 0; i < n_tiles; ++i) {
+        const uocr_b200_prefill_tile& t = h_tiles[i];
+        if (t.rows < 1 || t.rows > kTcTile || t.row0 < 0 || t.slot < 0 || t.pos0 < 0 || (t.kind != 0 && t.kind != 1))
+            return fail(UOCR_B200_ERR_INVALID, std::string(who) + ": bad tile descriptor");
+        any_text |= t.kind == 1;
+    }
+    static_assert(sizeof(uocr_b200_prefill_tile) == sizeof(PrefillTile), "tile descriptor layouts must match");
+    ws->plan_tiles = 0;
+    // pageable source: the copy has read the descriptors when the call returns
+    CHECK_CUDA(cudaMemcpyAsync(ws->tiles, h_tiles, sizeof(PrefillTile) * (size_t)n_tiles, cudaMemcpyHostToDevice, st),
+               "tile descriptors H2D");
+    PrefillParams pp{};
+    pp.tiles = ws->tiles;
+    pp.n_tiles = n_tiles;
+    pp.d_prefill_len = d_prefill_len;
+    pp.window = window;
+    if (score) {
+        pp.d_lo = score->d_lo;
+        pp.d_hi = score->d_hi;
+        rswa_prefill_order_kernel<true><<<1, 1024, 0, st>>>(pp, ws->tile_work);
+    } else {
+        rswa_prefill_order_kernel<false><<<1, 256, 0, st>>>(pp, ws->tile_work);
+    }
+    if (int rc = after_launch("prefill tile order")) return rc;
+    ws->plan_tiles = n_tiles;
+    ws->plan_window = window;
+    ws->plan_any_text = any_text;
+    ws->plan_scored = score != nullptr;
+    ++ws->plan_serial;
+    return UOCR_B200_OK;
+}
+
 }  // namespace uocr_b200
 
 extern "C" {
@@ -834,72 +902,11 @@ int uocr_b200_rswa_text_scatter_fill_paged(const uocr_b200_paged_kv* kv, void* t
     return after_launch("text scatter + ring fill");
 }
 
-// Tensor map of a K or V pool seen as a [rows][128] bf16 matrix, fetched in boxes of 16 rows x 64
-// elements (one 16-token block of one head, one 128-byte half of each row) with the 128-byte swizzle
-// the tensor-core operand layout uses.  Rows at or beyond `rows` read as zeros.
-static int make_kv_map(CUtensorMap* map, const void* pool, long rows) {
-    using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
-                                     const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
-                                     CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-    static EncodeTiled encode = [] {
-        void* fn = nullptr;
-        cudaDriverEntryPointQueryResult found;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &found) != cudaSuccess ||
-            found != cudaDriverEntryPointSuccess)
-            fn = nullptr;
-        return reinterpret_cast<EncodeTiled>(fn);
-    }();
-    if (!encode) return fail(UOCR_B200_ERR_CUDA, "prefill_attention_tc: the driver does not export the tensor-map encoder");
-    if (!aligned16(pool) || rows <= 0 || rows >= (1L << 31))
-        return fail(UOCR_B200_ERR_INVALID, "prefill_attention_tc: pool must be 16-byte aligned and hold fewer than 2^31 token rows");
-    const cuuint64_t dims[2] = {(cuuint64_t)kTcTile, (cuuint64_t)rows};
-    const cuuint64_t strides[1] = {(cuuint64_t)kTcTile * 2};
-    const cuuint32_t box[2] = {64, (cuuint32_t)kBlockTokens};
-    const cuuint32_t elem_strides[2] = {1, 1};
-    const CUresult rc = encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(pool), dims, strides, box, elem_strides,
-                               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
-                               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    if (rc != CUDA_SUCCESS) return fail(UOCR_B200_ERR_CUDA, "prefill_attention_tc: tensor-map encoding failed");
-    return UOCR_B200_OK;
-}
-
-// Uploads the tile descriptors and orders them on the device (the prefix lengths live there).
-static int prefill_plan(const uocr_b200_prefill_tile* h_tiles, int n_tiles, const int* d_prefill_len, int window,
-                        uocr_b200_workspace* ws, cudaStream_t st, const char* who) {
-    if (!h_tiles || !d_prefill_len || !ws) return fail(UOCR_B200_ERR_INVALID, std::string(who) + ": null pointer");
-    if (n_tiles <= 0 || window <= 0) return fail(UOCR_B200_ERR_INVALID, std::string(who) + ": tile count and window must be positive");
-    if (n_tiles > ws->tiles_cap) return fail(UOCR_B200_ERR_WORKSPACE, std::string(who) + ": more tiles than the workspace holds");
-    bool any_text = false;
-    for (int i = 0; i < n_tiles; ++i) {
-        const uocr_b200_prefill_tile& t = h_tiles[i];
-        if (t.rows < 1 || t.rows > kTcTile || t.row0 < 0 || t.slot < 0 || t.pos0 < 0 || (t.kind != 0 && t.kind != 1))
-            return fail(UOCR_B200_ERR_INVALID, std::string(who) + ": bad tile descriptor");
-        any_text |= t.kind == 1;
-    }
-    static_assert(sizeof(uocr_b200_prefill_tile) == sizeof(PrefillTile), "tile descriptor layouts must match");
-    ws->plan_tiles = 0;
-    // pageable source: the copy has read the descriptors when the call returns
-    CHECK_CUDA(cudaMemcpyAsync(ws->tiles, h_tiles, sizeof(PrefillTile) * (size_t)n_tiles, cudaMemcpyHostToDevice, st),
-               "tile descriptors H2D");
-    PrefillParams pp{};
-    pp.tiles = ws->tiles;
-    pp.n_tiles = n_tiles;
-    pp.d_prefill_len = d_prefill_len;
-    pp.window = window;
-    rswa_prefill_order_kernel<<<1, 256, 0, st>>>(pp, ws->tile_work);
-    if (int rc = after_launch("prefill tile order")) return rc;
-    ws->plan_tiles = n_tiles;
-    ws->plan_window = window;
-    ws->plan_any_text = any_text;
-    ++ws->plan_serial;
-    return UOCR_B200_OK;
-}
-
 unsigned uocr_b200_workspace_prefill_plan_serial(const uocr_b200_workspace* ws) { return ws ? ws->plan_serial : 0u; }
 
 int uocr_b200_rswa_prefill_plan_tc(const uocr_b200_prefill_tile* h_tiles, int n_tiles, const int* d_prefill_len, int window,
                                    uocr_b200_workspace* ws, uocr_b200_stream_t stream) {
-    return prefill_plan(h_tiles, n_tiles, d_prefill_len, window, ws, reinterpret_cast<cudaStream_t>(stream), "prefill_plan_tc");
+    return prefill_plan(h_tiles, n_tiles, d_prefill_len, window, nullptr, ws, reinterpret_cast<cudaStream_t>(stream), "prefill_plan_tc");
 }
 
 int uocr_b200_rswa_prefill_attention_tc(const uocr_b200_paged_kv* kv, const void* text_k_pool, const void* text_v_pool,
@@ -919,8 +926,8 @@ int uocr_b200_rswa_prefill_attention_tc(const uocr_b200_paged_kv* kv, const void
     if (int rc = device_info(&di)) return rc;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     if (h_tiles) {
-        if (int rc = prefill_plan(h_tiles, n_tiles, d_prefill_len, window, ws, st, "prefill_attention_tc")) return rc;
-    } else if (ws->plan_tiles != n_tiles || ws->plan_window != window) {
+        if (int rc = prefill_plan(h_tiles, n_tiles, d_prefill_len, window, nullptr, ws, st, "prefill_attention_tc")) return rc;
+    } else if (ws->plan_tiles != n_tiles || ws->plan_window != window || ws->plan_scored) {
         return fail(UOCR_B200_ERR_INVALID, "prefill_attention_tc: no tiles given and the workspace holds no plan of this size and window");
     }
     if (ws->plan_any_text && (!text_k_pool || !text_v_pool || text_blocks <= 0))
@@ -955,7 +962,7 @@ int uocr_b200_rswa_prefill_attention_tc(const uocr_b200_paged_kv* kv, const void
     int dev = 0;
     cudaGetDevice(&dev);
     if (!configured[dev & 63]) {
-        CHECK_CUDA(cudaFuncSetAttribute(rswa_prefill_tc_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kTcSmemBytes),
+        CHECK_CUDA(cudaFuncSetAttribute(rswa_prefill_tc_kernel<TcPlain>, cudaFuncAttributeMaxDynamicSharedMemorySize, kTcSmemBytes),
                    "prefill smem attribute");
         configured[dev & 63] = true;
     }
@@ -974,7 +981,7 @@ int uocr_b200_rswa_prefill_attention_tc(const uocr_b200_paged_kv* kv, const void
     // the persistent grid: one CTA per SM draws (tile, head) items in the plan's order
     const long long n_items = (long long)n_tiles * heads;
     const int grid = (int)std::min<long long>(n_items, di->sms);
-    rswa_prefill_tc_kernel<<<grid, kTcThreads, kTcSmemBytes, st>>>(pp, maps);
+    rswa_prefill_tc_kernel<TcPlain><<<grid, kTcThreads, kTcSmemBytes, st>>>(pp, maps);
     return after_launch("tensor-core prefill attention");
 }
 

@@ -49,6 +49,7 @@
 #include <cuda.h>  // CUtensorMap (type only; the encoder is fetched through the runtime)
 
 #include "rswa_device.cuh"
+#include "uocr_rswa_b200.h"
 
 namespace uocr_b200 {
 
@@ -60,6 +61,15 @@ struct PrefillTile {
     int pos0;    // position of the first row (prefix index for kind 0, text index for kind 1)
     int block0;  // kind 1: first block of the request's tokens in the text pool
 };
+
+// What a kernel instantiation computes.  SCORED: scores modified as uocr_b200_score says (CAP: tanh cap, BIAS: distance
+// bias) and visible ranges per row; PAIR_Q / PAIR_P: Q / P go to the tensor cores as bf16 pairs (fp32 queries / fp32
+// results) instead of as one bf16 each (bf16 queries, which are exact, / bf16 results, whose own rounding is no finer).
+template <bool SCORED, bool CAP, bool BIAS, bool PAIR_Q, bool PAIR_P>
+struct TcMode {
+    static constexpr bool kScored = SCORED, kCap = CAP, kBias = BIAS, kPairQ = PAIR_Q, kPairP = PAIR_P;
+};
+using TcPlain = TcMode<false, false, false, true, true>;
 
 struct TcWork;
 struct PrefillParams {
@@ -82,6 +92,13 @@ struct PrefillParams {
     int* status;
     uint32_t wait_limit;  // polls a wait may take before the role gives up (kWaitLimit unless a test lowers it); the
                           // drains of copies and MMAs in flight keep the full limit
+    // modified scores; all of them per packed row
+    const int* d_lo;
+    const int* d_hi;
+    const int* d_q_pos;
+    const float* slopes;
+    float score_mul;   // of q.k: 2 log2(e) scale / cap with a cap, log2(e) scale without
+    float cap_log2;    // cap * log2(e)
 };
 
 constexpr int kTcTile = 128;             // queries per CTA, keys per step, head_dim
@@ -153,6 +170,13 @@ __device__ __forceinline__ void tc_split2(float a, float b, uint32_t& hi, uint32
     hi = __byte_perm(ua, ub, 0x7632);
     const float ra = a - __uint_as_float(ua & 0xffff0000u), rb = b - __uint_as_float(ub & 0xffff0000u);
     lo = __byte_perm(__float_as_uint(ra), __float_as_uint(rb), 0x7632);
+}
+
+// The same split with both parts rounded to nearest: off by 2^-16 at most, a quarter of the truncating split's error,
+// for the same number of instructions.
+__device__ __forceinline__ void tc_split2_rn(float a, float b, uint32_t& hi, uint32_t& lo) {
+    hi = rn_bf16x2(a, b);
+    lo = rn_bf16x2(a - bf16_lo(hi), b - bf16_hi(hi));
 }
 
 __device__ __forceinline__ float tc_exp2(float x) {
@@ -233,6 +257,26 @@ __device__ __forceinline__ bool pair_sync(uint32_t bar, uint32_t parity, int* st
 // follows the maximum in steps.
 constexpr float kTcMaxSlack = 8.f;
 
+__device__ __forceinline__ float tc_rcp(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// Scores of 64 keys modified in place, into the log2 domain.  tanh(x) = 1 - 2 / (1 + e^2x): two special-function
+// instructions, off by 2^-22 at most, and right at both ends (e^2x = 0 or infinity).  d0: the query's position minus
+// that of key 0.
+template <typename Mode>
+__device__ __forceinline__ void tc_modify(uint32_t (&s)[64], float mul, float cap_log2, float slope_log2, float d0) {
+#pragma unroll
+    for (int j = 0; j < 64; ++j) {
+        float x = __uint_as_float(s[j]) * mul;
+        if constexpr (Mode::kCap) x = fmaf(-2.f * cap_log2, tc_rcp(1.f + tc_exp2(x)), cap_log2);
+        if constexpr (Mode::kBias) x = fmaf(-slope_log2, fabsf(d0 - (float)j), x);
+        s[j] = __float_as_uint(x);
+    }
+}
+
 // One key tile of the online softmax for this thread: its row, its half (64 keys) of the tile.
 // Reads S once, agrees on the row maximum with the thread that owns the other half (shared-memory
 // exchange + a 64-thread rendezvous), writes P as bf16 pairs over its own 64 columns of the S buffer:
@@ -242,11 +286,14 @@ constexpr float kTcMaxSlack = 8.f;
 // m_ref is the reference the row's probabilities are scaled by; alpha is the factor the row's
 // accumulator and sum take when the reference moved (1 otherwise).  False if the rendezvous ran out
 // of time.
+template <typename Mode>
 __device__ __forceinline__ bool tc_softmax_half(bool full, uint32_t tS, int h, int vlo, int vhi, float* my_max, const float* other_max,
                                                 uint32_t pair_bar, uint32_t pair_parity, int* status, uint32_t wait_limit,
-                                                float& m_ref, float& l_run, float& alpha) {
+                                                float& m_ref, float& l_run, float& alpha, float mul = 0.f, float cap_log2 = 0.f,
+                                                float slope_log2 = 0.f, float d0 = 0.f) {
     uint32_t s[64];
     tc_ld64(tS + h * 64, s);
+    if constexpr (Mode::kScored) tc_modify<Mode>(s, mul, cap_log2, slope_log2, d0);
     if (!full) {
         // Of this thread's 64 keys the visible ones are [lo, hi).  A causal edge only has an upper bound, a window
         // edge only a lower one: each bound is applied only where some row of the warp needs it.
@@ -277,17 +324,30 @@ __device__ __forceinline__ bool tc_softmax_half(bool full, uint32_t tS, int h, i
     }
     const float m_safe = (m_ref == -INFINITY) ? 0.f : m_ref;
     float lsum = 0.f;
-#pragma unroll
-    for (int qq = 0; qq < 2; ++qq) {  // 32 keys at a time: their 16 hi words, then their 16 lo words, over their own columns
+    if constexpr (!Mode::kPairP) {  // one bf16 per probability: 64 keys in the first 32 of this thread's columns
         uint32_t pk[32];
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-            const float p0 = tc_exp2(__uint_as_float(s[qq * 32 + 2 * e]) - m_safe);
-            const float p1 = tc_exp2(__uint_as_float(s[qq * 32 + 2 * e + 1]) - m_safe);
+        for (int e = 0; e < 32; ++e) {
+            const float p0 = tc_exp2(__uint_as_float(s[2 * e]) - m_safe);
+            const float p1 = tc_exp2(__uint_as_float(s[2 * e + 1]) - m_safe);
             lsum += p0 + p1;
-            tc_split2(p0, p1, pk[e], pk[16 + e]);
+            pk[e] = rn_bf16x2(p0, p1);
         }
-        tc_st32(tS + h * 64 + qq * 32, pk);
+        tc_st32(tS + h * 64, pk);
+    } else {
+#pragma unroll
+        for (int qq = 0; qq < 2; ++qq) {  // 32 keys at a time: their 16 hi words, then their 16 lo words, over their own columns
+            uint32_t pk[32];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const float p0 = tc_exp2(__uint_as_float(s[qq * 32 + 2 * e]) - m_safe);
+                const float p1 = tc_exp2(__uint_as_float(s[qq * 32 + 2 * e + 1]) - m_safe);
+                lsum += p0 + p1;
+                if constexpr (Mode::kScored) tc_split2_rn(p0, p1, pk[e], pk[16 + e]);
+                else tc_split2(p0, p1, pk[e], pk[16 + e]);
+            }
+            tc_st32(tS + h * 64 + qq * 32, pk);
+        }
     }
     asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
     l_run = l_run * alpha + lsum;
@@ -315,7 +375,7 @@ struct TcWork {
     int n_prefix_tiles;  // key tiles in the fixed region, then (text rows) in the text window from tile text_tile0
     int text_tile0;
     int n_steps;
-    int pad[2];
+    int fixed_lo, fixed_hi;  // modified scores: the tokens of the fixed region that some row sees
 };
 static_assert(sizeof(TcWork) == 48, "three 16-byte loads");
 
@@ -324,6 +384,7 @@ struct TcItem {
     PrefillTile t;
     int head, kvh;
     int pfx, n_prefix_tiles, text_tile0, n_steps;
+    int fixed_lo, fixed_hi;
     bool valid;
 };
 constexpr int kTcItemSlots = 8;  // items the CTA's scheduler may have published and not every role has read
@@ -347,19 +408,50 @@ __device__ __forceinline__ void tc_tile_steps(const PrefillTile& t, int pfx, int
 // one count is arbitrary), and leaves each with its counts in `work`.  The persistent grid hands out (tile, head)
 // items in this order, heads innermost: CTA c starts with item c, the counter (zero at launch) gives the rest.
 constexpr int kTcOrderBins = 256;
-__global__ void __launch_bounds__(256) rswa_prefill_order_kernel(const PrefillParams p, TcWork* work) {
+
+// What row r (packed row t.row0 + r) of a tile sees of the fixed region: tokens [lo, hi), hi <= lo if none.
+__device__ __forceinline__ void tc_row_range(const PrefillParams& p, const PrefillTile& t, int r, int pfx, int& lo, int& hi) {
+    lo = p.d_lo ? max(__ldg(p.d_lo + t.row0 + r), 0) : 0;
+    hi = min(p.d_hi ? __ldg(p.d_hi + t.row0 + r) : (t.kind == 0 ? t.pos0 + r + 1 : pfx), pfx);
+}
+
+template <bool SCORED>
+__global__ void __launch_bounds__(SCORED ? 1024 : 256) rswa_prefill_order_kernel(const PrefillParams p, TcWork* work) {
     __shared__ int hist[kTcOrderBins];
+    // With visible ranges a warp takes a tile (its lanes look at the rows), otherwise a thread does.
+    const int lane = threadIdx.x & 31;
+    const int first = SCORED ? threadIdx.x >> 5 : threadIdx.x, step = SCORED ? blockDim.x >> 5 : blockDim.x;
     auto work_of = [&](int i) {
         TcWork w;
         w.t = p.tiles[i];
         w.pfx = max(__ldg(p.d_prefill_len + w.t.slot), 0);
         tc_tile_steps(w.t, w.pfx, p.window, w.n_prefix_tiles, w.text_tile0, w.n_steps);
-        w.pad[0] = w.pad[1] = 0;
+        w.fixed_lo = w.fixed_hi = 0;
+        if constexpr (SCORED) {
+            int ulo = 0x7fffffff, uhi = 0;
+            for (int r = lane; r < w.t.rows; r += 32) {
+                int lo, hi;
+                tc_row_range(p, w.t, r, w.pfx, lo, hi);
+                if (hi > lo) {
+                    ulo = min(ulo, lo);
+                    uhi = max(uhi, hi);
+                }
+            }
+            w.fixed_lo = __reduce_min_sync(0xffffffffu, ulo);
+            w.fixed_hi = __reduce_max_sync(0xffffffffu, uhi);
+            const int text_tiles = w.n_steps - w.n_prefix_tiles;
+            if (w.fixed_hi == 0) w.fixed_lo = 0;
+            w.n_prefix_tiles = (w.fixed_hi + kTcTile - 1) / kTcTile - w.fixed_lo / kTcTile;
+            w.n_steps = w.n_prefix_tiles + text_tiles;
+        }
         return w;
     };
     for (int i = threadIdx.x; i < kTcOrderBins; i += blockDim.x) hist[i] = 0;
     __syncthreads();
-    for (int i = threadIdx.x; i < p.n_tiles; i += blockDim.x) atomicAdd(&hist[min(work_of(i).n_steps, kTcOrderBins - 1)], 1);
+    for (int i = first; i < p.n_tiles; i += step) {
+        const int bin = min(work_of(i).n_steps, kTcOrderBins - 1);
+        if (!SCORED || lane == 0) atomicAdd(&hist[bin], 1);
+    }
     __syncthreads();
     if (threadIdx.x == 0) {  // first index of each count, largest count first
         int at = 0;
@@ -370,9 +462,9 @@ __global__ void __launch_bounds__(256) rswa_prefill_order_kernel(const PrefillPa
         }
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < p.n_tiles; i += blockDim.x) {
+    for (int i = first; i < p.n_tiles; i += step) {
         const TcWork w = work_of(i);
-        work[atomicAdd(&hist[min(w.n_steps, kTcOrderBins - 1)], 1)] = w;
+        if (!SCORED || lane == 0) work[atomicAdd(&hist[min(w.n_steps, kTcOrderBins - 1)], 1)] = w;
     }
 }
 
@@ -382,6 +474,7 @@ __global__ void __launch_bounds__(256) rswa_prefill_order_kernel(const PrefillPa
 #define UOCR_TC_REGS_HELPER 104
 #define UOCR_TC_REGS_ISSUE 64
 
+template <typename Mode>
 __global__ void __launch_bounds__(kTcThreads, 1)
 rswa_prefill_tc_kernel(const PrefillParams p, const __grid_constant__ PrefillMaps maps) {
     extern __shared__ uint8_t smem_raw[];
@@ -419,6 +512,22 @@ rswa_prefill_tc_kernel(const PrefillParams p, const __grid_constant__ PrefillMap
     // written; item_empty: every reading warp (8 softmax, 4 helper, V producer, the two issuers) has read it.
     auto item_full = [&](uint32_t sl) { return bar0 + (32 + sl) * 8; };
     auto item_empty = [&](uint32_t sl) { return bar0 + (40 + sl) * 8; };
+    // Modified scores: the rows of V stage b outside the tokens that some row sees have been zeroed.  Such a partly
+    // visible block is one phase of the stage's barrier.
+    auto v_clean = [&](uint32_t b) { return bar0 + (48 + b) * 8; };
+    // Token range [lo, hi) of the item's key tile n that some row sees, relative to the tile's first token t0.
+    auto tile_span = [&](const TcItem& it, bool text, int t0, int& lo, int& hi) {
+        lo = (text ? max(0, it.t.pos0 - p.window + 1) : it.fixed_lo) - t0;
+        hi = (text ? it.t.pos0 + it.t.rows : it.fixed_hi) - t0;
+    };
+    auto cuts_block = [&](int lo, int hi) {
+        return (lo > 0 && (lo & (kBlockTokens - 1))) || (hi < kTcTile && (hi & (kBlockTokens - 1)));
+    };
+    auto first_token = [&](const TcItem& it, int n) {  // of key tile n
+        if (n >= it.n_prefix_tiles) return (it.text_tile0 + n - it.n_prefix_tiles) * kTcTile;
+        if constexpr (Mode::kScored) return (it.fixed_lo / kTcTile + n) * kTcTile;
+        else return n * kTcTile;
+    };
     constexpr uint32_t kItemReaders = 8 + 4 + 1 + 1 + 1;
     auto read_slot = [&](uint32_t sl) {
         const int* w = item_ring + sl * kTcItemInts;
@@ -426,6 +535,10 @@ rswa_prefill_tc_kernel(const PrefillParams p, const __grid_constant__ PrefillMap
         it.t.row0 = w[0]; it.t.rows = w[1]; it.t.slot = w[2]; it.t.kind = w[3]; it.t.pos0 = w[4]; it.t.block0 = w[5];
         it.head = w[6]; it.pfx = w[7]; it.n_prefix_tiles = w[8]; it.text_tile0 = w[9]; it.n_steps = w[10];
         it.valid = w[11] != 0;
+        if constexpr (Mode::kScored) {
+            it.fixed_lo = w[12];
+            it.fixed_hi = w[13];
+        }
         it.kvh = it.head / p.group;
         if (!it.valid) it.n_steps = 0;
         return it;
@@ -466,6 +579,7 @@ rswa_prefill_tc_kernel(const PrefillParams p, const __grid_constant__ PrefillMap
             mbar_init(o_full(b), 1);
             mbar_init(q_full(b), kTcHelperThreads);
             mbar_init(l_ready(b), kTcSoftmaxThreads);
+            mbar_init(v_clean(b), 1);
         }
         mbar_init(q_landed, kTcHelperThreads);
         mbar_init(o_read, kTcHelperThreads);
@@ -507,7 +621,16 @@ rswa_prefill_tc_kernel(const PrefillParams p, const __grid_constant__ PrefillMap
             const PrefillTile& t = cur.t;
             const bool live = r < t.rows;
             const int i = t.pos0 + r;
-            const int phi = !live ? 0 : (t.kind == 0 ? min(i + 1, cur.pfx) : cur.pfx);  // fixed-region tokens [0, phi)
+            int plo = 0, phi = !live ? 0 : (t.kind == 0 ? min(i + 1, cur.pfx) : cur.pfx);  // fixed-region tokens [plo, phi)
+            int q_pos = i;
+            float slope_log2 = 0.f;
+            if constexpr (Mode::kScored) {
+                if (live) tc_row_range(p, t, r, cur.pfx, plo, phi);
+                if constexpr (Mode::kBias) {
+                    if (live && p.d_q_pos) q_pos = __ldg(p.d_q_pos + t.row0 + r);
+                    slope_log2 = __ldg(p.slopes + cur.head) * 1.4426950408889634f;
+                }
+            }
             const int tlo = max(0, i - p.window + 1);
             const int thi = (live && t.kind == 1) ? i + 1 : 0;                           // text tokens [tlo, thi)
             // Q of this item is in TMEM: the helpers have also taken the sums of the item before last out of xsum
@@ -516,8 +639,8 @@ rswa_prefill_tc_kernel(const PrefillParams p, const __grid_constant__ PrefillMap
             for (int n = 0; n < cur.n_steps; ++n) {
                 const uint32_t gn = g + n, b = gn & 1u, par = (gn >> 1) & 1u;
                 const bool text = n >= cur.n_prefix_tiles;
-                const int t0 = text ? (cur.text_tile0 + n - cur.n_prefix_tiles) * kTcTile : n * kTcTile;
-                const int vlo = text ? tlo - t0 : -(1 << 30);
+                const int t0 = first_token(cur, n);
+                const int vlo = text ? tlo - t0 : (Mode::kScored ? plo - t0 : -(1 << 30));
                 const int vhi = (text ? thi : phi) - t0;
                 // warp-uniform outcome: the TMEM instructions below need the whole warp
                 if (!__all_sync(0xffffffffu, mbar_wait_bounded(s_full(b), par, p.status, p.wait_limit))) { ok = false; break; }
@@ -527,7 +650,11 @@ rswa_prefill_tc_kernel(const PrefillParams p, const __grid_constant__ PrefillMap
                 const float* other_max = xmax + (b * 2 + (h ^ 1)) * 128 + r;
                 float alpha = 1.f;
                 const bool full = __all_sync(0xffffffffu, vlo <= 0 && vhi >= kTcTile);
-                ok = tc_softmax_half(full, tS, h, vlo, vhi, my_max, other_max, pair_bar(quad), pp & 1u, p.status, p.wait_limit, m_ref, l_run, alpha);
+                if constexpr (Mode::kScored)
+                    ok = tc_softmax_half<Mode>(full, tS, h, vlo, vhi, my_max, other_max, pair_bar(quad), pp & 1u, p.status, p.wait_limit, m_ref, l_run, alpha,
+                                               p.score_mul, p.cap_log2, slope_log2, (float)((long long)(text ? i : q_pos) - t0 - h * 64));
+                else
+                    ok = tc_softmax_half<Mode>(full, tS, h, vlo, vhi, my_max, other_max, pair_bar(quad), pp & 1u, p.status, p.wait_limit, m_ref, l_run, alpha);
                 ++pp;
                 if (!ok) break;
                 // A row whose reference moved takes the factor on its accumulator before this tile's product is
@@ -563,8 +690,10 @@ rswa_prefill_tc_kernel(const PrefillParams p, const __grid_constant__ PrefillMap
             if (!it.valid) return;
             ++fetched;
             if (r < it.t.rows) {
-                mbar_arrive_expect_tx(q_landed, 512u);
-                bulk_copy_g2s(my_row_s, p.q + ((size_t)(it.t.row0 + r) * p.heads + it.head) * kTcTile, 512u, q_landed);
+                constexpr uint32_t kRowBytes = Mode::kPairQ ? 512u : 256u;  // fp32 or bf16 queries
+                mbar_arrive_expect_tx(q_landed, kRowBytes);
+                bulk_copy_g2s(my_row_s, reinterpret_cast<const uint8_t*>(p.q) + ((size_t)(it.t.row0 + r) * p.heads + it.head) * kRowBytes, kRowBytes,
+                              q_landed);
             } else {
                 mbar_arrive(q_landed);
             }
@@ -573,16 +702,34 @@ rswa_prefill_tc_kernel(const PrefillParams p, const __grid_constant__ PrefillMap
         auto convert_q = [&](const TcItem& it, uint32_t m) -> bool {
             if (!__all_sync(0xffffffffu, mbar_wait_bounded(q_landed, m & 1u, p.status, p.wait_limit))) return false;
             const bool live = r < it.t.rows;
-            const float s = p.scale_log2e;
+            if constexpr (!Mode::kPairQ) {  // bf16 queries are the operand already
+                const uint4* w4 = reinterpret_cast<const uint4*>(my_row);
+#pragma unroll 1
+                for (int g4 = 0; g4 < 4; ++g4) {
+                    uint32_t w[16];
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        const uint4 v = live ? w4[g4 * 4 + c] : make_uint4(0u, 0u, 0u, 0u);
+                        w[4 * c] = v.x; w[4 * c + 1] = v.y; w[4 * c + 2] = v.z; w[4 * c + 3] = v.w;
+                    }
+                    tc_st16(tmem + lane_base + kTcColQ + g4 * 16, w);
+                }
+            }
+            const float s = Mode::kScored ? 1.f : p.scale_log2e;
             const float4* q4 = reinterpret_cast<const float4*>(my_row);
 #pragma unroll 1
-            for (int g4 = 0; g4 < 4; ++g4) {  // 32 dims at a time: 16 hi words and 16 lo words (rolled: this runs once per item)
+            for (int g4 = 0; Mode::kPairQ && g4 < 4; ++g4) {  // 32 dims at a time: 16 hi words and 16 lo words (rolled: this runs once per item)
                 uint32_t hi[16], lo[16];
 #pragma unroll
                 for (int c = 0; c < 8; ++c) {
                     const float4 v = live ? q4[g4 * 8 + c] : make_float4(0.f, 0.f, 0.f, 0.f);
-                    tc_split2(v.x * s, v.y * s, hi[2 * c], lo[2 * c]);
-                    tc_split2(v.z * s, v.w * s, hi[2 * c + 1], lo[2 * c + 1]);
+                    if constexpr (Mode::kScored) {
+                        tc_split2_rn(v.x, v.y, hi[2 * c], lo[2 * c]);
+                        tc_split2_rn(v.z, v.w, hi[2 * c + 1], lo[2 * c + 1]);
+                    } else {
+                        tc_split2(v.x * s, v.y * s, hi[2 * c], lo[2 * c]);
+                        tc_split2(v.z * s, v.w * s, hi[2 * c + 1], lo[2 * c + 1]);
+                    }
                 }
                 tc_st16(tmem + lane_base + kTcColQ + g4 * 16, hi);
                 tc_st16(tmem + lane_base + kTcColQ + 64 + g4 * 16, lo);
@@ -630,7 +777,15 @@ rswa_prefill_tc_kernel(const PrefillParams p, const __grid_constant__ PrefillMap
                     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                     mbar_arrive(o_read);
                 }
-                if (p.out_bf16) {
+                if (Mode::kScored && p.out_bf16) {
+                    uint4* so = reinterpret_cast<uint4*>(my_row) + hh * 8;
+#pragma unroll
+                    for (int c = 0; c < 8; ++c)
+                        so[c] = make_uint4(rn_bf16x2(__uint_as_float(o[8 * c]) * inv, __uint_as_float(o[8 * c + 1]) * inv),
+                                           rn_bf16x2(__uint_as_float(o[8 * c + 2]) * inv, __uint_as_float(o[8 * c + 3]) * inv),
+                                           rn_bf16x2(__uint_as_float(o[8 * c + 4]) * inv, __uint_as_float(o[8 * c + 5]) * inv),
+                                           rn_bf16x2(__uint_as_float(o[8 * c + 6]) * inv, __uint_as_float(o[8 * c + 7]) * inv));
+                } else if (p.out_bf16) {
                     uint4* so = reinterpret_cast<uint4*>(my_row) + hh * 8;
 #pragma unroll
                     for (int c = 0; c < 8; ++c)
@@ -704,6 +859,7 @@ rswa_prefill_tc_kernel(const PrefillParams p, const __grid_constant__ PrefillMap
                 reinterpret_cast<int4*>(w)[0] = a;                                        // row0 rows slot kind
                 reinterpret_cast<int4*>(w)[1] = make_int4(b4.x, b4.y, (int)(k_next - (long long)ti * p.heads), b4.z);  // pos0 block0 head pfx
                 reinterpret_cast<int4*>(w)[2] = make_int4(b4.w, c.x, c.y, 1);             // n_prefix_tiles text_tile0 n_steps valid
+                if constexpr (Mode::kScored) reinterpret_cast<int4*>(w)[3] = make_int4(c.z, c.w, 0, 0);  // fixed_lo fixed_hi
             } else {
                 w[11] = 0;
                 more = false;
@@ -731,17 +887,25 @@ rswa_prefill_tc_kernel(const PrefillParams p, const __grid_constant__ PrefillMap
                 const uint32_t full = is_v ? v_full(b) : k_full(b), freed = is_v ? v_free(b) : k_free(b);
                 if (gn >= 2 && !__all_sync(0xffffffffu, mbar_wait_bounded(freed, ((gn >> 1) - 1) & 1u, p.status, p.wait_limit))) { ok = false; break; }
                 const bool text = n >= it.n_prefix_tiles;
-                const int t0 = text ? (it.text_tile0 + n - it.n_prefix_tiles) * kTcTile : n * kTcTile;
+                const int t0 = first_token(it, n);
                 const int idx = t0 / kBlockTokens + blk_i;  // block index within the request's region
+                int span_lo = 0, span_hi = kTcTile;
+                bool block_seen = true;  // some row sees a token of this lane's block
+                if constexpr (Mode::kScored) {
+                    tile_span(it, text, t0, span_lo, span_hi);
+                    block_seen = (blk_i + 1) * kBlockTokens > span_lo && blk_i * kBlockTokens < span_hi;
+                }
                 int y;
                 const CUtensorMap* map;
                 if (text) {
                     const int blk = it.t.block0 + idx;
-                    y = blk < p.text_blocks ? (blk * p.kv_heads + it.kvh) * kBlockTokens : text_rows;
+                    if (Mode::kScored && block_seen && (blk < 0 || blk >= p.text_blocks)) atomicOr(p.status, kStatusBadBlock);
+                    y = block_seen && blk >= 0 && blk < p.text_blocks ? (blk * p.kv_heads + it.kvh) * kBlockTokens : text_rows;
                     map = is_v ? &maps.tv : &maps.tk;
                 } else {
                     y = pool_rows;
-                    if (idx < prefix_blocks && idx < p.table_stride) {
+                    if (Mode::kScored && block_seen && idx >= p.table_stride) atomicOr(p.status, kStatusBadSlot);
+                    if (block_seen && idx < prefix_blocks && idx < p.table_stride) {
                         const int blk = __ldg(p.table + (size_t)it.t.slot * p.table_stride + idx);
                         if (blk < 0 || blk >= p.num_blocks)
                             atomicOr(p.status, kStatusBadBlock);
@@ -755,6 +919,24 @@ rswa_prefill_tc_kernel(const PrefillParams p, const __grid_constant__ PrefillMap
                 const uint32_t dst = smem_addr(sKV) + b * kTcStageBytes + is_v * kTcTileBytes + half * kTcHalfBytes + blk_i * 2048;
                 if (lane < 16) tma_load_box(dst, map, half * 64, y, full);
                 issued = gn + 1;
+                // V outside the span of keys that the tile's rows see may hold anything (the unwritten end of a block,
+                // another page), and zero times a NaN is a NaN: whole blocks were not fetched, the rows of a block that the
+                // span cuts are zeroed before the product reads them.
+                if constexpr (Mode::kScored) {
+                    if (is_v && cuts_block(span_lo, span_hi)) {
+                        if (!__all_sync(0xffffffffu, mbar_wait_bounded(full, (gn >> 1) & 1u, p.status, p.wait_limit))) { ok = false; break; }
+                        uint8_t* tile_v = sKV + b * kTcStageBytes + kTcTileBytes;
+                        auto zero_rows = [&](int from, int to) {  // tokens of the tile; 2 halves of 128 bytes each
+                            for (int c = lane; c < (to - from) * 16; c += 32)
+                                *reinterpret_cast<uint4*>(tile_v + ((c >> 3) & 1) * kTcHalfBytes + (from + (c >> 4)) * 128 + (c & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+                        };
+                        if (span_lo > 0) zero_rows(span_lo & ~(kBlockTokens - 1), span_lo);
+                        if (span_hi < kTcTile) zero_rows(span_hi, (span_hi + kBlockTokens - 1) & ~(kBlockTokens - 1));
+                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(v_clean(b));
+                    }
+                }
             }
             g += it.n_steps;
         }
@@ -790,7 +972,7 @@ rswa_prefill_tc_kernel(const PrefillParams p, const __grid_constant__ PrefillMap
                     const uint32_t tS = tmem + b * 128;
                     // Q: 16 dims = 8 TMEM columns per MMA, 64 columns of hi words, then 64 of lo words
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) tc_mma_ts(tS, tmem + kTcColQ + 8 * j, dK[j & 7] + stage, idesc_s, (uint32_t)j);
+                    for (int j = 0; j < (Mode::kPairQ ? 16 : 8); ++j) tc_mma_ts(tS, tmem + kTcColQ + 8 * j, dK[j & 7] + stage, idesc_s, (uint32_t)j);
                     tc_commit(s_full(b));
                     tc_commit(k_free(b));
                 }
@@ -810,6 +992,7 @@ rswa_prefill_tc_kernel(const PrefillParams p, const __grid_constant__ PrefillMap
             for (int j = 0; j < 8; ++j)  // V is [key][dim]: MN-major B operand; 64-dim halves are 16 KB apart (LBO), 8-key groups 1 KB (SBO)
                 dV[j] = tc_smem_desc(smem_addr(sKV) + kTcTileBytes + j * 2048, kTcHalfBytes, 1024);
             uint32_t g = 0, m = 0;
+            uint32_t cleaned = 0;  // bit b: parity of the next phase of v_clean(b)
             bool ok = true;
             for (TcItem it = get_item_1(0); it.valid && ok; it = get_item_1(++m)) {
                 // the item's first product overwrites the accumulator: the previous item's rows must have been read
@@ -817,6 +1000,14 @@ rswa_prefill_tc_kernel(const PrefillParams p, const __grid_constant__ PrefillMap
                 for (int n = 0; n < it.n_steps; ++n) {
                     const uint32_t gn = g + n, b = gn & 1u;
                     if (!mbar_wait_bounded(v_full(b), (gn >> 1) & 1u, p.status, p.wait_limit)) { ok = false; break; }
+                    if constexpr (Mode::kScored) {
+                        int lo, hi;
+                        tile_span(it, n >= it.n_prefix_tiles, first_token(it, n), lo, hi);
+                        if (cuts_block(lo, hi)) {
+                            if (!mbar_wait_bounded(v_clean(b), (cleaned >> b) & 1u, p.status, p.wait_limit)) { ok = false; break; }
+                            cleaned ^= 1u << b;
+                        }
+                    }
                     if (!mbar_wait_bounded(p_full(b), (gn >> 1) & 1u, p.status, p.wait_limit)) { ok = false; break; }
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                     const uint64_t stage = (uint64_t)(b * (kTcStageBytes >> 4));
@@ -824,10 +1015,15 @@ rswa_prefill_tc_kernel(const PrefillParams p, const __grid_constant__ PrefillMap
                     // P: 16 keys = 8 TMEM columns per MMA; every 32 keys hold their 16 hi words, then their 16 lo words.
                     // The accumulator carries over from tile to tile (the item's first product overwrites it).
                     tc_mma_ts(tO, tP, dV[0] + stage, idesc_o, (uint32_t)n);
+                    if constexpr (Mode::kPairP) {
 #pragma unroll
-                    for (int u = 1; u < 16; ++u) {
-                        const int hp = u >> 3, j = u & 7;
-                        tc_mma_ts(tO, tP + (j >> 1) * 32 + hp * 16 + (j & 1) * 8, dV[j] + stage, idesc_o, 1u);
+                        for (int u = 1; u < 16; ++u) {
+                            const int hp = u >> 3, j = u & 7;
+                            tc_mma_ts(tO, tP + (j >> 1) * 32 + hp * 16 + (j & 1) * 8, dV[j] + stage, idesc_o, 1u);
+                        }
+                    } else {  // every 64 keys hold 32 words, then 32 unused columns
+#pragma unroll
+                        for (int j = 1; j < 8; ++j) tc_mma_ts(tO, tP + (j >> 2) * 64 + (j & 3) * 8, dV[j] + stage, idesc_o, 1u);
                     }
                     tc_commit(o_full(b));
                     tc_commit(v_free(b));
@@ -850,5 +1046,11 @@ rswa_prefill_tc_kernel(const PrefillParams p, const __grid_constant__ PrefillMap
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
     }
 }
+
+// Host side (rswa_c_api.cu): the tensor map of a K or V pool, and the tile plan of a workspace -- with the visible
+// ranges of `score`, or, where that is null, causal / whole-region rows.
+int make_kv_map(CUtensorMap* map, const void* pool, long rows);
+int prefill_plan(const uocr_b200_prefill_tile* h_tiles, int n_tiles, const int* d_prefill_len, int window, const uocr_b200_score* score,
+                 uocr_b200_workspace* ws, cudaStream_t st, const char* who);
 
 }  // namespace uocr_b200

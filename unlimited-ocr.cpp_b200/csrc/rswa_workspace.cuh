@@ -82,6 +82,7 @@ struct uocr_b200_workspace {
     int plan_tiles = 0;            // tiles of the plan in tile_work (0: none)
     int plan_window = 0;
     bool plan_any_text = false;
+    bool plan_scored = false;      // made for visible ranges (the call with modified scores)
     unsigned plan_serial = 0;      // plans made on this workspace so far
     int tiles_cap = 0;
     bool out_bf16 = false;  // attention results are written as bf16 instead of fp32
