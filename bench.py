@@ -458,7 +458,7 @@ def kernel_source_sha():
     """Hash of the sources the dominant kernel is compiled from; ties an ncu traffic record to the code."""
     import hashlib
     h = hashlib.sha256()
-    for f in ("rswa_attention.cuh", "rswa_device.cuh"):
+    for f in ("rswa_attention.cuh", "rswa_split.cuh", "rswa_device.cuh"):
         h.update(open(os.path.join(ROOT, "unlimited-ocr.cpp_b200", "csrc", f), "rb").read())
     return h.hexdigest()[:16]
 
