@@ -206,10 +206,17 @@ def _p(t):
     return t.ctypes.data
 
 
+_current_raw_stream = None  # torch's raw handle of a device's current stream, without building a Stream object
+
+
 def stream_handle(stream=None):
+    if stream is not None:
+        return stream.cuda_stream
+    global _current_raw_stream
     import torch
-    s = stream if stream is not None else torch.cuda.current_stream()
-    return s.cuda_stream
+    if _current_raw_stream is None:
+        _current_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda d: torch.cuda.current_stream(d).cuda_stream)
+    return _current_raw_stream(torch.cuda.current_device())
 
 
 class Workspace:
@@ -514,48 +521,67 @@ class Rope:
             pass
 
 
+def _dp(t):
+    """Device address of a tensor / None (the light form of _p for calls that are short themselves)."""
+    return None if t is None else t.data_ptr()
+
+
 def _dtype_of(t):
     import torch
-    if t.dtype == torch.float32:
+    dt = t.dtype
+    if dt is torch.float32:
         return F32
-    if t.dtype == torch.bfloat16:
+    if dt is torch.bfloat16:
         return BF16
-    raise ValueError(f"rows must be float32 or bfloat16, got {t.dtype}")
+    raise ValueError(f"rows must be float32 or bfloat16, got {dt}")
 
 
-def _qkv_rows(q, k, v, q_out, heads):
-    """Packed rows, [rows, width] each with its own row stride and contiguous elements."""
+def _row_stride(t, ref, n):
+    """Elements between the rows of t: a [n, width] matrix of ref's type with contiguous rows."""
+    if t.dtype is not ref.dtype or t.size(0) != n or t.stride(1) != 1:
+        raise ValueError("rows must have one type and count, and contiguous elements")
+    return t.stride(0) if n > 1 else max(t.stride(0), t.size(1))
+
+
+def _qkv_rows(q, k, v, q_out, heads, n):
+    """Packed rows, [n, width] each with its own row stride."""
     ref = q if q is not None else k
-    for t in (q, k, v, q_out):
-        if t is not None and (t.dtype != ref.dtype or t.shape[0] != ref.shape[0] or t.stride(1) != 1 or t.device != ref.device):
-            raise ValueError("q, k, v and q_out must have one type, row count and device, and contiguous rows")
-    s = lambda t: 0 if t is None else (t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1]))
-    return QkvRows(_p(q), _p(k), _p(v), _p(q_out), s(q), s(k), s(v), s(q_out), _dtype_of(ref), heads)
+    r = QkvRows()
+    r.dtype, r.heads = _dtype_of(ref), heads
+    if q is not None:
+        r.q, r.q_stride = q.data_ptr(), _row_stride(q, ref, n)
+        if q_out is not None:
+            r.q_out, r.q_out_stride = q_out.data_ptr(), _row_stride(q_out, ref, n)
+    if k is not None:
+        r.k, r.k_stride = k.data_ptr(), _row_stride(k, ref, n)
+        if v is not None:
+            r.v, r.v_stride = v.data_ptr(), _row_stride(v, ref, n)
+    return r
 
 
 def rope_rows(rope, q, k, q_out, k_out, d_positions, heads, kv_heads, head_dim, stream=None):
     """Rotates the packed rows of q and k (either may be None with 0 heads; outputs may be the inputs)."""
-    rows = _qkv_rows(q, k, None, q_out, heads)
-    if k_out is not None and (k_out.dtype != k.dtype or k_out.stride(1) != 1 or k_out.shape != k.shape):
-        raise ValueError("k_out must have k's type and shape, and contiguous rows")
-    check(lib().uocr_b200_rswa_rope_rows(rope.h, C.byref(rows), _p(k_out), k_out.stride(0) if k_out is not None else 0, _p(d_positions),
-                                         (q if q is not None else k).shape[0], kv_heads, head_dim, stream_handle(stream)))
+    n = (q if q is not None else k).size(0)
+    rows = _qkv_rows(q, k, None, q_out, heads, n)
+    check(lib().uocr_b200_rswa_rope_rows(rope.h, rows, _dp(k_out), _row_stride(k_out, k, n) if k_out is not None else 0, d_positions.data_ptr(),
+                                         n, kv_heads, head_dim, stream_handle(stream)))
 
 
 def rope_write_prefill_paged(layer, rope, q, k, v, q_out, d_positions, d_slots, d_pos, heads, ws=None, stream=None):
     """rope + write_prefill_ragged_paged in one pass."""
-    rows = _qkv_rows(q, k, v, q_out, heads)
-    check(lib().uocr_b200_rswa_rope_write_prefill_paged(layer.ref(), rope.h, C.byref(rows), _p(d_positions), _p(d_slots), _p(d_pos),
-                                                        k.shape[0], ws.h if ws else None, stream_handle(stream)))
+    n = k.size(0)
+    check(lib().uocr_b200_rswa_rope_write_prefill_paged(
+        layer.desc, rope.h, _qkv_rows(q, k, v, q_out, heads, n), d_positions.data_ptr(), d_slots.data_ptr(), d_pos.data_ptr(), n,
+        ws.h if ws else None, stream_handle(stream)))
 
 
 def rope_append_decode_batch_paged(layer, rope, q, k, v, q_out, d_positions, d_len, d_ring, d_prefill, d_slots, window, heads, ws=None,
                                    stream=None):
     """rope + append_decode_batch_paged in one pass."""
-    rows = _qkv_rows(q, k, v, q_out, heads)
-    check(lib().uocr_b200_rswa_rope_append_decode_batch_paged(layer.ref(), rope.h, C.byref(rows), _p(d_positions), _p(d_len), _p(d_ring),
-                                                              _p(d_prefill), _p(d_slots), k.shape[0], window, ws.h if ws else None,
-                                                              stream_handle(stream)))
+    n = k.size(0)
+    check(lib().uocr_b200_rswa_rope_append_decode_batch_paged(
+        layer.desc, rope.h, _qkv_rows(q, k, v, q_out, heads, n), d_positions.data_ptr(), d_len.data_ptr(), d_ring.data_ptr(), d_prefill.data_ptr(),
+        d_slots.data_ptr(), n, window, ws.h if ws else None, stream_handle(stream)))
 
 
 # ---- attention with modified scores --------------------------------------------------------------------
@@ -591,29 +617,29 @@ class Mass:
 def attention_scored_batch_paged(layer, score, q, d_len, d_ring, d_prefill, d_slots, batch, window, heads, out, ws, mass=None, stream=None):
     """Decode attention with modified scores; `mass` also accumulates the attention weights."""
     check(lib().uocr_b200_rswa_attention_scored_batch_paged(
-        layer.ref(), C.byref(score.desc), _p(q), _dtype_of(q), _p(d_len), _p(d_ring), _p(d_prefill), _p(d_slots), batch, window, heads,
-        _p(out), C.byref(mass.desc) if mass is not None else None, ws.h, stream_handle(stream)))
+        layer.desc, score.desc, _dp(q), _dtype_of(q), _dp(d_len), _dp(d_ring), _dp(d_prefill), _dp(d_slots), batch, window, heads,
+        _dp(out), C.addressof(mass.desc) if mass is not None else None, ws.h, stream_handle(stream)))
 
 
 def attention_scored_ragged_paged(layer, score, q, d_prefill, d_slots, d_pos, total, heads, out, ws, stream=None):
     """Packed vision rows with modified scores, any geometry."""
-    check(lib().uocr_b200_rswa_attention_scored_ragged_paged(layer.ref(), C.byref(score.desc), _p(q), _dtype_of(q), _p(d_prefill), _p(d_slots),
-                                                             _p(d_pos), total, heads, _p(out), ws.h, stream_handle(stream)))
+    check(lib().uocr_b200_rswa_attention_scored_ragged_paged(layer.desc, score.desc, _dp(q), _dtype_of(q), _dp(d_prefill), _dp(d_slots),
+                                                             _dp(d_pos), total, heads, _dp(out), ws.h, stream_handle(stream)))
 
 
 def prefill_text_scored_paged(layer, text_k, text_v, text_blocks, score, q, d_prefill, d_slots, d_pos, d_block0, total, window, heads, out, ws,
                               stream=None):
     """Packed text rows over prefix + text window with modified scores, any geometry (K and V already in the text pool)."""
-    check(lib().uocr_b200_rswa_prefill_text_scored_paged(layer.ref(), _p(text_k), _p(text_v), text_blocks, C.byref(score.desc), _p(q),
-                                                         _dtype_of(q), _p(d_prefill), _p(d_slots), _p(d_pos), _p(d_block0), total, window,
-                                                         heads, _p(out), ws.h, stream_handle(stream)))
+    check(lib().uocr_b200_rswa_prefill_text_scored_paged(layer.desc, _dp(text_k), _dp(text_v), text_blocks, score.desc, _dp(q),
+                                                         _dtype_of(q), _dp(d_prefill), _dp(d_slots), _dp(d_pos), _dp(d_block0), total, window,
+                                                         heads, _dp(out), ws.h, stream_handle(stream)))
 
 
 def prefill_plan_scored_tc(score, tiles, d_prefill, window, ws, stream=None):
     """Uploads and orders the query tiles for the score's visible ranges; later calls with reuse_plan=True share the plan."""
     import numpy as np
     t = np.ascontiguousarray(tiles, dtype=np.int32)
-    check(lib().uocr_b200_rswa_prefill_plan_scored_tc(C.byref(score.desc), t.ctypes.data, t.shape[0], _p(d_prefill), window, ws.h, stream_handle(stream)))
+    check(lib().uocr_b200_rswa_prefill_plan_scored_tc(score.desc, t.ctypes.data, t.shape[0], _dp(d_prefill), window, ws.h, stream_handle(stream)))
 
 
 def prefill_attention_scored_tc(layer, text_k, text_v, text_blocks, score, q, d_prefill, tiles, window, heads, out, ws, stream=None, reuse_plan=False):
@@ -621,23 +647,23 @@ def prefill_attention_scored_tc(layer, text_k, text_v, text_blocks, score, q, d_
     import numpy as np
     t = np.ascontiguousarray(tiles, dtype=np.int32)
     check(lib().uocr_b200_rswa_prefill_attention_scored_tc(
-        layer.ref(), _p(text_k), _p(text_v), text_blocks, C.byref(score.desc), _p(q), _dtype_of(q), _p(d_prefill),
-        None if reuse_plan else t.ctypes.data, t.shape[0], window, heads, _p(out), ws.h, stream_handle(stream)))
+        layer.desc, _dp(text_k), _dp(text_v), text_blocks, score.desc, _dp(q), _dtype_of(q), _dp(d_prefill),
+        None if reuse_plan else t.ctypes.data, t.shape[0], window, heads, _dp(out), ws.h, stream_handle(stream)))
 
 
 # ---- eviction from the fixed region ----------------------------------------------------------------------
 
 def evict_select(mass, d_prefill, d_slots, n, keep, sinks, recent, d_keep, d_keep_len, ws=None, stream=None):
     """The `keep` heaviest tokens of each slot's fixed region, ascending: d_keep int32 [n, keep], d_keep_len int32 [n]."""
-    check(lib().uocr_b200_rswa_evict_select(_p(mass), mass.shape[1], _p(d_prefill), _p(d_slots), n, keep, sinks, recent, _p(d_keep),
-                                            _p(d_keep_len), ws.h if ws else None, stream_handle(stream)))
+    check(lib().uocr_b200_rswa_evict_select(_dp(mass), mass.size(1), _dp(d_prefill), _dp(d_slots), n, keep, sinks, recent, _dp(d_keep),
+                                            _dp(d_keep_len), ws.h if ws else None, stream_handle(stream)))
 
 
 def evict_compact_paged_layers(layers, d_prefill, d_slots, n, d_keep, d_keep_len, d_new_blocks=None, ws=None, stream=None):
     """Moves the kept rows of every layer to the new blocks (None: in place).  layers: PagedLayers, or their layer_array."""
     arr = layers if isinstance(layers, C.Array) else layer_array(layers)
     check(lib().uocr_b200_rswa_evict_compact_paged_layers(
-        arr, len(arr), _p(d_prefill), _p(d_slots), n, _p(d_keep), d_keep.shape[1], _p(d_keep_len), _p(d_new_blocks),
+        arr, len(arr), _dp(d_prefill), _dp(d_slots), n, _dp(d_keep), d_keep.size(1), _dp(d_keep_len), _dp(d_new_blocks),
         d_new_blocks.shape[1] if d_new_blocks is not None else 0, ws.h if ws else None, stream_handle(stream)))
 
 
@@ -646,6 +672,6 @@ def evict_publish(table, d_slots, n, d_keep, d_keep_len, d_len, d_prefill, windo
     """Puts the new regions in force: table rows, d_len [layers, slots], d_prefill, and the per-token arrays."""
     width = lambda t: t.shape[1] if t is not None else 0
     check(lib().uocr_b200_rswa_evict_publish(
-        _p(table), table.shape[1], _p(d_slots), n, _p(d_keep), d_keep.shape[1], _p(d_keep_len), _p(d_new_blocks), width(d_new_blocks), _p(d_len),
-        d_len.stride(0), d_len.shape[0], _p(d_prefill), window, _p(mass), width(mass), _p(d_key_pos), width(d_key_pos),
+        _dp(table), table.shape[1], _dp(d_slots), n, _dp(d_keep), d_keep.size(1), _dp(d_keep_len), _dp(d_new_blocks), width(d_new_blocks), _dp(d_len),
+        d_len.stride(0), d_len.shape[0], _dp(d_prefill), window, _dp(mass), width(mass), _dp(d_key_pos), width(d_key_pos),
         ws.h if ws else None, stream_handle(stream)))

@@ -8,11 +8,12 @@
 // integer multiply, good to 2^-33 turns for any 32-bit position.  What is left after the quadrant is taken
 // off is at most an eighth of a turn and goes to sincospi in fp32.
 //
-// The kernel moves bytes (q, k, v in; q and the pool rows out) and is bound by HBM.  A CTA takes four rows
-// at a time: 256 threads first fill the rows' cosine / sine table in shared memory (one entry per pair of
-// one head, used by all heads), then run over the rows' 16-byte chunks.  In the half layout a thread owns
-// a chunk and its partner rotary_dim / 2 further on, in the interleaved layout a chunk holds whole pairs;
-// every element is read and written by one thread, so a call may work in place.
+// The kernel moves bytes (q, k, v in; q and the pool rows out) and is bound by HBM, which takes few instructions a chunk and
+// loads in flight with nothing to wait on.  A warp takes a row, or a share of its heads.  A lane keeps one 16-byte chunk position
+// of a head and walks over the heads: the position's cosines and sines stay in registers, the loads of a batch of heads start
+// before anything else, the warp's table of the row's angles (one entry per pair of one head) is filled meanwhile.  In the half
+// layout a lane owns a chunk and its partner rotary_dim / 2 further on, in the interleaved layout a chunk holds whole pairs; every
+// element is read and written by one lane, so a call may work in place.
 #pragma once
 
 #include "rswa_paged.cuh"
@@ -24,16 +25,10 @@ constexpr int kRopeThreads = 256;
 
 enum RopeMode : int { kRopeRows = 0, kRopeWrite = 1, kRopeAppend = 2 };
 
-// n / d for n * d < 2^32, as a multiply
-struct FastDiv {
-    uint32_t d, m;
-};
-__device__ __forceinline__ uint32_t fast_div(uint32_t n, const FastDiv& f) { return f.d == 1 ? n : __umulhi(n, f.m); }
-
 struct RopeParams {
     unsigned long long turn[kRopeMaxPairs];  // freq_i / 2 pi in units of 2^-64 turns
     float amplitude;
-    int interleaved, rotary_dim;
+    int rotary_dim;
     const void* q;
     const void* k;
     const void* v;
@@ -50,8 +45,9 @@ struct RopeParams {
     int window;
     PagedView pv;
     int* status;
-    int rows_per_cta;
-    FastDiv per_row, per_head, per_v;  // work items of a row, of a rotated head, of a head of v
+    int parts_log2;  // 2^x warps share a row
+    int per_head;    // chunks of a rotated head a lane each (half layout: a chunk and its partner are one), or elements / pairs
+    int items;       // element by element: items of a row
 };
 
 __device__ __forceinline__ void rope_sincos(unsigned long long turn, int position, float& sn, float& cs) {
@@ -71,19 +67,6 @@ __device__ __forceinline__ void rope_turn(float& x0, float& x1, float2 t) {
     const float y = __fmaf_rn(x0, t.x, -__fmul_rn(x1, t.y));
     x1 = __fmaf_rn(x0, t.y, __fmul_rn(x1, t.x));
     x0 = y;
-}
-
-template <typename T>
-__device__ __forceinline__ void load8(const void* base, long long at, float (&f)[8]) {
-    if constexpr (T::kBytes == 2) {
-        const uint4 w = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(base) + at);
-        T::unpack(w, f);
-    } else {
-        const float4 a = *reinterpret_cast<const float4*>(static_cast<const float*>(base) + at);
-        const float4 b = *reinterpret_cast<const float4*>(static_cast<const float*>(base) + at + 4);
-        f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w;
-        f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
-    }
 }
 
 template <typename T>
@@ -108,148 +91,258 @@ __device__ __forceinline__ void store1(void* base, long long at, float f) {
     else static_cast<float*>(base)[at] = f;
 }
 
-// ROW: type of the q / k / v rows, KV: of the pool (ROW again where nothing goes to the pool).
-// VEC: every chunk of 8 elements is 16-byte aligned and lies in one half of the rotated dims; otherwise element by element.
-template <typename ROW, typename KV, int MODE, bool VEC>
-__global__ void __launch_bounds__(kRopeThreads) rswa_rope_kernel(const __grid_constant__ RopeParams p) {
-    constexpr int kMaxRows = 4;
-    __shared__ float2 cs[kMaxRows * kRopeMaxPairs];
-    __shared__ int s_blk[kMaxRows], s_off[kMaxRows];
-    const int tid = threadIdx.x;
-    const int half = p.rotary_dim >> 1, hd = p.head_dim;
-    const int rotated = (p.heads + p.kv_heads) * (int)p.per_head.d;
+// Where row `row` goes in the pool: block (-1: nowhere) and token of the block.
+template <int MODE>
+__device__ __forceinline__ void rope_write_place(const RopeParams& p, int row, int& blk, int& off) {
+    const int slot = __ldg(p.d_slots + row), at = __ldg(p.d_pos + row);
+    blk = -1;
+    off = at & (kBlockTokens - 1);
+    if (at >= 0 && at / kBlockTokens < p.pv.table_stride) {
+        blk = __ldg(p.pv.table + (size_t)slot * p.pv.table_stride + at / kBlockTokens);
+        if (blk < 0 || blk >= p.pv.num_blocks) {
+            if (p.status) atomicOr(p.status, kStatusBadBlock);
+            blk = -1;
+        }
+    } else if (p.status) {
+        atomicOr(p.status, kStatusBadSlot);
+    }
+}
 
-    for (int row0 = blockIdx.x * p.rows_per_cta; row0 < p.rows; row0 += gridDim.x * p.rows_per_cta) {
-        const int nrows = min(p.rows_per_cta, p.rows - row0);
-        if constexpr (MODE == kRopeAppend) {  // one row per CTA
-            const int slot = __ldg(p.d_slots + row0);
-            bool again = false;  // an earlier row of the batch appends to this slot: one token per slot and call
-            for (int j = tid; j < row0; j += kRopeThreads) again |= __ldg(p.d_slots + j) == slot;
-            again = __syncthreads_or(again);
-            if (tid == 0) {
-                int blk = -1, off = 0;
-                if (again) {
-                    if (p.status) atomicOr(p.status, kStatusBadSlot);
+// The append of row `row`, block-wide: one token per slot and call, for the first row that names the slot.  Thread 0 gets the place.
+__device__ __forceinline__ void rope_append_place(const RopeParams& p, int row, int& blk, int& off) {
+    const int slot = __ldg(p.d_slots + row);
+    bool again = false;
+    for (int j = threadIdx.x; j < row; j += blockDim.x) again |= __ldg(p.d_slots + j) == slot;
+    again = __syncthreads_or(again);
+    blk = -1;
+    off = 0;
+    if (threadIdx.x != 0) return;
+    if (again) {
+        if (p.status) atomicOr(p.status, kStatusBadSlot);
+        return;
+    }
+    const int pfx = __ldg(p.d_prefill_len + slot);
+    const int ring = ring_advance(p.d_len + slot, p.d_ring_pos + slot, pfx, p.window) - pfx;
+    const int entry = (pfx + kBlockTokens - 1) / kBlockTokens + ring / kBlockTokens;
+    off = ring & (kBlockTokens - 1);
+    if (ring >= 0 && entry < p.pv.table_stride) blk = __ldg(p.pv.table + (size_t)slot * p.pv.table_stride + entry);
+    else if (p.status) atomicOr(p.status, kStatusBadSlot);
+    if (blk < 0 || blk >= p.pv.num_blocks) {
+        if (p.status) atomicOr(p.status, kStatusBadBlock);
+        blk = -1;
+    }
+}
+
+// ROW: type of the q / k / v rows, KV: of the pool (ROW again where nothing goes to the pool).  Every chunk of 8 elements is
+// 16-byte aligned and, in the half layout, lies in one half of the rotated dims.  Append: one row per CTA, 8 warps to a row.
+template <typename ROW, typename KV, int MODE, bool INTERLEAVED>
+__global__ void __launch_bounds__(kRopeThreads, 4) rswa_rope_kernel(const __grid_constant__ RopeParams p) {
+    constexpr int W = ROW::kBytes / 2;               // 16-byte words of a chunk
+    constexpr int U = INTERLEAVED ? 4 / W : 2 / W;   // heads of a batch: 64 bytes of loads a lane
+    constexpr int T = INTERLEAVED ? 4 : 8;           // pairs a lane's chunk takes part in
+    __shared__ float2 tables[kRopeThreads / 32][kRopeMaxPairs];
+    __shared__ int s_place[2];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int half = p.rotary_dim >> 1, hd = p.head_dim, per_head = p.per_head;
+    const int parts = 1 << p.parts_log2, n_rot = p.heads + p.kv_heads;
+    float2* tab = tables[warp];
+    // This lane's chunk of a head and its first head: 32 / per_head heads side by side, wider heads in rounds of 32 chunks.
+    const int abreast = per_head < 32 ? 32 / per_head : 1;
+    const int my_head = per_head < 32 ? lane / per_head : 0;
+    const int my_chunk = per_head < 32 ? lane - my_head * per_head : lane;
+
+    const long long units = (long long)p.rows << p.parts_log2;
+    for (long long unit = (long long)blockIdx.x * (kRopeThreads / 32) + warp; unit < units; unit += (long long)gridDim.x * (kRopeThreads / 32)) {
+        const int row = (int)(unit >> p.parts_log2), part = (int)(unit & (parts - 1));
+        const uint8_t* q_row = static_cast<const uint8_t*>(p.q) + row * p.q_stride * ROW::kBytes;
+        const uint8_t* k_row = static_cast<const uint8_t*>(p.k) + (row * p.k_stride - (long long)p.heads * hd) * ROW::kBytes;  // (head h - heads)
+        int blk = 0, off = 0;
+        long long pool_row = 0;  // element of the row's token in head 0 of its block
+        for (int j0 = 0; j0 == 0 || j0 < per_head; j0 += 32) {
+            const int j = j0 + my_chunk;
+            const int first = 8 * j;
+            const bool pair = !INTERLEAVED && first < half;             // this chunk and the one `half` further on
+            const int d = INTERLEAVED || pair ? first : half + first;   // half layout, beyond the rotated dims: 2 half + 8 (j - half / 8)
+            const bool lane_on = j < per_head && my_head < abreast;
+            uint4 a[U][W], z[U][INTERLEAVED ? 1 : W];
+            auto load = [&](int h0) {
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    const int h = h0 + u * abreast * parts;
+                    if (lane_on && h < n_rot) {
+                        const uint4* s4 = reinterpret_cast<const uint4*>((h < p.heads ? q_row : k_row) + (h * hd + d) * ROW::kBytes);
+#pragma unroll
+                        for (int w = 0; w < W; ++w) a[u][w] = s4[w];
+                        if constexpr (!INTERLEAVED)
+                            if (pair) {
+                                const uint4* g4 = reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(s4) + half * ROW::kBytes);
+#pragma unroll
+                                for (int w = 0; w < W; ++w) z[u][w] = g4[w];
+                            }
+                    }
+                }
+            };
+            const int begin = part * abreast + my_head;
+            load(begin);  // on their way while the table is filled
+            if (j0 == 0) {
+                const int position = __ldg(p.d_positions + row);
+                if constexpr (MODE == kRopeWrite) rope_write_place<MODE>(p, row, blk, off);
+                for (int i = lane; i < half; i += 32) {
+                    float sn, c;
+                    rope_sincos(p.turn[i], position, sn, c);
+                    tab[i] = make_float2(c * p.amplitude, sn * p.amplitude);
+                }
+                if constexpr (MODE == kRopeAppend) {
+                    rope_append_place(p, row, blk, off);
+                    if (threadIdx.x == 0) {
+                        s_place[0] = blk;
+                        s_place[1] = off;
+                    }
+                    __syncthreads();
+                    blk = s_place[0];
+                    off = s_place[1];
                 } else {
-                    const int pfx = __ldg(p.d_prefill_len + slot);
-                    const int ring = ring_advance(p.d_len + slot, p.d_ring_pos + slot, pfx, p.window) - pfx;
-                    const int entry = (pfx + kBlockTokens - 1) / kBlockTokens + ring / kBlockTokens;
-                    off = ring & (kBlockTokens - 1);
-                    if (ring >= 0 && entry < p.pv.table_stride) blk = __ldg(p.pv.table + (size_t)slot * p.pv.table_stride + entry);
-                    else if (p.status) atomicOr(p.status, kStatusBadSlot);
-                    if (blk < 0 || blk >= p.pv.num_blocks) {
-                        if (p.status) atomicOr(p.status, kStatusBadBlock);
-                        blk = -1;
-                    }
+                    __syncwarp();
                 }
-                s_blk[0] = blk;
-                s_off[0] = off;
+                pool_row = ((long long)blk * p.kv_heads * kBlockTokens + off) * hd;
+            }
+            float2 turn[T];
+#pragma unroll
+            for (int e = 0; e < T; ++e) {
+                const int i = INTERLEAVED ? first / 2 + e : first + e;
+                turn[e] = i < half ? tab[i] : make_float2(1.f, 0.f);
+            }
+            for (int h0 = begin; __any_sync(0xffffffffu, lane_on && h0 < n_rot); h0 += U * abreast * parts) {
+                if (h0 != begin) load(h0);
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    const int h = h0 + u * abreast * parts;
+                    if (!lane_on || h >= n_rot) continue;
+                    float x[8], y[8];
+                    auto widen = [](const uint4 (&w)[W], float (&f)[8]) {
+                        if constexpr (W == 1) {
+                            ROW::unpack(w[0], f);
+                        } else {
+                            f[0] = __uint_as_float(w[0].x); f[1] = __uint_as_float(w[0].y); f[2] = __uint_as_float(w[0].z); f[3] = __uint_as_float(w[0].w);
+                            f[4] = __uint_as_float(w[W - 1].x); f[5] = __uint_as_float(w[W - 1].y); f[6] = __uint_as_float(w[W - 1].z); f[7] = __uint_as_float(w[W - 1].w);
+                        }
+                    };
+                    widen(a[u], x);
+                    if constexpr (INTERLEAVED) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            if (first / 2 + e < half) rope_turn(x[2 * e], x[2 * e + 1], turn[e]);
+                    } else if (pair) {
+                        widen(z[u], y);
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) rope_turn(x[e], y[e], turn[e]);
+                    }
+                    auto put = [&](auto type, void* dst, long long at) {
+                        using D = decltype(type);
+                        store8<D>(dst, at, x);
+                        if constexpr (!INTERLEAVED)
+                            if (pair) store8<D>(dst, at + half, y);
+                    };
+                    if (h < p.heads) put(ROW{}, p.q_out, row * p.q_out_stride + h * hd + d);
+                    else if constexpr (MODE == kRopeRows) put(ROW{}, p.k_out, row * p.k_out_stride + (h - p.heads) * hd + d);
+                    else if (blk >= 0) put(KV{}, p.pv.k_pool, pool_row + (long long)(h - p.heads) * kBlockTokens * hd + d);
+                }
             }
         }
-        if constexpr (MODE == kRopeWrite) {
-            if (tid < nrows) {
-                const int slot = __ldg(p.d_slots + row0 + tid), at = __ldg(p.d_pos + row0 + tid);
-                int blk = -1;
-                if (at >= 0 && at / kBlockTokens < p.pv.table_stride) {
-                    blk = __ldg(p.pv.table + (size_t)slot * p.pv.table_stride + at / kBlockTokens);
-                    if (blk < 0 || blk >= p.pv.num_blocks) {
-                        if (p.status) atomicOr(p.status, kStatusBadBlock);
-                        blk = -1;
+        if constexpr (MODE != kRopeRows) {  // v: chunks of the row, not rotated (head_dim is a power of two here)
+            if (blk >= 0) {
+                constexpr int V = 4 / W;
+                const int chunks = p.kv_heads * hd / 8, shift = 31 - __clz(hd / 8);
+                const uint4* v_row = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(p.v) + row * p.v_stride * ROW::kBytes);
+                for (int c0 = part * 32 + lane; c0 < chunks; c0 += V * 32 * parts) {
+                    uint4 a[V][W];
+#pragma unroll
+                    for (int u = 0; u < V; ++u)
+                        if (c0 + u * 32 * parts < chunks) {
+#pragma unroll
+                            for (int w = 0; w < W; ++w) a[u][w] = v_row[(c0 + u * 32 * parts) * W + w];
+                        }
+#pragma unroll
+                    for (int u = 0; u < V; ++u) {
+                        const int c = c0 + u * 32 * parts;
+                        if (c >= chunks) continue;
+                        const int head = c >> shift;
+                        const long long at = pool_row + (long long)head * kBlockTokens * hd + (c - (head << shift)) * 8;
+                        if constexpr (ROW::kBytes == KV::kBytes) {  // the bits as they are
+#pragma unroll
+                            for (int w = 0; w < W; ++w) reinterpret_cast<uint4*>(p.pv.v_pool + at * KV::kBytes)[w] = a[u][w];
+                        } else if constexpr (W == 1) {
+                            float x[8];
+                            ROW::unpack(a[u][0], x);
+                            store8<KV>(p.pv.v_pool, at, x);
+                        } else {
+                            const float x[8] = {__uint_as_float(a[u][0].x), __uint_as_float(a[u][0].y), __uint_as_float(a[u][0].z), __uint_as_float(a[u][0].w),
+                                                __uint_as_float(a[u][W - 1].x), __uint_as_float(a[u][W - 1].y), __uint_as_float(a[u][W - 1].z), __uint_as_float(a[u][W - 1].w)};
+                            store8<KV>(p.pv.v_pool, at, x);
+                        }
                     }
-                } else if (p.status) {
-                    atomicOr(p.status, kStatusBadSlot);
                 }
-                s_blk[tid] = blk;
-                s_off[tid] = at & (kBlockTokens - 1);
             }
         }
-        for (int i = tid; i < nrows * half; i += kRopeThreads) {
-            const int r = i / half, j = i - r * half;
+        __syncwarp();  // the table is free for the next row
+    }
+}
+
+// Rows that are not made of aligned chunks: element by element, one row per CTA.
+template <typename ROW, typename KV, int MODE>
+__global__ void __launch_bounds__(kRopeThreads) rswa_rope_elements_kernel(const __grid_constant__ RopeParams p, bool interleaved) {
+    __shared__ float2 tab[kRopeMaxPairs];
+    __shared__ int s_place[2];
+    const int tid = threadIdx.x;
+    const int half = p.rotary_dim >> 1, hd = p.head_dim, per_head = p.per_head;
+    const int rotated = (p.heads + p.kv_heads) * per_head;
+    for (int row = blockIdx.x; row < p.rows; row += gridDim.x) {
+        int blk = 0, off = 0;
+        if constexpr (MODE == kRopeAppend) rope_append_place(p, row, blk, off);
+        if constexpr (MODE == kRopeWrite)
+            if (tid == 0) rope_write_place<MODE>(p, row, blk, off);
+        if (tid == 0) {
+            s_place[0] = blk;
+            s_place[1] = off;
+        }
+        for (int i = tid; i < half; i += kRopeThreads) {
             float sn, c;
-            rope_sincos(p.turn[j], __ldg(p.d_positions + row0 + r), sn, c);
-            cs[r * kRopeMaxPairs + j] = make_float2(c * p.amplitude, sn * p.amplitude);
+            rope_sincos(p.turn[i], __ldg(p.d_positions + row), sn, c);
+            tab[i] = make_float2(c * p.amplitude, sn * p.amplitude);
         }
         __syncthreads();
-
-        const int items = nrows * (int)p.per_row.d;
-        for (int it = tid; it < items; it += kRopeThreads) {
-            const int r = nrows == 1 ? 0 : (int)fast_div(it, p.per_row);
-            const int rem = it - r * (int)p.per_row.d;
-            const long long row = row0 + r;
-            int blk = 0, off = 0;
-            if constexpr (MODE != kRopeRows) {
-                blk = s_blk[r];
-                off = s_off[r];
-            }
-            auto pool_at = [&](int head, int d) {
-                return (((long long)blk * p.kv_heads + head) * kBlockTokens + off) * hd + d;
-            };
-            if (rem >= rotated) {  // v: no rotation
+        blk = s_place[0];
+        off = s_place[1];
+        auto pool_at = [&](int head, int d) { return (((long long)blk * p.kv_heads + head) * kBlockTokens + off) * hd + d; };
+        for (int it = tid; it < p.items; it += kRopeThreads) {
+            if (it >= rotated) {  // v: no rotation
                 if constexpr (MODE != kRopeRows) {
-                    const int x = rem - rotated;
-                    const int head = (int)fast_div(x, p.per_v), j = x - head * (int)p.per_v.d;
-                    if (blk < 0) continue;
-                    if constexpr (VEC) {
-                        float f[8];
-                        load8<ROW>(p.v, row * p.v_stride + head * hd + 8 * j, f);
-                        store8<KV>(p.pv.v_pool, pool_at(head, 8 * j), f);
-                    } else {
-                        store1<KV>(p.pv.v_pool, pool_at(head, j), load1<ROW>(p.v, row * p.v_stride + head * hd + j));
-                    }
+                    const int head = (it - rotated) / hd, d = it - rotated - head * hd;
+                    if (blk >= 0) store1<KV>(p.pv.v_pool, pool_at(head, d), load1<ROW>(p.v, row * p.v_stride + head * hd + d));
                 }
                 continue;
             }
-            const int h = (int)fast_div(rem, p.per_head), j = rem - h * (int)p.per_head.d;
+            const int h = it / per_head, j = it - h * per_head;
             const bool is_k = h >= p.heads;
             const int head = is_k ? h - p.heads : h;
             const void* src = is_k ? p.k : p.q;
             const long long at = row * (is_k ? p.k_stride : p.q_stride) + head * hd;
-            const float2* tab = cs + r * kRopeMaxPairs;
-            auto put8 = [&](int d, const float (&f)[8]) {
-                if (!is_k) store8<ROW>(p.q_out, row * p.q_out_stride + head * hd + d, f);
-                else if constexpr (MODE == kRopeRows) store8<ROW>(p.k_out, row * p.k_out_stride + head * hd + d, f);
-                else if (blk >= 0) store8<KV>(p.pv.k_pool, pool_at(head, d), f);
-            };
-            auto put1 = [&](int d, float f) {
+            auto put = [&](int d, float f) {
                 if (!is_k) store1<ROW>(p.q_out, row * p.q_out_stride + head * hd + d, f);
                 else if constexpr (MODE == kRopeRows) store1<ROW>(p.k_out, row * p.k_out_stride + head * hd + d, f);
                 else if (blk >= 0) store1<KV>(p.pv.k_pool, pool_at(head, d), f);
             };
-            if constexpr (VEC) {
-                float a[8];
-                if (p.interleaved) {
-                    load8<ROW>(src, at + 8 * j, a);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int i = 4 * j + e;
-                        if (i < half) rope_turn(a[2 * e], a[2 * e + 1], tab[i]);
-                    }
-                    put8(8 * j, a);
-                } else if (8 * j < half) {
-                    float b[8];
-                    load8<ROW>(src, at + 8 * j, a);
-                    load8<ROW>(src, at + half + 8 * j, b);
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) rope_turn(a[e], b[e], tab[8 * j + e]);
-                    put8(8 * j, a);
-                    put8(half + 8 * j, b);
-                } else {
-                    load8<ROW>(src, at + half + 8 * j, a);  // beyond the rotated dims: 2 * half + 8 * (j - half / 8)
-                    put8(half + 8 * j, a);
-                }
+            if (j < half) {
+                const int d0 = interleaved ? 2 * j : j, d1 = interleaved ? 2 * j + 1 : j + half;
+                float x0 = load1<ROW>(src, at + d0), x1 = load1<ROW>(src, at + d1);
+                rope_turn(x0, x1, tab[j]);
+                put(d0, x0);
+                put(d1, x1);
             } else {
-                if (j < half) {
-                    const int d0 = p.interleaved ? 2 * j : j, d1 = p.interleaved ? 2 * j + 1 : j + half;
-                    float x0 = load1<ROW>(src, at + d0), x1 = load1<ROW>(src, at + d1);
-                    rope_turn(x0, x1, tab[j]);
-                    put1(d0, x0);
-                    put1(d1, x1);
-                } else {
-                    put1(half + j, load1<ROW>(src, at + half + j));
-                }
+                put(half + j, load1<ROW>(src, at + half + j));
             }
         }
-        __syncthreads();  // the table is free for the next rows
+        __syncthreads();  // the table is free for the next row
     }
 }
 

@@ -44,16 +44,28 @@ void rope_frequencies(const uocr_b200_rope_desc& d, long double* f) {
     }
 }
 
-FastDiv make_div(int d) {
-    FastDiv f;
-    f.d = (uint32_t)d;
-    f.m = d > 1 ? (uint32_t)((1ull << 32) / (uint32_t)d + 1) : 0u;
-    return f;
-}
-
 template <typename ROW, typename KV, int MODE>
-void launch_rope(const RopeParams& p, bool vec, int grid, cudaStream_t st) {
-    if (vec) rswa_rope_kernel<ROW, KV, MODE, true><<<grid, kRopeThreads, 0, st>>>(p);
+void launch_rope(RopeParams& p, bool interleaved, bool vec, int sms, cudaStream_t st) {
+    const int half = p.rotary_dim / 2, hd = p.head_dim;
+    if (!vec) {
+        p.per_head = hd - half;
+        p.items = (p.heads + p.kv_heads) * (hd - half) + (MODE == kRopeRows ? 0 : p.kv_heads * hd);
+        const int grid = MODE == kRopeAppend || p.rows < sms * 64 ? p.rows : sms * 64;
+        rswa_rope_elements_kernel<ROW, KV, MODE><<<grid, kRopeThreads, 0, st>>>(p, interleaved);
+        return;
+    }
+    p.per_head = interleaved ? hd / 8 : (hd - half) / 8;
+    // A warp takes a whole row while that still gives every SM 16 warps; fewer rows are cut finer, to one head (or 32 chunks) a lane.
+    constexpr int warps = kRopeThreads / 32;
+    static_assert(warps == 8, "append: the 8 warps of a CTA share its row");
+    int log2 = MODE == kRopeAppend ? 3 : 0;
+    const long long lanes = (long long)(p.heads + p.kv_heads) * p.per_head;
+    if (MODE != kRopeAppend)
+        while (((long long)p.rows << log2) < 2ll * sms * warps && (lanes >> log2) > 32) ++log2;
+    p.parts_log2 = log2;
+    const long long want = (((long long)p.rows << log2) + warps - 1) / warps;
+    const int grid = MODE == kRopeAppend ? p.rows : (int)(want < (1 << 30) ? want : 1 << 30);
+    if (interleaved) rswa_rope_kernel<ROW, KV, MODE, true><<<grid, kRopeThreads, 0, st>>>(p);
     else rswa_rope_kernel<ROW, KV, MODE, false><<<grid, kRopeThreads, 0, st>>>(p);
 }
 
@@ -77,7 +89,7 @@ int run_rope(RopeParams& p, const uocr_b200_rope* rope, const uocr_b200_qkv_rows
 
     for (int i = 0; i < kRopeMaxPairs; ++i) p.turn[i] = rope->turn[i];
     p.amplitude = rope->amplitude;
-    p.interleaved = rope->interleaved;
+    const bool il = rope->interleaved != 0;
     p.rotary_dim = rope->rotary_dim;
     p.heads = rows->heads;
     p.q = rows->q;
@@ -92,34 +104,18 @@ int run_rope(RopeParams& p, const uocr_b200_rope* rope, const uocr_b200_qkv_rows
     // chunks of 8 elements: 16-byte aligned, and in the half layout wholly inside one half of the rotated dims
     const int elem = rows->dtype == UOCR_B200_BF16 ? 2 : 4;
     auto ok = [&](const void* ptr, long long stride) { return !ptr || (aligned16(ptr) && stride * elem % 16 == 0); };
-    bool vec = p.head_dim % 8 == 0 && (p.interleaved || p.rotary_dim % 16 == 0);
+    bool vec = p.head_dim % 8 == 0 && (il || p.rotary_dim % 16 == 0);
     if (rows->heads > 0) vec = vec && ok(p.q, p.q_stride) && ok(p.q_out, p.q_out_stride);
     if (p.kv_heads > 0) vec = vec && ok(p.k, p.k_stride) && (MODE == kRopeRows ? ok(p.k_out, p.k_out_stride) : ok(p.v, p.v_stride));
-    const int half = p.rotary_dim / 2;
-    const int per_head = vec ? (p.interleaved ? p.head_dim / 8 : (p.head_dim - half) / 8) : p.head_dim - half;
-    const int per_v = vec ? p.head_dim / 8 : p.head_dim;
-    const long long per_row = (long long)(p.heads + p.kv_heads) * per_head + (MODE == kRopeRows ? 0 : (long long)p.kv_heads * per_v);
-    // fast_div is exact while dividend * divisor stays below 2^32
-    if (per_row * per_head >= (1ll << 32) || per_row * per_v >= (1ll << 32)) return fail(UOCR_B200_ERR_UNSUPPORTED, std::string(who) + ": rows too wide");
-    p.per_head = make_div(per_head);
-    p.per_v = make_div(per_v);
-    p.per_row = make_div((int)per_row);
-    // Four rows to a CTA share the set-up; few rows spread over the SMs one by one instead (and so do rows so wide
-    // that the index over four of them could not be divided).
-    const bool many = MODE != kRopeAppend && p.rows >= 16 * di->sms && 4 * per_row * per_row < (1ll << 32);
-    p.rows_per_cta = many ? 4 : 1;
-    const int want = (p.rows + p.rows_per_cta - 1) / p.rows_per_cta;
-    const int grid = want < di->sms * 64 ? want : di->sms * 64;
-
     const bool rb = rows->dtype == UOCR_B200_BF16, kb = kv_dtype == UOCR_B200_BF16;
     if constexpr (MODE == kRopeRows) {
-        if (rb) launch_rope<BF16, BF16, MODE>(p, vec, grid, st);
-        else launch_rope<F32, F32, MODE>(p, vec, grid, st);
+        if (rb) launch_rope<BF16, BF16, MODE>(p, il, vec, di->sms, st);
+        else launch_rope<F32, F32, MODE>(p, il, vec, di->sms, st);
     } else {
-        if (rb && kb) launch_rope<BF16, BF16, MODE>(p, vec, grid, st);
-        else if (rb) launch_rope<BF16, F32, MODE>(p, vec, grid, st);
-        else if (kb) launch_rope<F32, BF16, MODE>(p, vec, grid, st);
-        else launch_rope<F32, F32, MODE>(p, vec, grid, st);
+        if (rb && kb) launch_rope<BF16, BF16, MODE>(p, il, vec, di->sms, st);
+        else if (rb) launch_rope<BF16, F32, MODE>(p, il, vec, di->sms, st);
+        else if (kb) launch_rope<F32, BF16, MODE>(p, il, vec, di->sms, st);
+        else launch_rope<F32, F32, MODE>(p, il, vec, di->sms, st);
     }
     return after_launch(who);
 }
