@@ -573,7 +573,8 @@ UOCR_B200_API int uocr_b200_rswa_prefill_text_scored_paged(
  * queries and fp32 results go through the tensor cores as bf16 pairs; bf16 queries are taken as they are and, for bf16
  * results, the probabilities are rounded to bf16 (half a step, as the result itself).  K and V outside
  * the span of keys that the rows of a query tile see -- from the first to the last -- may hold anything; inside it
- * they must be finite, since the rows that do not see a key multiply its value by zero.  d_key_pos is not supported (UNSUPPORTED): keys
+ * they must be finite, since the rows that do not see a key multiply its value by zero. A query row that holds a NaN or an
+ * infinity gives NaN (0 if it sees no key).  d_key_pos is not supported (UNSUPPORTED): keys
  * stand at their own index. */
 UOCR_B200_API int uocr_b200_rswa_prefill_attention_scored_tc(
     const uocr_b200_paged_kv* kv, const void* text_k_pool, const void* text_v_pool, int text_blocks,

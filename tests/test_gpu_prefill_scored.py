@@ -225,6 +225,30 @@ def test_nan_outside_the_span(b, lo, hi):
     w.run(lo=full(lo), hi=full(hi))
 
 
+@pytest.mark.parametrize("cap,bias,q_dtype,out", MODES)
+def test_nan_in_a_query_stays_in_its_row(b, cap, bias, q_dtype, out):
+    import torch
+    w = Wave(b, torch, [(200, 0, 200, 0), (60, 0, 140, 1), (0, 0, 1, 0)], 2, 2, seed=31)
+    q_pos = torch.cat([torch.arange(200, device="cuda"), 60 + torch.arange(140, device="cuda"), torch.zeros(1, device="cuda")]).to(torch.int32)
+    score = b.Score(softcap=cap, slopes=slopes_of(torch, 2) if bias else None, d_q_pos=q_pos)
+    ws = b.Workspace(64)
+    ws.set_out_dtype(b.BF16 if out == "bfloat16" else b.F32)
+    bad = [0, 5, 127, 128, 199, 200, 339, 340]  # the last one sees nothing
+    q, hurt = w.q.to(getattr(torch, q_dtype)), w.q.clone()
+    for i, r in enumerate(bad):
+        hurt[r, 128 + i * 7] = float("nan") if i % 2 else float("inf")  # head 1 only
+    res = []
+    for x in (q, hurt.to(q.dtype)):
+        o = torch.full((341, 256), 7.0, dtype=getattr(torch, out), device="cuda")
+        b.prefill_attention_scored_tc(w.layer, *w.text, w.text_blocks, score, x, w.d_prefill, w.tiles, 100, 2, o, ws)
+        res.append(o)
+    assert ws.status() == 0
+    good = torch.ones(341, dtype=torch.bool, device="cuda")
+    good[bad[:-1]] = False
+    assert torch.isnan(res[1][~good][:, 128:]).all() and not res[1][340].any()
+    assert torch.equal(res[0][good], res[1][good]) and torch.equal(res[0][:, :128], res[1][:, :128])
+
+
 def test_against_the_call_for_any_geometry(b):
     """Many items per CTA, plan reused by two calls, results next to the CUDA-core call's."""
     import torch

@@ -240,6 +240,7 @@ int uocr_b200_workspace_status(uocr_b200_workspace* ws, uocr_b200_stream_t strea
     if (v != 0 && ws->counters) {
         // a kernel that gave up may have left arrival counters half-way: start clean again
         CHECK_CUDA(cudaMemsetAsync(ws->counters, 0, sizeof(int) * ((size_t)ws->pieces_max + 64), st), "counter clear");
+        if (ws->item_counter) CHECK_CUDA(cudaMemsetAsync(ws->item_counter, 0, 2 * sizeof(int), st), "item counter clear");
         CHECK_CUDA(cudaStreamSynchronize(st), "counter clear sync");
     }
     *device_status = v;

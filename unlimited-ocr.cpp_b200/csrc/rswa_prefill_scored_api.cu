@@ -80,7 +80,7 @@ int uocr_b200_rswa_prefill_attention_scored_tc(const uocr_b200_paged_kv* kv, con
     const bool any_text = ws->plan_any_text;
     if (any_text && (!text_k_pool || !text_v_pool || text_blocks <= 0)) return bad("text tiles need the text pool");
     if (any_text && score->slopes && !score->d_q_pos) return bad("a distance bias on text rows needs d_q_pos");
-    CHECK_CUDA(cudaMemsetAsync(ws->item_counter, 0, sizeof(int), st), "prefill item counter");
+    if ((long long)n_tiles * heads >= (1ll << 31)) return fail(UOCR_B200_ERR_UNSUPPORTED, std::string(who) + ": too many tiles");
     PrefillParams pp{};
     pp.q = static_cast<const float*>(q);
     pp.out = static_cast<float*>(out);
@@ -93,7 +93,7 @@ int uocr_b200_rswa_prefill_attention_scored_tc(const uocr_b200_paged_kv* kv, con
     pp.d_prefill_len = d_prefill_len;
     pp.tiles = ws->tiles;
     pp.work = ws->tile_work;
-    pp.counter = ws->item_counter;
+    pp.counter = ws->item_counter + 1;  // (the plain call has its own)
     pp.n_tiles = n_tiles;
     pp.table_stride = pv.table_stride;
     pp.num_blocks = pv.num_blocks;

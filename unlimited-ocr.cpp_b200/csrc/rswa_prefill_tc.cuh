@@ -263,18 +263,81 @@ __device__ __forceinline__ float tc_rcp(float x) {
     return y;
 }
 
-// Scores of 64 keys modified in place, into the log2 domain.  tanh(x) = 1 - 2 / (1 + e^2x): two special-function
-// instructions, off by 2^-22 at most, and right at both ends (e^2x = 0 or infinity).  d0: the query's position minus
-// that of key 0.
+// 2^x for x in [-126, 126] without a special-function instruction: x = n + f with |f| <= 1/2 (adding 1.5 * 2^23 rounds to
+// the integer n, which is then in the low bits), a polynomial of degree 4 of least maximum relative error for 2^f, n added to
+// the exponent.  Relative error 2.7e-6.  Two values at a time.
+__device__ __forceinline__ float2 tc_exp2_poly(float2 x) {
+    constexpr float M = 12582912.f;
+    const float2 r = __fadd2_rn(x, make_float2(M, M));
+    const float2 n = __fadd2_rn(r, make_float2(-M, -M));
+    const float2 f = __ffma2_rn(n, make_float2(-1.f, -1.f), x);
+    auto horner = [&](float2 acc, float c) { return __ffma2_rn(acc, f, make_float2(c, c)); };
+    float2 y = horner(make_float2(0.009570102207362652f, 0.009570102207362652f), 0.05591785907745361f);
+    y = horner(horner(horner(y, 0.240247443318367f), 0.6931217908859253f), 0.9999992847442627f);
+    return make_float2(__uint_as_float(__float_as_uint(y.x) + (__float_as_uint(r.x) << 23)),
+                       __uint_as_float(__float_as_uint(y.y) + (__float_as_uint(r.y) << 23)));
+}
+
+// Keys that the softmax with modified scores handles, or leaves out, together.  (Two softmax warps share a scheduler, so it is the
+// independent keys of a chunk that hide the latencies: chunks of 16 keys were 5 % slower than chunks of 32, where one chunk of 64 gave
+// away what half-hidden tiles allow.)
+constexpr int kTcChunk = 32;
+
+// Scores of a chunk of keys modified in place, into the log2 domain.  tanh(x) = 1 - 2 / (1 + e^2x), right at both ends.  Special
+// functions are the scarce resource (16 results a cycle and SM), so four reciprocals are taken as one, of the product of the four
+// denominators (e^2x is cut at 2^30, where the tanh is 1 already: the product stays below 2^121), and with bf16 results half of
+// the powers go to the polynomial.  The cut also turns the NaN of a key that the row does not see into a number, so it cannot
+// reach the three others through the product; a NaN in the query is reported by the helpers.  d0: the query's position minus that
+// of key 0.
 template <typename Mode>
-__device__ __forceinline__ void tc_modify(uint32_t (&s)[64], float mul, float cap_log2, float slope_log2, float d0) {
+__device__ __forceinline__ void tc_modify(uint32_t* s, float mul, float cap_log2, float slope_log2, float d0) {
 #pragma unroll
-    for (int j = 0; j < 64; ++j) {
-        float x = __uint_as_float(s[j]) * mul;
-        if constexpr (Mode::kCap) x = fmaf(-2.f * cap_log2, tc_rcp(1.f + tc_exp2(x)), cap_log2);
-        if constexpr (Mode::kBias) x = fmaf(-slope_log2, fabsf(d0 - (float)j), x);
-        s[j] = __float_as_uint(x);
+    for (int j = 0; j < kTcChunk; j += 4) {
+        float2 x[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            x[i] = __fmul2_rn(make_float2(__uint_as_float(s[j + 2 * i]), __uint_as_float(s[j + 2 * i + 1])), make_float2(mul, mul));
+        if constexpr (Mode::kCap) {
+            float2 e[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const float2 t = make_float2(fminf(x[i].x, 30.f), fminf(x[i].y, 30.f));
+                if (i == 1 && !Mode::kPairP) e[i] = tc_exp2_poly(make_float2(fmaxf(t.x, -126.f), fmaxf(t.y, -126.f)));
+                else e[i] = make_float2(tc_exp2(t.x), tc_exp2(t.y));
+                e[i] = __fadd2_rn(e[i], make_float2(1.f, 1.f));
+            }
+            const float ab = e[0].x * e[0].y, cd = e[1].x * e[1].y;
+            const float r = tc_rcp(ab * cd) * (-2.f * cap_log2);
+            const float r_ab = r * cd, r_cd = r * ab;  // -2 cap / (e0 e1), / (e2 e3)
+            const float2 cap2 = make_float2(cap_log2, cap_log2);
+            x[0] = __ffma2_rn(make_float2(r_ab, r_ab), make_float2(e[0].y, e[0].x), cap2);
+            x[1] = __ffma2_rn(make_float2(r_cd, r_cd), make_float2(e[1].y, e[1].x), cap2);
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            if constexpr (Mode::kBias) {
+                x[i].x = fmaf(-slope_log2, fabsf(d0 - (float)(j + 2 * i)), x[i].x);
+                x[i].y = fmaf(-slope_log2, fabsf(d0 - (float)(j + 2 * i + 1)), x[i].y);
+            }
+            s[j + 2 * i] = __float_as_uint(x[i].x);
+            s[j + 2 * i + 1] = __float_as_uint(x[i].y);
+        }
     }
+}
+
+// Keys of a region that the rows of a warp see: every row sees [lo_max, hi_min), some row [lo_min, hi_max).  Rows that the
+// tile does not have do not count.
+struct TcSpan {
+    int lo_min, lo_max, hi_min, hi_max;
+};
+__device__ __forceinline__ TcSpan tc_span(bool live, int lo, int hi) {
+    constexpr int kFar = 0x3fffffff;
+    TcSpan w;
+    w.lo_min = __reduce_min_sync(0xffffffffu, live && lo < hi ? lo : kFar);
+    w.hi_max = __reduce_max_sync(0xffffffffu, live && lo < hi ? hi : -kFar);
+    w.lo_max = __reduce_max_sync(0xffffffffu, live ? lo : -kFar);
+    w.hi_min = __reduce_min_sync(0xffffffffu, live ? hi : kFar);
+    return w;
 }
 
 // One key tile of the online softmax for this thread: its row, its half (64 keys) of the tile.
@@ -286,14 +349,11 @@ __device__ __forceinline__ void tc_modify(uint32_t (&s)[64], float mul, float ca
 // m_ref is the reference the row's probabilities are scaled by; alpha is the factor the row's
 // accumulator and sum take when the reference moved (1 otherwise).  False if the rendezvous ran out
 // of time.
-template <typename Mode>
 __device__ __forceinline__ bool tc_softmax_half(bool full, uint32_t tS, int h, int vlo, int vhi, float* my_max, const float* other_max,
                                                 uint32_t pair_bar, uint32_t pair_parity, int* status, uint32_t wait_limit,
-                                                float& m_ref, float& l_run, float& alpha, float mul = 0.f, float cap_log2 = 0.f,
-                                                float slope_log2 = 0.f, float d0 = 0.f) {
+                                                float& m_ref, float& l_run, float& alpha) {
     uint32_t s[64];
     tc_ld64(tS + h * 64, s);
-    if constexpr (Mode::kScored) tc_modify<Mode>(s, mul, cap_log2, slope_log2, d0);
     if (!full) {
         // Of this thread's 64 keys the visible ones are [lo, hi).  A causal edge only has an upper bound, a window
         // edge only a lower one: each bound is applied only where some row of the warp needs it.
@@ -324,33 +384,90 @@ __device__ __forceinline__ bool tc_softmax_half(bool full, uint32_t tS, int h, i
     }
     const float m_safe = (m_ref == -INFINITY) ? 0.f : m_ref;
     float lsum = 0.f;
-    if constexpr (!Mode::kPairP) {  // one bf16 per probability: 64 keys in the first 32 of this thread's columns
+#pragma unroll
+    for (int qq = 0; qq < 2; ++qq) {  // 32 keys at a time: their 16 hi words, then their 16 lo words, over their own columns
         uint32_t pk[32];
 #pragma unroll
-        for (int e = 0; e < 32; ++e) {
-            const float p0 = tc_exp2(__uint_as_float(s[2 * e]) - m_safe);
-            const float p1 = tc_exp2(__uint_as_float(s[2 * e + 1]) - m_safe);
+        for (int e = 0; e < 16; ++e) {
+            const float p0 = tc_exp2(__uint_as_float(s[qq * 32 + 2 * e]) - m_safe);
+            const float p1 = tc_exp2(__uint_as_float(s[qq * 32 + 2 * e + 1]) - m_safe);
             lsum += p0 + p1;
-            pk[e] = rn_bf16x2(p0, p1);
+            tc_split2(p0, p1, pk[e], pk[16 + e]);
         }
-        tc_st32(tS + h * 64, pk);
-    } else {
-#pragma unroll
-        for (int qq = 0; qq < 2; ++qq) {  // 32 keys at a time: their 16 hi words, then their 16 lo words, over their own columns
-            uint32_t pk[32];
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                const float p0 = tc_exp2(__uint_as_float(s[qq * 32 + 2 * e]) - m_safe);
-                const float p1 = tc_exp2(__uint_as_float(s[qq * 32 + 2 * e + 1]) - m_safe);
-                lsum += p0 + p1;
-                if constexpr (Mode::kScored) tc_split2_rn(p0, p1, pk[e], pk[16 + e]);
-                else tc_split2(p0, p1, pk[e], pk[16 + e]);
-            }
-            tc_st32(tS + h * 64 + qq * 32, pk);
-        }
+        tc_st32(tS + h * 64 + qq * 32, pk);
     }
     asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
     l_run = l_run * alpha + lsum;
+    return true;
+}
+
+// The same with modified scores.  Chunks of keys that no row of the warp sees are left out of everything (their
+// probabilities are zero), the scores of hidden keys are only looked for in chunks that some row does not see whole.  lo / hi: what
+// this row sees of this thread's 64 keys; w: what the warp's rows see of them.
+template <typename Mode>
+__device__ __forceinline__ bool tc_softmax_half_scored(uint32_t tS, int h, int lo, int hi, const TcSpan& w, float* my_max, const float* other_max,
+                                                       uint32_t pair_bar, uint32_t pair_parity, int* status, uint32_t wait_limit, float& m_ref,
+                                                       float& l_run, float& alpha, float mul, float cap_log2, float slope_log2, float d0) {
+    uint32_t s[64];
+    tc_ld64(tS + h * 64, s);
+    auto some_see = [&](int c) { return c < w.hi_max && c + kTcChunk > w.lo_min; };
+    float mx = -INFINITY;
+#pragma unroll
+    for (int c = 0; c < 64; c += kTcChunk) {
+        if (!some_see(c)) continue;
+        tc_modify<Mode>(s + c, mul, cap_log2, slope_log2, d0 - (float)c);
+        if (c + kTcChunk > w.hi_min || c < w.lo_max) {
+#pragma unroll
+            for (int j = c; j < c + kTcChunk; ++j)
+                if (j < lo || j >= hi) s[j] = 0xff800000u;  // -inf
+        }
+        float m0 = -INFINITY, m1 = -INFINITY;
+#pragma unroll
+        for (int j = c; j < c + kTcChunk; j += 2) {
+            m0 = fmaxf(m0, __uint_as_float(s[j]));
+            m1 = fmaxf(m1, __uint_as_float(s[j + 1]));
+        }
+        mx = fmaxf(mx, fmaxf(m0, m1));
+    }
+    *my_max = mx;
+    // also: both halves of S are in registers from here on, P may overwrite them
+    if (!pair_sync(pair_bar, pair_parity, status, wait_limit)) return false;
+    const float m_tile = fmaxf(mx, *other_max);
+    alpha = 1.f;
+    if (m_tile > m_ref + kTcMaxSlack) {  // also the first visible key of the row (m_ref = -inf)
+        alpha = tc_exp2(m_ref - m_tile);
+        m_ref = m_tile;
+    }
+    const float m_safe = (m_ref == -INFINITY) ? 0.f : m_ref;
+    float2 l2 = make_float2(0.f, 0.f);
+    uint32_t pk[32];
+#pragma unroll
+    for (int c = 0; c < 64; c += kTcChunk) {
+        // pairs: the chunk's 16 hi words, then its 16 lo words, over its own columns; single bf16: 64 keys in the first 32 of
+        // this thread's columns
+        const int at = Mode::kPairP ? 0 : c / 2;
+        if (some_see(c)) {
+#pragma unroll
+            for (int e = 0; e < kTcChunk / 2; ++e) {
+                const float2 x = __fadd2_rn(make_float2(__uint_as_float(s[c + 2 * e]), __uint_as_float(s[c + 2 * e + 1])), make_float2(-m_safe, -m_safe));
+                const float2 pr = make_float2(tc_exp2(x.x), tc_exp2(x.y));
+                l2 = __fadd2_rn(l2, pr);
+                if constexpr (Mode::kPairP) tc_split2_rn(pr.x, pr.y, pk[at + e], pk[16 + at + e]);
+                else pk[at + e] = rn_bf16x2(pr.x, pr.y);
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < kTcChunk / 2; ++e) {
+                pk[at + e] = 0u;
+                if constexpr (Mode::kPairP) pk[16 + at + e] = 0u;
+            }
+        }
+        if constexpr (Mode::kPairP) tc_st32(tS + h * 64 + c, pk);
+    }
+    static_assert(kTcChunk == 32, "the layout of a pair of words above");
+    if constexpr (!Mode::kPairP) tc_st32(tS + h * 64, pk);
+    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+    l_run = l_run * alpha + l2.x + l2.y;
     return true;
 }
 
@@ -622,17 +739,20 @@ rswa_prefill_tc_kernel(const PrefillParams p, const __grid_constant__ PrefillMap
             const bool live = r < t.rows;
             const int i = t.pos0 + r;
             int plo = 0, phi = !live ? 0 : (t.kind == 0 ? min(i + 1, cur.pfx) : cur.pfx);  // fixed-region tokens [plo, phi)
+            const int tlo = max(0, i - p.window + 1);
+            const int thi = (live && t.kind == 1) ? i + 1 : 0;                           // text tokens [tlo, thi)
             int q_pos = i;
             float slope_log2 = 0.f;
+            TcSpan fixed_span = {}, text_span = {};
             if constexpr (Mode::kScored) {
                 if (live) tc_row_range(p, t, r, cur.pfx, plo, phi);
+                fixed_span = tc_span(live, plo, phi);
+                if (t.kind == 1) text_span = tc_span(live, tlo, thi);
                 if constexpr (Mode::kBias) {
                     if (live && p.d_q_pos) q_pos = __ldg(p.d_q_pos + t.row0 + r);
                     slope_log2 = __ldg(p.slopes + cur.head) * 1.4426950408889634f;
                 }
             }
-            const int tlo = max(0, i - p.window + 1);
-            const int thi = (live && t.kind == 1) ? i + 1 : 0;                           // text tokens [tlo, thi)
             // Q of this item is in TMEM: the helpers have also taken the sums of the item before last out of xsum
             if (!__all_sync(0xffffffffu, mbar_wait_bounded(q_full(itc), (itc >> 1) & 1u, p.status, p.wait_limit))) { ok = false; break; }
             float m_ref = -INFINITY, l_run = 0.f;
@@ -649,12 +769,19 @@ rswa_prefill_tc_kernel(const PrefillParams p, const __grid_constant__ PrefillMap
                 float* my_max = xmax + (b * 2 + h) * 128 + r;
                 const float* other_max = xmax + (b * 2 + (h ^ 1)) * 128 + r;
                 float alpha = 1.f;
-                const bool full = __all_sync(0xffffffffu, vlo <= 0 && vhi >= kTcTile);
-                if constexpr (Mode::kScored)
-                    ok = tc_softmax_half<Mode>(full, tS, h, vlo, vhi, my_max, other_max, pair_bar(quad), pp & 1u, p.status, p.wait_limit, m_ref, l_run, alpha,
-                                               p.score_mul, p.cap_log2, slope_log2, (float)((long long)(text ? i : q_pos) - t0 - h * 64));
-                else
-                    ok = tc_softmax_half<Mode>(full, tS, h, vlo, vhi, my_max, other_max, pair_bar(quad), pp & 1u, p.status, p.wait_limit, m_ref, l_run, alpha);
+                if constexpr (Mode::kScored) {
+                    const int k0 = t0 + h * 64;  // this thread's first key
+                    TcSpan w = text ? text_span : fixed_span;
+                    w.lo_min -= k0;
+                    w.lo_max -= k0;
+                    w.hi_min -= k0;
+                    w.hi_max -= k0;
+                    ok = tc_softmax_half_scored<Mode>(tS, h, vlo - h * 64, vhi - h * 64, w, my_max, other_max, pair_bar(quad), pp & 1u, p.status, p.wait_limit,
+                                                      m_ref, l_run, alpha, p.score_mul, p.cap_log2, slope_log2, (float)((long long)(text ? i : q_pos) - k0));
+                } else {
+                    const bool full = __all_sync(0xffffffffu, vlo <= 0 && vhi >= kTcTile);
+                    ok = tc_softmax_half(full, tS, h, vlo, vhi, my_max, other_max, pair_bar(quad), pp & 1u, p.status, p.wait_limit, m_ref, l_run, alpha);
+                }
                 ++pp;
                 if (!ok) break;
                 // A row whose reference moved takes the factor on its accumulator before this tile's product is
@@ -699,9 +826,13 @@ rswa_prefill_tc_kernel(const PrefillParams p, const __grid_constant__ PrefillMap
             }
         };
         // Q row of item m -> TMEM (lane = row, column c of a 64-column block = dims 2c, 2c+1; hi words, then lo words)
+        // Modified scores: whether the row holds a NaN or an infinity (its result is NaN; the cap would hide it).
+        bool q_bad = false, next_bad = false;
         auto convert_q = [&](const TcItem& it, uint32_t m) -> bool {
             if (!__all_sync(0xffffffffu, mbar_wait_bounded(q_landed, m & 1u, p.status, p.wait_limit))) return false;
             const bool live = r < it.t.rows;
+            q_bad = next_bad;
+            next_bad = false;
             if constexpr (!Mode::kPairQ) {  // bf16 queries are the operand already
                 const uint4* w4 = reinterpret_cast<const uint4*>(my_row);
 #pragma unroll 1
@@ -710,6 +841,7 @@ rswa_prefill_tc_kernel(const PrefillParams p, const __grid_constant__ PrefillMap
 #pragma unroll
                     for (int c = 0; c < 4; ++c) {
                         const uint4 v = live ? w4[g4 * 4 + c] : make_uint4(0u, 0u, 0u, 0u);
+                        for (uint32_t x : {v.x, v.y, v.z, v.w}) next_bad |= (x & 0x7f80u) == 0x7f80u || (x & 0x7f800000u) == 0x7f800000u;
                         w[4 * c] = v.x; w[4 * c + 1] = v.y; w[4 * c + 2] = v.z; w[4 * c + 3] = v.w;
                     }
                     tc_st16(tmem + lane_base + kTcColQ + g4 * 16, w);
@@ -724,6 +856,7 @@ rswa_prefill_tc_kernel(const PrefillParams p, const __grid_constant__ PrefillMap
                 for (int c = 0; c < 8; ++c) {
                     const float4 v = live ? q4[g4 * 8 + c] : make_float4(0.f, 0.f, 0.f, 0.f);
                     if constexpr (Mode::kScored) {
+                        next_bad |= !(fabsf(v.x) < INFINITY && fabsf(v.y) < INFINITY && fabsf(v.z) < INFINITY && fabsf(v.w) < INFINITY);
                         tc_split2_rn(v.x, v.y, hi[2 * c], lo[2 * c]);
                         tc_split2_rn(v.z, v.w, hi[2 * c + 1], lo[2 * c + 1]);
                     } else {
@@ -761,7 +894,8 @@ rswa_prefill_tc_kernel(const PrefillParams p, const __grid_constant__ PrefillMap
             const uint32_t um = (uint32_t)m;
             if (!__all_sync(0xffffffffu, mbar_wait_bounded(l_ready(um), (um >> 1) & 1u, p.status, p.wait_limit))) { ok = false; break; }
             const float l_tot = xsum[((um & 1u) * 2 + 0) * 128 + r] + xsum[((um & 1u) * 2 + 1) * 128 + r];
-            const float inv = l_tot > 0.f ? 1.f / l_tot : 0.f;
+            float inv = l_tot > 0.f ? 1.f / l_tot : 0.f;
+            if (Mode::kScored && (nxt.valid ? q_bad : next_bad) && l_tot != 0.f) inv = __uint_as_float(0x7fffffffu);  // (convert_q has moved on to the next item's row)
             if (!__all_sync(0xffffffffu, mbar_wait_bounded(o_done, um & 1u, p.status, p.wait_limit))) { ok = false; break; }
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll 1
@@ -866,7 +1000,8 @@ rswa_prefill_tc_kernel(const PrefillParams p, const __grid_constant__ PrefillMap
             }
             mbar_arrive(item_full(sl));  // (release: the slot's contents are visible to whoever sees the phase)
             ++pub;
-            if (valid) k_next = (long long)gridDim.x + atomicAdd(p.counter, 1);
+            // (modified scores: as many draws as items, so the counter wraps back to zero by itself)
+            if (valid) k_next = (long long)gridDim.x + (Mode::kScored ? (int)atomicInc(reinterpret_cast<unsigned*>(p.counter), (unsigned)n_items - 1) : atomicAdd(p.counter, 1));
             return true;
         };
         for (;; ++m) {
