@@ -9,7 +9,8 @@
 // sequence and a batch of many short ones load the SMs alike; a warp streams its piece's K and V tiles
 // through a private ring of shared memory with bulk copies, and the last warp to finish an item that
 // straddles pieces joins the partial results (maximum, sum, accumulator).  What differs:
-//   - an item is a row and up to four query heads of one KV head (G), so grouped heads read a tile once;
+//   - an item is a row and up to four query heads of one KV head (G), so grouped heads read a tile once, and where it pays
+//     (bf16, head_dim 64 or 128) their products run on the tensor cores;
 //   - only tiles that hold a visible token are on the line: the cost of a page is the page;
 //   - the line is planned by every CTA in its own shared memory when the rows fit (one launch), else by
 //     rswa_scored_plan_kernel;
@@ -183,13 +184,444 @@ constexpr uint32_t kSuText = 1u << 12;     // tile of the text pool
 constexpr int kScoreRing = 2;              // tile slots per warp
 constexpr int kScoreThreads = 512;
 
+// The item (row, head group) a warp is working on, as both consumers below need it.
+struct ScoreItem {
+    uint32_t index;  // row * items_per_row + group
+    int slot, q_pos;
+};
+
+__device__ __forceinline__ float score_distance(const ScoreParams& p, const ScoreItem& it, uint32_t meta, int tok0, int t, bool visible) {
+    if (meta & kSuFixed) {
+        int at = tok0 + t;
+        if (p.d_key_pos && visible && at < p.key_pos_stride) at = __ldg(p.d_key_pos + (size_t)it.slot * p.key_pos_stride + at);
+        return __uint2float_rn((uint32_t)max(it.q_pos, at) - (uint32_t)min(it.q_pos, at));
+    }
+    const int a = tok0 - t;
+    return (float)(a < 0 ? a + p.plan.window : a);
+}
+
+// x = q.k times q_scale -> the modified score in the log2 domain
+__device__ __forceinline__ float score_modify(const ScoreParams& p, float x, float slope, float dist) {
+    if (p.cap_log2 > 0.f) x = p.cap_log2 * tanhf(x);
+    if (p.slopes) x = fmaf(-slope, dist, x);
+    return x;
+}
+
+__device__ __forceinline__ void score_record(const ScoreParams& p, size_t head_row, int at, float x) {
+    if (at < p.score_stride) __stcs(p.scores + head_row * p.score_stride + at, x);
+}
+
+__device__ __forceinline__ void score_store8(const ScoreParams& p, size_t at, const float (&v)[8]) {
+    if (p.out_bf16) {
+        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + at) =
+            make_uint4(rn_bf16x2(v[0], v[1]), rn_bf16x2(v[2], v[3]), rn_bf16x2(v[4], v[5]), rn_bf16x2(v[6], v[7]));
+    } else {
+        float4* o = reinterpret_cast<float4*>(static_cast<float*>(p.out) + at);
+        o[0] = make_float4(v[0], v[1], v[2], v[3]);
+        o[1] = make_float4(v[4], v[5], v[6], v[7]);
+    }
+}
+
+// -------------------------------------------------------------------------------------------------
+// consumer on the CUDA cores: LPR lanes share a cache row, every lane keeps its chunk of q and of the accumulator
+// -------------------------------------------------------------------------------------------------
 template <typename KV, int HD, int G>
-__global__ void __launch_bounds__(kScoreThreads, 1) rswa_scored_kernel(const __grid_constant__ ScoreParams p) {
+struct ScoreFma {
     using M = TileMap<KV, HD>;
-    constexpr int LPR = M::kLanesPerRow, CPL = M::kChunksPerLane, RPW = M::kRowsPerLoad;
-    constexpr int ITER = M::kIters, EPC = KV::kPerChunk, EPL = M::kElemsPerLane;
-    constexpr int PPC = EPC / 2, PPL = EPL / 2;
-    constexpr int ROWB = M::kRowBytes, TILE = M::kTileBytes;
+    static constexpr int kGroup = G, kTile = M::kTileBytes, kThreads = kScoreThreads;
+    static constexpr int LPR = M::kLanesPerRow, CPL = M::kChunksPerLane, RPW = M::kRowsPerLoad;
+    static constexpr int ITER = M::kIters, EPC = KV::kPerChunk, EPL = M::kElemsPerLane;
+    static constexpr int PPC = EPC / 2, PPL = EPL / 2, ROWB = M::kRowBytes;
+
+    float2 q2[G][PPL], acc2[G][PPL];
+    float m_run[G], l_run[G], slope[G], pr[G];
+    int g, rg, my_tok;
+    bool one_of_pair;
+
+    __device__ __forceinline__ void init(int lane) {
+        g = lane % LPR;   // chunk position inside the row
+        rg = lane / LPR;  // which of the RPW rows of a warp-wide load
+        my_tok = (LPR >= 2 ? (g >> 1) * RPW : 0) + rg;  // the token whose score this lane ends up with
+        one_of_pair = LPR < 2 || (g & 1) == 0;
+    }
+    __device__ __forceinline__ void load(const ScoreParams& p, const ScoreItem& it) {
+        const size_t at = (size_t)it.index * (G * HD);  // items_per_row * G == heads
+        const int h0 = (int)(it.index % (uint32_t)p.plan.items_per_row) * G;
+#pragma unroll
+        for (int i = 0; i < G; ++i) {
+#pragma unroll
+            for (int cp = 0; cp < CPL; ++cp) {
+                const int d0 = (g + 32 * cp) * EPC;
+#pragma unroll
+                for (int e = 0; e < EPC; e += 4) {
+                    float4 t;
+                    if (p.q_bf16) {
+                        const uint2 w = __ldg(reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p.q) + at + i * HD + d0 + e));
+                        t = make_float4(bf16_lo(w.x), bf16_hi(w.x), bf16_lo(w.y), bf16_hi(w.y));
+                    } else {
+                        t = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(p.q) + at + i * HD + d0 + e));
+                    }
+                    q2[i][(cp * EPC + e) / 2] = make_float2(t.x * p.q_scale, t.y * p.q_scale);
+                    q2[i][(cp * EPC + e) / 2 + 1] = make_float2(t.z * p.q_scale, t.w * p.q_scale);
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < PPL; ++e) acc2[i][e] = make_float2(0.f, 0.f);
+            m_run[i] = -INFINITY;
+            l_run[i] = 0.f;
+            slope[i] = p.slopes ? __ldg(p.slopes + h0 + i) * 1.4426950408889634f : 0.f;
+        }
+    }
+    // dot products of the tile's 16 tokens; `released` is called once the tile has been read
+    template <typename F>
+    __device__ __forceinline__ void scores(const ScoreParams& p, const ScoreItem& it, const uint8_t* ktile, uint32_t meta, int tok0, int nskip, int nvalid,
+                                           int lane, F released) {
+        float sc[G][ITER];
+#pragma unroll
+        for (int i = 0; i < ITER; ++i) {
+            const int t = (i * RPW + rg) & (kBlockTokens - 1);
+            float2 d2[G];
+#pragma unroll
+            for (int h = 0; h < G; ++h) d2[h] = make_float2(0.f, 0.f);
+#pragma unroll
+            for (int cp = 0; cp < CPL; ++cp) {
+                const uint4 w = *reinterpret_cast<const uint4*>(ktile + t * ROWB + (g + 32 * cp) * 16);
+                float2 f[PPC];
+                unpack2<KV>(w, f);
+#pragma unroll
+                for (int h = 0; h < G; ++h)
+#pragma unroll
+                    for (int e = 0; e < PPC; ++e) d2[h] = fma2(q2[h][cp * PPC + e], f[e], d2[h]);
+            }
+#pragma unroll
+            for (int h = 0; h < G; ++h) sc[h][i] = d2[h].x + d2[h].y;
+        }
+        released();
+        const bool visible = my_tok >= nskip && my_tok < nvalid;
+        const float dist = p.slopes ? score_distance(p, it, meta, tok0, my_tok, visible) : 0.f;
+#pragma unroll
+        for (int h = 0; h < G; ++h) {
+            RowReduce<ITER, LPR / 2>::run(sc[h], lane);
+            float x = score_modify(p, sc[h][0], slope[h], dist);
+            if (p.scores && (meta & kSuFixed) && visible && one_of_pair) score_record(p, (size_t)it.index * G + h, tok0 + my_tok, x);
+            x = visible ? x : -INFINITY;
+            // online softmax, one running maximum per row group
+            float mt = x;
+#pragma unroll
+            for (int d = LPR / 2; d >= 2; d >>= 1) mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, d));
+            const float m_new = fmaxf(m_run[h], mt);
+            const float m_safe = (m_new == -INFINITY) ? 0.f : m_new;
+            const float alpha = fast_exp2(m_run[h] - m_safe);
+            pr[h] = fast_exp2(x - m_safe);
+            l_run[h] = l_run[h] * alpha + pr[h];
+            m_run[h] = m_new;
+            const float2 alpha2 = make_float2(alpha, alpha);
+#pragma unroll
+            for (int e = 0; e < PPL; ++e) acc2[h][e] = mul2(acc2[h][e], alpha2);
+        }
+    }
+    __device__ __forceinline__ void values(const uint8_t* vtile, int nskip, int nvalid, int) {
+        const bool all = nvalid == kBlockTokens && nskip == 0;
+#pragma unroll
+        for (int i = 0; i < ITER; ++i) {
+            const int t = i * RPW + rg;
+            float2 pi2[G];
+#pragma unroll
+            for (int h = 0; h < G; ++h) {
+                const float pi = (LPR >= 2) ? __shfl_sync(0xffffffffu, pr[h], rg * LPR + 2 * i) : pr[h];
+                pi2[h] = make_float2(pi, pi);
+            }
+            if (all ? (RPW <= kBlockTokens || t < kBlockTokens) : (t >= nskip && t < nvalid)) {  // rows outside may hold anything
+#pragma unroll
+                for (int cp = 0; cp < CPL; ++cp) {
+                    const uint4 w = *reinterpret_cast<const uint4*>(vtile + t * ROWB + (g + 32 * cp) * 16);
+                    float2 f[PPC];
+                    unpack2<KV>(w, f);
+#pragma unroll
+                    for (int h = 0; h < G; ++h)
+#pragma unroll
+                        for (int e = 0; e < PPC; ++e) acc2[h][cp * PPC + e] = fma2(pi2[h], f[e], acc2[h][cp * PPC + e]);
+                }
+            }
+        }
+    }
+    // the item's result, or this segment's partial into slot my_slot
+    __device__ __forceinline__ void emit(const ScoreParams& p, const ScoreItem& it, bool whole, int my_slot, int lane) {
+#pragma unroll
+        for (int h = 0; h < G; ++h) {
+            float mx = m_run[h];
+#pragma unroll
+            for (int d = LPR; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+            const float mx_safe = (mx == -INFINITY) ? 0.f : mx;
+            const float wgt = fast_exp2(m_run[h] - mx_safe);
+            float lsum = l_run[h] * wgt;
+#pragma unroll
+            for (int d = 16; d >= 1; d >>= 1) lsum += __shfl_xor_sync(0xffffffffu, lsum, d);
+            if (LPR >= 2) lsum *= 0.5f;  // the two lanes of a pair carry the same token
+            float acc[EPL];
+#pragma unroll
+            for (int e = 0; e < PPL; ++e) {
+                acc[2 * e] = acc2[h][e].x * wgt;
+                acc[2 * e + 1] = acc2[h][e].y * wgt;
+            }
+#pragma unroll
+            for (int e = 0; e < EPL; ++e)
+#pragma unroll
+                for (int d = LPR; d < 32; d <<= 1) acc[e] += __shfl_xor_sync(0xffffffffu, acc[e], d);
+            const float inv = lsum == 0.f ? 0.f : 1.f / lsum;
+            if (lane < LPR) {
+                float* dst = p.part_acc + (size_t)my_slot * (G * HD) + h * HD;
+                const size_t at = ((size_t)it.index * G + h) * HD;
+#pragma unroll
+                for (int cp = 0; cp < CPL; ++cp)
+#pragma unroll
+                    for (int e = 0; e < EPC; e += 4) {
+                        const int d0 = (g + 32 * cp) * EPC + e;
+                        const float* a = acc + cp * EPC + e;
+                        if (!whole)
+                            __stcg(reinterpret_cast<float4*>(dst + d0), make_float4(a[0], a[1], a[2], a[3]));
+                        else if (p.out_bf16)
+                            *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + at + d0) = make_uint2(rn_bf16x2(a[0] * inv, a[1] * inv), rn_bf16x2(a[2] * inv, a[3] * inv));
+                        else
+                            *reinterpret_cast<float4*>(static_cast<float*>(p.out) + at + d0) = make_float4(a[0] * inv, a[1] * inv, a[2] * inv, a[3] * inv);
+                    }
+            }
+            if (lane == 0) {
+                if (!whole) __stcg(reinterpret_cast<float2*>(p.part_ml + (size_t)my_slot * (2 * G) + 2 * h), make_float2(mx, lsum));
+                else if (p.scores) *reinterpret_cast<float2*>(p.score_ml + 2 * ((size_t)it.index * G + h)) = make_float2(mx_safe, inv);
+            }
+        }
+    }
+};
+
+// -------------------------------------------------------------------------------------------------
+// consumer on the tensor cores (mma.sync m16n8k16), for two or four query heads of a bf16 KV head: a product per head on the CUDA
+// cores costs as many instructions as the memory leaves time for, and here the heads are columns that cost nothing.  fp32 operands
+// (queries, weights) go in as three bf16 whose sum is exact to 24 bits, as columns of their own:
+//   scores   S[16 tokens][8 columns] = K[16 x HD] Q^T: A is the tile's rows, lane (g, c) = (lane / 4, lane % 4) reads chunks
+//            c + 4 i of rows g and g + 8 -- the order of the dims is the same permutation for Q, so no element is moved;
+//   values   out^T[HD][8] = V^T[HD x 16 tokens] P: lane (g, c) reads chunk(s) g of tokens 2c, 2c + 1, 2c + 8, 2c + 9 and pairs
+//            the tokens' elements with byte permutes; P comes from the lanes that hold the scores by four shuffles.
+// Column n of a product is part n % (8 / G) of head n / (8 / G); with four heads the third parts are a second product into the same
+// accumulators (the columns of a head are summed in the end, whatever they hold).  Two-way (K) and four-way (V) bank conflicts
+// of the unswizzled tiles are left: they stay below the time the tile takes to arrive.
+// -------------------------------------------------------------------------------------------------
+__device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// Part 0, 1 or 2 of the split of two values into three bf16 each, packed.
+__device__ __forceinline__ uint32_t split3(float a, float b, int part) {
+    const uint32_t hi = rn_bf16x2(a, b);
+    if (part == 0) return hi;
+    const float ra = a - bf16_lo(hi), rb = b - bf16_hi(hi);
+    const uint32_t mid = rn_bf16x2(ra, rb);
+    if (part == 1) return mid;
+    return part == 2 ? rn_bf16x2(ra - bf16_lo(mid), rb - bf16_hi(mid)) : 0u;
+}
+
+template <int HD, int G>
+struct ScoreMma {
+    static_assert((HD == 64 || HD == 128) && (G == 2 || G == 4), "what the fragments below are laid out for");
+    static constexpr int kGroup = G, kTile = kBlockTokens * HD * 2, kThreads = 384;  // 12 warps: 168 registers a thread
+    static constexpr int NT = G == 4 ? 2 : 1;   // products per K / V fragment
+    static constexpr int CH = HD / 32;          // chunks of a K row per lane
+    static constexpr int MT = HD / 16;          // 16-dim tiles of the accumulator
+    static constexpr int VC = HD / 64;          // chunks of a V row per lane
+    static constexpr int ROWB = HD * 2;
+
+    uint4 qf[NT][CH];
+    float acc[MT][4];
+    float p0, p1;  // weights of tokens g and g + 8, of this lane's head
+    float m_run, l_run, slope;
+    int g, c, head;
+
+    __device__ __forceinline__ void init(int lane) {
+        g = lane >> 2;
+        c = lane & 3;
+        head = G == 4 ? c : c >> 1;  // whose scores and accumulator columns (2c, 2c + 1) this lane holds
+    }
+    __device__ __forceinline__ int part_of(int column, int nt) const {
+        return G == 4 ? (nt == 0 ? column & 1 : (column & 1) ? 3 : 2) : column & 3;  // 3: nothing
+    }
+    __device__ __forceinline__ void load(const ScoreParams& p, const ScoreItem& it) {
+        const int col_head = G == 4 ? g >> 1 : g >> 2;  // column g of the B operand
+        const size_t at = ((size_t)it.index * G + col_head) * HD;
+#pragma unroll
+        for (int i = 0; i < CH; ++i) {
+            const int d0 = (c + 4 * i) * 8;
+            float f[8];
+            if (p.q_bf16) {
+                BF16::unpack(__ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.q) + at + d0)), f);
+            } else {
+                const float4 a = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(p.q) + at + d0));
+                const float4 b = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(p.q) + at + d0 + 4));
+                f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w;
+                f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
+            }
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                const int part = part_of(g, nt);
+                qf[nt][i] = make_uint4(split3(f[0], f[1], part), split3(f[2], f[3], part), split3(f[4], f[5], part), split3(f[6], f[7], part));
+            }
+        }
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[m][e] = 0.f;
+        m_run = -INFINITY;
+        l_run = 0.f;
+        slope = p.slopes ? __ldg(p.slopes + (int)(it.index % (uint32_t)p.plan.items_per_row) * G + head) * 1.4426950408889634f : 0.f;
+    }
+    template <typename F>
+    __device__ __forceinline__ void scores(const ScoreParams& p, const ScoreItem& it, const uint8_t* ktile, uint32_t meta, int tok0, int nskip, int nvalid,
+                                           int, F released) {
+        uint4 lo[CH], hi[CH];  // rows g and g + 8
+#pragma unroll
+        for (int i = 0; i < CH; ++i) {
+            lo[i] = *reinterpret_cast<const uint4*>(ktile + g * ROWB + (c + 4 * i) * 16);
+            hi[i] = *reinterpret_cast<const uint4*>(ktile + (g + 8) * ROWB + (c + 4 * i) * 16);
+        }
+        released();
+        float s0[4] = {0.f, 0.f, 0.f, 0.f}, s1[4] = {0.f, 0.f, 0.f, 0.f};  // two chains
+#pragma unroll
+        for (int i = 0; i < CH; ++i)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                mma_16816(s0, lo[i].x, hi[i].x, lo[i].y, hi[i].y, qf[nt][i].x, qf[nt][i].y);
+                mma_16816(s1, lo[i].z, hi[i].z, lo[i].w, hi[i].w, qf[nt][i].z, qf[nt][i].w);
+            }
+        float x0 = (s0[0] + s1[0]) + (s0[1] + s1[1]), x1 = (s0[2] + s1[2]) + (s0[3] + s1[3]);
+        if constexpr (G == 2) {  // the third part is in the neighbour's columns
+            x0 += __shfl_xor_sync(0xffffffffu, x0, 1);
+            x1 += __shfl_xor_sync(0xffffffffu, x1, 1);
+        }
+        const bool v0 = g >= nskip && g < nvalid, v1 = g + 8 >= nskip && g + 8 < nvalid;
+        float d0 = 0.f, d1 = 0.f;
+        if (p.slopes) {
+            d0 = score_distance(p, it, meta, tok0, g, v0);
+            d1 = score_distance(p, it, meta, tok0, g + 8, v1);
+        }
+        x0 = score_modify(p, x0 * p.q_scale, slope, d0);
+        x1 = score_modify(p, x1 * p.q_scale, slope, d1);
+        if (p.scores && (meta & kSuFixed) && (G == 4 || !(c & 1))) {
+            if (v0) score_record(p, (size_t)it.index * G + head, tok0 + g, x0);
+            if (v1) score_record(p, (size_t)it.index * G + head, tok0 + g + 8, x1);
+        }
+        x0 = v0 ? x0 : -INFINITY;
+        x1 = v1 ? x1 : -INFINITY;
+        float mt = fmaxf(x0, x1);
+#pragma unroll
+        for (int d = 4; d <= 16; d <<= 1) mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, d));
+        const float m_new = fmaxf(m_run, mt);
+        const float m_safe = (m_new == -INFINITY) ? 0.f : m_new;
+        const float alpha = fast_exp2(m_run - m_safe);
+        p0 = fast_exp2(x0 - m_safe);
+        p1 = fast_exp2(x1 - m_safe);
+        l_run = l_run * alpha + (p0 + p1);
+        const bool moved = m_new != m_run;
+        m_run = m_new;
+        if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[m][e] *= alpha;
+        }
+    }
+    __device__ __forceinline__ void values(const uint8_t* vtile, int nskip, int nvalid, int) {
+        // weights of tokens 2c, 2c + 1, 2c + 8, 2c + 9 for column g
+        const int col_head = G == 4 ? g >> 1 : (g >> 2) * 2;
+        const float w0 = __shfl_sync(0xffffffffu, p0, 8 * c + col_head), w1 = __shfl_sync(0xffffffffu, p0, 8 * c + 4 + col_head);
+        const float w2 = __shfl_sync(0xffffffffu, p1, 8 * c + col_head), w3 = __shfl_sync(0xffffffffu, p1, 8 * c + 4 + col_head);
+        uint32_t b[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            b[nt][0] = split3(w0, w1, part_of(g, nt));
+            b[nt][1] = split3(w2, w3, part_of(g, nt));
+        }
+        uint4 v[VC][4];
+#pragma unroll
+        for (int k = 0; k < VC; ++k)
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                const int tok = 2 * c + (t & 1) + (t >> 1) * 8;
+                v[k][t] = *reinterpret_cast<const uint4*>(vtile + tok * ROWB + (g + 8 * k) * 16);
+                if ((nskip > 0 || nvalid < kBlockTokens) && !(tok >= nskip && tok < nvalid)) v[k][t] = make_uint4(0u, 0u, 0u, 0u);  // may hold anything
+            }
+        // element e of chunk k, as (token 2c, token 2c + 1) and (2c + 8, 2c + 9) pairs
+        auto word = [](const uint4& w, int e) { return e < 2 ? w.x : e < 4 ? w.y : e < 6 ? w.z : w.w; };
+        auto pair = [&](int k, int e, int t) { return __byte_perm(word(v[k][t], e), word(v[k][t + 1], e), (e & 1) ? 0x7632 : 0x5410); };
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+            // rows g and g + 8 of the 16-dim tile: with 128 dims element m of chunks g and g + 8, with 64 elements m and m + 4 of chunk g
+            constexpr bool kTwo = VC == 2;
+            const int k1 = kTwo ? 1 : 0, e1 = kTwo ? m : m + 4;
+            const uint32_t a0 = pair(0, m, 0), a1 = pair(k1, e1, 0), a2 = pair(0, m, 2), a3 = pair(k1, e1, 2);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) mma_16816(acc[m], a0, a1, a2, a3, b[nt][0], b[nt][1]);
+        }
+    }
+    __device__ __forceinline__ void emit(const ScoreParams& p, const ScoreItem& it, bool whole, int my_slot, int) {
+        const float m_safe = (m_run == -INFINITY) ? 0.f : m_run;
+        float lsum = l_run;
+#pragma unroll
+        for (int d = 4; d <= 16; d <<= 1) lsum += __shfl_xor_sync(0xffffffffu, lsum, d);
+        const float inv = lsum == 0.f ? 0.f : 1.f / lsum;
+        float lo[MT], hi[MT];  // rows g, g + 8 of the tiles
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+            lo[m] = acc[m][0] + acc[m][1];
+            hi[m] = acc[m][2] + acc[m][3];
+            if constexpr (G == 2) {
+                lo[m] += __shfl_xor_sync(0xffffffffu, lo[m], 1);
+                hi[m] += __shfl_xor_sync(0xffffffffu, hi[m], 1);
+            }
+        }
+        const size_t at = ((size_t)it.index * G + head) * HD;
+        float* part = p.part_acc + (size_t)my_slot * (G * HD) + head * HD;
+        auto put = [&](int chunk, float (&f)[8]) {
+            if (whole) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) f[e] *= inv;
+                score_store8(p, at + chunk * 8, f);
+            } else {
+                __stcg(reinterpret_cast<float4*>(part + chunk * 8), make_float4(f[0], f[1], f[2], f[3]));
+                __stcg(reinterpret_cast<float4*>(part + chunk * 8 + 4), make_float4(f[4], f[5], f[6], f[7]));
+            }
+        };
+        if constexpr (VC == 2) {
+            float f[8];
+            if (G == 4 || !(c & 1)) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) f[e] = lo[e];
+                put(g, f);
+            }
+            if (G == 4 || (c & 1)) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) f[e] = hi[e];
+                put(g + 8, f);
+            }
+        } else if (G == 4 || !(c & 1)) {
+            float f[8];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                f[e] = lo[e];
+                f[4 + e] = hi[e];
+            }
+            put(g, f);
+        }
+        if (g == 0 && (G == 4 || !(c & 1))) {
+            if (!whole) __stcg(reinterpret_cast<float2*>(p.part_ml + (size_t)my_slot * (2 * G) + 2 * head), make_float2(m_run, lsum));
+            else if (p.scores) *reinterpret_cast<float2*>(p.score_ml + 2 * ((size_t)it.index * G + head)) = make_float2(m_safe, inv);
+        }
+    }
+};
+
+template <typename C, int HD>
+__global__ void __launch_bounds__(C::kThreads, 1) rswa_scored_kernel(const __grid_constant__ ScoreParams p) {
+    constexpr int G = C::kGroup, TILE = C::kTile;
     constexpr unsigned FULL = 0xffffffffu;
 
     extern __shared__ __align__(128) uint8_t smem[];
@@ -230,10 +662,8 @@ __global__ void __launch_bounds__(kScoreThreads, 1) rswa_scored_kernel(const __g
     const long long u0 = pm.start(piece);
     const long long n_units = pm.end(piece) - u0;
 
-    const int g = lane % LPR;   // chunk position inside the row
-    const int rg = lane / LPR;  // which of the RPW rows of a warp-wide load
-    const int my_tok = (LPR >= 2 ? (g >> 1) * RPW : 0) + rg;  // the token whose score this lane ends up with
-    const bool one_of_pair = LPR < 2 || (g & 1) == 0;
+    C work;
+    work.init(lane);
 
     // ---- unit descriptors: lane l describes unit desc_base + l of this piece ----------------------------
     uint32_t d_tile = 0, d_meta = 0, d_item = 0;
@@ -324,47 +754,15 @@ __global__ void __launch_bounds__(kScoreThreads, 1) rswa_scored_kernel(const __g
         return t;
     };
 
-    // ---- the item under way ------------------------------------------------------------------------------
-    float2 q2[G][PPL], acc2[G][PPL];
-    float m_run[G], l_run[G], slope[G];
-    int cur_slot = 0, cur_q_pos = 0;
-    auto load_item = [&](uint32_t item) {
-        const size_t at = (size_t)item * (G * HD);  // items_per_row * G == heads
-#pragma unroll
-        for (int i = 0; i < G; ++i) {
-#pragma unroll
-            for (int cp = 0; cp < CPL; ++cp) {
-                const int d0 = (g + 32 * cp) * EPC;
-#pragma unroll
-                for (int e = 0; e < EPC; e += 4) {
-                    float4 t;
-                    if (p.q_bf16) {
-                        const uint2 w = __ldg(reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p.q) + at + i * HD + d0 + e));
-                        t = make_float4(bf16_lo(w.x), bf16_hi(w.x), bf16_lo(w.y), bf16_hi(w.y));
-                    } else {
-                        t = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(p.q) + at + i * HD + d0 + e));
-                    }
-                    q2[i][(cp * EPC + e) / 2] = make_float2(t.x * p.q_scale, t.y * p.q_scale);
-                    q2[i][(cp * EPC + e) / 2 + 1] = make_float2(t.z * p.q_scale, t.w * p.q_scale);
-                }
-            }
-#pragma unroll
-            for (int e = 0; e < PPL; ++e) acc2[i][e] = make_float2(0.f, 0.f);
-            m_run[i] = -INFINITY;
-            l_run[i] = 0.f;
-        }
-        const int r = (int)(item / (uint32_t)items_per_row);
+    ScoreItem item{};
+    auto start_item = [&](uint32_t index) {
+        item.index = index;
         if (p.slopes) {
-            const int h0 = (int)(item - (uint32_t)r * (uint32_t)items_per_row) * G;
-#pragma unroll
-            for (int i = 0; i < G; ++i) slope[i] = __ldg(p.slopes + h0 + i) * 1.4426950408889634f;
-            cur_slot = info[r].slot;
-            cur_q_pos = info[r].q_pos;
+            const ScoreRow& o = info[index / (uint32_t)items_per_row];
+            item.slot = o.slot;
+            item.q_pos = o.q_pos;
         }
-    };
-    auto store_out = [&](size_t at, float a, float b, float c, float d) {
-        if (p.out_bf16) *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + at) = make_uint2(rn_bf16x2(a, b), rn_bf16x2(c, d));
-        else *reinterpret_cast<float4*>(static_cast<float*>(p.out) + at) = make_float4(a, b, c, d);
+        work.load(p, item);
     };
 
     uint32_t pend[2];  // items this piece left a partial of: the first and the last
@@ -373,8 +771,7 @@ __global__ void __launch_bounds__(kScoreThreads, 1) rswa_scored_kernel(const __g
     build_desc(0);
 #pragma unroll
     for (int s = 0; s < kScoreRing; ++s) issue_next();
-    uint32_t cur_item = __shfl_sync(FULL, d_item, 0);
-    load_item(cur_item);
+    start_item(__shfl_sync(FULL, d_item, 0));
     bool first_segment = true, gave_up = false;
     bool from_start = (__shfl_sync(FULL, d_meta, 0) & kSuFirst) != 0;
 
@@ -384,97 +781,15 @@ __global__ void __launch_bounds__(kScoreThreads, 1) rswa_scored_kernel(const __g
         const int tok0 = __shfl_sync(FULL, d_tok, (int)(it - desc_base));
         const int nvalid = (int)(meta & kSuValid), nskip = (int)((meta >> kSuSkipShift) & 15);
 
-        // ---- scores of the tile's 16 tokens -------------------------------------------------------------
         const uint8_t* ktile = wait_tile();
         if (!ktile) { gave_up = true; break; }
-        float sc[G][ITER];
-#pragma unroll
-        for (int i = 0; i < ITER; ++i) {
-            const int t = (i * RPW + rg) & (kBlockTokens - 1);
-            float2 d2[G];
-#pragma unroll
-            for (int h = 0; h < G; ++h) d2[h] = make_float2(0.f, 0.f);
-#pragma unroll
-            for (int cp = 0; cp < CPL; ++cp) {
-                const uint4 w = *reinterpret_cast<const uint4*>(ktile + t * ROWB + (g + 32 * cp) * 16);
-                float2 f[PPC];
-                unpack2<KV>(w, f);
-#pragma unroll
-                for (int h = 0; h < G; ++h)
-#pragma unroll
-                    for (int e = 0; e < PPC; ++e) d2[h] = fma2(q2[h][cp * PPC + e], f[e], d2[h]);
-            }
-#pragma unroll
-            for (int h = 0; h < G; ++h) sc[h][i] = d2[h].x + d2[h].y;
-        }
-        __syncwarp();
-        issue_next();  // the K slot is free
-
-        const bool visible = my_tok >= nskip && my_tok < nvalid;
-        float dist = 0.f;
-        if (p.slopes) {
-            int a;
-            if (meta & kSuFixed) {
-                int at = tok0 + my_tok;
-                if (p.d_key_pos && visible && at < p.key_pos_stride) at = __ldg(p.d_key_pos + (size_t)cur_slot * p.key_pos_stride + at);
-                dist = __uint2float_rn((uint32_t)max(cur_q_pos, at) - (uint32_t)min(cur_q_pos, at));
-            } else {
-                a = tok0 - my_tok;
-                if (a < 0) a += p.plan.window;
-                dist = (float)a;
-            }
-        }
-        float pr[G];
-#pragma unroll
-        for (int h = 0; h < G; ++h) {
-            RowReduce<ITER, LPR / 2>::run(sc[h], lane);
-            float x = sc[h][0];
-            if (p.cap_log2 > 0.f) x = p.cap_log2 * tanhf(x);
-            if (p.slopes) x = fmaf(-slope[h], dist, x);
-            if (p.scores && (meta & kSuFixed) && visible && one_of_pair && tok0 + my_tok < p.score_stride)
-                __stcs(p.scores + ((size_t)cur_item * G + h) * p.score_stride + tok0 + my_tok, x);
-            x = visible ? x : -INFINITY;
-            // ---- online softmax, one running maximum per row group -----------------------------------------
-            float mt = x;
-#pragma unroll
-            for (int d = LPR / 2; d >= 2; d >>= 1) mt = fmaxf(mt, __shfl_xor_sync(FULL, mt, d));
-            const float m_new = fmaxf(m_run[h], mt);
-            const float m_safe = (m_new == -INFINITY) ? 0.f : m_new;
-            const float alpha = fast_exp2(m_run[h] - m_safe);
-            pr[h] = fast_exp2(x - m_safe);
-            l_run[h] = l_run[h] * alpha + pr[h];
-            m_run[h] = m_new;
-            const float2 alpha2 = make_float2(alpha, alpha);
-#pragma unroll
-            for (int e = 0; e < PPL; ++e) acc2[h][e] = mul2(acc2[h][e], alpha2);
-        }
-
-        // ---- acc += p . v ------------------------------------------------------------------------------------
+        work.scores(p, item, ktile, meta, tok0, nskip, nvalid, lane, [&]() {
+            __syncwarp();
+            issue_next();  // the K slot is free
+        });
         const uint8_t* vtile = wait_tile();
         if (!vtile) { gave_up = true; break; }
-        const bool all = nvalid == kBlockTokens && nskip == 0;
-#pragma unroll
-        for (int i = 0; i < ITER; ++i) {
-            const int t = i * RPW + rg;
-            float2 pi2[G];
-#pragma unroll
-            for (int h = 0; h < G; ++h) {
-                const float pi = (LPR >= 2) ? __shfl_sync(FULL, pr[h], rg * LPR + 2 * i) : pr[h];
-                pi2[h] = make_float2(pi, pi);
-            }
-            if (all ? (RPW <= kBlockTokens || t < kBlockTokens) : (t >= nskip && t < nvalid)) {  // rows outside may hold anything
-#pragma unroll
-                for (int cp = 0; cp < CPL; ++cp) {
-                    const uint4 w = *reinterpret_cast<const uint4*>(vtile + t * ROWB + (g + 32 * cp) * 16);
-                    float2 f[PPC];
-                    unpack2<KV>(w, f);
-#pragma unroll
-                    for (int h = 0; h < G; ++h)
-#pragma unroll
-                        for (int e = 0; e < PPC; ++e) acc2[h][cp * PPC + e] = fma2(pi2[h], f[e], acc2[h][cp * PPC + e]);
-                }
-            }
-        }
+        work.values(vtile, nskip, nvalid, lane);
         __syncwarp();
         issue_next();  // the V slot is free
 
@@ -482,55 +797,12 @@ __global__ void __launch_bounds__(kScoreThreads, 1) rswa_scored_kernel(const __g
         const bool item_done = (meta & kSuLast) != 0, piece_done = it == n_units - 1;
         if (item_done || piece_done) {
             const bool whole = item_done && from_start;
-            const int my_slot = 2 * piece + (first_segment ? 0 : 1);
-#pragma unroll
-            for (int h = 0; h < G; ++h) {
-                float mx = m_run[h];
-#pragma unroll
-                for (int d = LPR; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(FULL, mx, d));
-                const float mx_safe = (mx == -INFINITY) ? 0.f : mx;
-                const float wgt = fast_exp2(m_run[h] - mx_safe);
-                float lsum = l_run[h] * wgt;
-#pragma unroll
-                for (int d = 16; d >= 1; d >>= 1) lsum += __shfl_xor_sync(FULL, lsum, d);
-                if (LPR >= 2) lsum *= 0.5f;  // the two lanes of a pair carry the same token
-                float acc[EPL];
-#pragma unroll
-                for (int e = 0; e < PPL; ++e) {
-                    acc[2 * e] = acc2[h][e].x * wgt;
-                    acc[2 * e + 1] = acc2[h][e].y * wgt;
-                }
-#pragma unroll
-                for (int e = 0; e < EPL; ++e)
-#pragma unroll
-                    for (int d = LPR; d < 32; d <<= 1) acc[e] += __shfl_xor_sync(FULL, acc[e], d);
-                const float inv = lsum == 0.f ? 0.f : 1.f / lsum;
-                if (lane < LPR) {
-                    float* dst = p.part_acc + (size_t)my_slot * (G * HD) + h * HD;
-#pragma unroll
-                    for (int cp = 0; cp < CPL; ++cp)
-#pragma unroll
-                        for (int e = 0; e < EPC; e += 4) {
-                            const int d0 = (g + 32 * cp) * EPC + e;
-                            const float* a = acc + cp * EPC + e;
-                            if (whole) store_out((size_t)cur_item * (G * HD) + h * HD + d0, a[0] * inv, a[1] * inv, a[2] * inv, a[3] * inv);
-                            else __stcg(reinterpret_cast<float4*>(dst + d0), make_float4(a[0], a[1], a[2], a[3]));
-                        }
-                }
-                if (lane == 0) {
-                    if (whole) {
-                        if (p.scores) *reinterpret_cast<float2*>(p.score_ml + 2 * ((size_t)cur_item * G + h)) = make_float2(mx_safe, inv);
-                    } else {
-                        __stcg(reinterpret_cast<float2*>(p.part_ml + (size_t)my_slot * (2 * G) + 2 * h), make_float2(mx, lsum));
-                    }
-                }
-            }
-            if (!whole) pend[pend_n++ & 1] = cur_item;
+            work.emit(p, item, whole, 2 * piece + (first_segment ? 0 : 1), lane);
+            if (!whole) pend[pend_n++ & 1] = item.index;
             first_segment = false;
             if (!piece_done) {
-                cur_item = __shfl_sync(FULL, d_item, (int)(it + 1 - desc_base));
+                start_item(__shfl_sync(FULL, d_item, (int)(it + 1 - desc_base)));
                 from_start = true;
-                load_item(cur_item);
             }
         }
     }
@@ -548,10 +820,10 @@ __global__ void __launch_bounds__(kScoreThreads, 1) rswa_scored_kernel(const __g
     // ---- arrivals: whoever completes an item's set of partials joins them ------------------------------------
     __syncwarp();  // the partial stores of every lane come before the arriving lane's release
     for (int k = 0; k < pend_n; ++k) {
-        const uint32_t item = pend[k];
-        const int r = (int)(item / (uint32_t)items_per_row);
+        const uint32_t done = pend[k];
+        const int r = (int)(done / (uint32_t)items_per_row);
         const int n = (int)((rs[r + 1] - rs[r]) / items_per_row);
-        const long long s0 = rs[r] + (long long)(item - (uint32_t)r * (uint32_t)items_per_row) * n;
+        const long long s0 = rs[r] + (long long)(done - (uint32_t)r * (uint32_t)items_per_row) * n;
         const int wf = pm.of(s0), wl = pm.of(s0 + n - 1);
         int old = 0;
         if (lane == 0)  // release: this warp's partials (ordered before by the barrier above); acquire: the others'
@@ -611,12 +883,12 @@ __global__ void __launch_bounds__(kScoreThreads, 1) rswa_scored_kernel(const __g
             for (int kk = 0; kk < NK; ++kk) {
                 const int d = lane + 32 * kk;
                 if (d < HD) {
-                    const size_t at = (size_t)item * (G * HD) + h * HD + d;
+                    const size_t at = (size_t)done * (G * HD) + h * HD + d;
                     if (p.out_bf16) static_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(o[kk] * inv);
                     else static_cast<float*>(p.out)[at] = o[kk] * inv;
                 }
             }
-            if (p.scores && lane == 0) *reinterpret_cast<float2*>(p.score_ml + 2 * ((size_t)item * G + h)) = make_float2(m_safe, inv);
+            if (p.scores && lane == 0) *reinterpret_cast<float2*>(p.score_ml + 2 * ((size_t)done * G + h)) = make_float2(m_safe, inv);
         }
         if (lane == 0) p.counters[wf] = 0;  // for the next launch
     }
