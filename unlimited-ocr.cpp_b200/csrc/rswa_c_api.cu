@@ -101,6 +101,10 @@ int uocr_b200_workspace_create(int max_rows, uocr_b200_workspace** out) {
     cudaGetDevice(&ws->device);
     ws->max_rows = max_rows;
     ws->total_warps_max = di->sms * kMaxWarpsPerCta;
+    if (ws->total_warps_max > 4096) {
+        delete ws;
+        return fail(UOCR_B200_ERR_UNSUPPORTED, "workspace_create: more SMs than the partial results are laid out for");
+    }
     auto up = [](size_t x) { return (x + 255) & ~size_t(255); };
     const size_t o_status = 0;
     const size_t o_rs = up(256);
@@ -115,7 +119,8 @@ int uocr_b200_workspace_create(int max_rows, uocr_b200_workspace** out) {
     const size_t o_count = o_order + up(sizeof(TcWork) * (size_t)ws->tiles_cap);
     const size_t o_srow = o_count + 256;
     const size_t o_srs = o_srow + up(kScoreRowBytes * (size_t)max_rows);
-    ws->bytes = o_srs + up(sizeof(long long) * (size_t)(max_rows + 1));
+    const size_t o_scnt = o_srs + up(sizeof(long long) * (size_t)(max_rows + 1));
+    ws->bytes = o_scnt + up(sizeof(int) * 2 * kScoreJoinLevels * (size_t)ws->pieces_max);
     cudaError_t e = cudaMalloc(&ws->base, ws->bytes);
     if (e != cudaSuccess) {
         delete ws;
@@ -139,6 +144,7 @@ int uocr_b200_workspace_create(int max_rows, uocr_b200_workspace** out) {
     ws->item_counter = reinterpret_cast<int*>(ws->base + o_count);
     ws->score_rows = reinterpret_cast<ScoreRow*>(ws->base + o_srow);
     ws->score_rs = reinterpret_cast<long long*>(ws->base + o_srs);
+    ws->score_counters = reinterpret_cast<int*>(ws->base + o_scnt);
     *out = ws;
     return UOCR_B200_OK;
 }
@@ -240,6 +246,8 @@ int uocr_b200_workspace_status(uocr_b200_workspace* ws, uocr_b200_stream_t strea
     if (v != 0 && ws->counters) {
         // a kernel that gave up may have left arrival counters half-way: start clean again
         CHECK_CUDA(cudaMemsetAsync(ws->counters, 0, sizeof(int) * ((size_t)ws->pieces_max + 64), st), "counter clear");
+        if (ws->score_counters)
+            CHECK_CUDA(cudaMemsetAsync(ws->score_counters, 0, sizeof(int) * 2 * kScoreJoinLevels * (size_t)ws->pieces_max, st), "counter clear");
         if (ws->item_counter) CHECK_CUDA(cudaMemsetAsync(ws->item_counter, 0, 2 * sizeof(int), st), "item counter clear");
         CHECK_CUDA(cudaStreamSynchronize(st), "counter clear sync");
     }

@@ -7,8 +7,8 @@
 // The work model is that of the plain attention kernel: the 16-token tiles a row's heads can see are laid
 // out on one line and cut into equal pieces, one per warp of a persistent grid, so a batch of one long
 // sequence and a batch of many short ones load the SMs alike; a warp streams its piece's K and V tiles
-// through a private ring of shared memory with bulk copies, and the last warp to finish an item that
-// straddles pieces joins the partial results (maximum, sum, accumulator).  What differs:
+// through a private ring of shared memory with bulk copies, and the partial results (maximum, sum,
+// accumulator) of an item that straddles pieces are joined by the warps that finish last.  What differs:
 //   - an item is a row and up to four query heads of one KV head (G), so grouped heads read a tile once, and where it pays
 //     (bf16, head_dim 64 or 128) their products run on the tensor cores;
 //   - only tiles that hold a visible token are on the line: the cost of a page is the page;
@@ -83,11 +83,14 @@ struct ScoreParams {
     long long* rs;
     float* part_acc;  // [2 * pieces][G * head_dim]
     float* part_ml;   // [2 * pieces][2 G]
-    int* counters;
+    int* counters;  // [2 kScoreJoinLevels][pieces] arrival counters of the joins, zero between launches
+    int pieces;
     int* status;
     uint32_t wait_limit;
     int total_warps;
 };
+
+constexpr int kScoreJoin = 8;  // partials joined at a time
 
 constexpr int kScoreSharedRows = 512;  // rows a CTA plans in its own shared memory
 
@@ -817,80 +820,87 @@ __global__ void __launch_bounds__(C::kThreads, 1) rswa_scored_kernel(const __gri
         return;
     }
 
-    // ---- arrivals: whoever completes an item's set of partials joins them ------------------------------------
-    __syncwarp();  // the partial stores of every lane come before the arriving lane's release
+    // ---- partials are joined in a tree: eight at a time, by the warp that arrives last at the eight ------------------------
+    // (One warp that joins everything is the tail of the launch when a long row is cut into many pieces: 74 partials of four heads
+    // took 40 of 100 us.)  Level l joins entries of kScoreJoin^l consecutive pieces of the item into the first one's slot; the last
+    // level writes the result.  A group's counter is that of its first piece, in an array of its own per level and for the groups
+    // that start the item (a piece can end one item and begin the next).
     for (int k = 0; k < pend_n; ++k) {
         const uint32_t done = pend[k];
         const int r = (int)(done / (uint32_t)items_per_row);
         const int n = (int)((rs[r + 1] - rs[r]) / items_per_row);
         const long long s0 = rs[r] + (long long)(done - (uint32_t)r * (uint32_t)items_per_row) * n;
-        const int wf = pm.of(s0), wl = pm.of(s0 + n - 1);
-        int old = 0;
-        if (lane == 0)  // release: this warp's partials (ordered before by the barrier above); acquire: the others'
-            asm volatile("atom.add.acq_rel.gpu.global.s32 %0, [%1], 1;" : "=r"(old) : "l"(p.counters + wf) : "memory");
-        old = __shfl_sync(FULL, old, 0);
-        if (old != wl - wf) continue;
-        const int n_part = wl - wf + 1;
+        const int wf = pm.of(s0), n_part = pm.of(s0 + n - 1) - wf + 1;
         const bool wf_second = pm.start(wf) < s0;  // the item is piece wf's second segment
         auto slot_of = [&](int i) { return (size_t)(2 * (wf + i) + ((i == 0 && wf_second) ? 1 : 0)); };
-        constexpr int NK = (HD + 31) / 32, kBatch = NK > 4 ? 4 : 8;
-#pragma unroll 1
-        for (int h = 0; h < G; ++h) {
-            // The accumulators come in batches whose loads are all issued before any is used, the first together with
-            // the (max, sum) loads: a join costs about one round trip to L2 per batch.
-            float tmp[kBatch][NK], o[NK];
-            auto load_batch = [&](int b0) {
+        int i = piece - wf;
+        for (int span = 1, level = 0;; span *= kScoreJoin, ++level) {
+            const int entries = (n_part + span - 1) / span, group = i / (span * kScoreJoin);
+            const int members = min(kScoreJoin, entries - group * kScoreJoin);
+            i = group * span * kScoreJoin;
+            if (members == 1) continue;  // the odd one out goes up as it is
+            __syncwarp();  // the stores of every lane come before the arriving lane's release
+            int* counter = p.counters + (size_t)(2 * level + (group > 0 ? 1 : 0)) * p.pieces + wf + i;
+            int old = 0;
+            if (lane == 0)  // release: this warp's partial (ordered before by the barrier above); acquire: the others'
+                asm volatile("atom.add.acq_rel.gpu.global.s32 %0, [%1], 1;" : "=r"(old) : "l"(counter) : "memory");
+            old = __shfl_sync(FULL, old, 0);
+            if (old != members - 1) break;
+            if (lane == 0) *counter = 0;  // for the next launch
+            const bool last = entries <= kScoreJoin;
+            // lane 4 m + h holds (max, sum) of member m, head h; the accumulators follow in 16-byte columns, 128 floats a round
+            const int m_lane = lane >> 2, h_lane = lane & 3;
+            const bool on = m_lane < members && h_lane < G;
+            const float2 ml = on ? __ldcg(reinterpret_cast<const float2*>(p.part_ml + slot_of(i + m_lane * span) * (2 * G) + 2 * h_lane)) : make_float2(-INFINITY, 0.f);
+            constexpr int kRounds = (G * HD + 127) / 128;
+            float4 o[kRounds];
+            float mx = ml.x;
 #pragma unroll
-                for (int i = 0; i < kBatch; ++i) {
-                    const float* pa = p.part_acc + slot_of(b0 + i) * (G * HD) + h * HD;
+            for (int d = 4; d <= 16; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(FULL, mx, d));
+            const float m_safe = (mx == -INFINITY) ? 0.f : mx;
+            const float wgt = on ? fast_exp2(ml.x - m_safe) : 0.f;
+            float lsum = on ? ml.y * wgt : 0.f;
 #pragma unroll
-                    for (int kk = 0; kk < NK; ++kk) {
-                        const int d = lane + 32 * kk;
-                        tmp[i][kk] = (b0 + i < n_part && d < HD) ? __ldcg(pa + d) : 0.f;
-                    }
-                }
-            };
-            load_batch(0);
-            float mall = -INFINITY, lall = 0.f;
-            for (int w0 = lane; w0 < n_part; w0 += 32) mall = fmaxf(mall, __ldcg(p.part_ml + slot_of(w0) * (2 * G) + 2 * h));
+            for (int d = 4; d <= 16; d <<= 1) lsum += __shfl_xor_sync(FULL, lsum, d);
 #pragma unroll
-            for (int d = 16; d >= 1; d >>= 1) mall = fmaxf(mall, __shfl_xor_sync(FULL, mall, d));
-            const float m_safe = (mall == -INFINITY) ? 0.f : mall;
+            for (int c = 0; c < kRounds; ++c) {
+                const int col = c * 128 + lane * 4;
+                float4 t[kScoreJoin];
 #pragma unroll
-            for (int kk = 0; kk < NK; ++kk) o[kk] = 0.f;
-            float wg = 0.f;
-            for (int b0 = 0; b0 < n_part; b0 += kBatch) {
-                if ((b0 & 31) == 0) {
-                    wg = 0.f;
-                    if (b0 + lane < n_part) {
-                        const float2 ml = __ldcg(reinterpret_cast<const float2*>(p.part_ml + slot_of(b0 + lane) * (2 * G) + 2 * h));
-                        wg = fast_exp2(ml.x - m_safe);
-                        lall += ml.y * wg;
-                    }
-                }
-                if (b0) load_batch(b0);
+                for (int m = 0; m < kScoreJoin; ++m)
+                    t[m] = m < members && col < G * HD ? __ldcg(reinterpret_cast<const float4*>(p.part_acc + slot_of(i + m * span) * (G * HD) + col)) : make_float4(0.f, 0.f, 0.f, 0.f);
+                const int head = min(col / HD, G - 1);
+                o[c] = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-                for (int i = 0; i < kBatch; ++i) {
-                    const float wi = __shfl_sync(FULL, wg, (b0 + i) & 31);
-#pragma unroll
-                    for (int kk = 0; kk < NK; ++kk) o[kk] = fmaf(tmp[i][kk], wi, o[kk]);
-                }
-            }
-#pragma unroll
-            for (int d = 16; d >= 1; d >>= 1) lall += __shfl_xor_sync(FULL, lall, d);
-            const float inv = lall == 0.f ? 0.f : 1.f / lall;
-#pragma unroll
-            for (int kk = 0; kk < NK; ++kk) {
-                const int d = lane + 32 * kk;
-                if (d < HD) {
-                    const size_t at = (size_t)done * (G * HD) + h * HD + d;
-                    if (p.out_bf16) static_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(o[kk] * inv);
-                    else static_cast<float*>(p.out)[at] = o[kk] * inv;
+                for (int m = 0; m < kScoreJoin; ++m) {
+                    const float w = __shfl_sync(FULL, wgt, 4 * m + head);
+                    o[c].x = fmaf(t[m].x, w, o[c].x);
+                    o[c].y = fmaf(t[m].y, w, o[c].y);
+                    o[c].z = fmaf(t[m].z, w, o[c].z);
+                    o[c].w = fmaf(t[m].w, w, o[c].w);
                 }
             }
-            if (p.scores && lane == 0) *reinterpret_cast<float2*>(p.score_ml + 2 * ((size_t)done * G + h)) = make_float2(m_safe, inv);
+            const float inv_lane = lsum == 0.f ? 0.f : 1.f / lsum;
+#pragma unroll
+            for (int c = 0; c < kRounds; ++c) {
+                const int col = c * 128 + lane * 4;
+                const float inv = __shfl_sync(FULL, inv_lane, min(col / HD, G - 1));
+                if (col >= G * HD) continue;
+                if (!last) {
+                    __stcg(reinterpret_cast<float4*>(p.part_acc + slot_of(i) * (G * HD) + col), o[c]);
+                } else if (p.out_bf16) {
+                    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + (size_t)done * (G * HD) + col) =
+                        make_uint2(rn_bf16x2(o[c].x * inv, o[c].y * inv), rn_bf16x2(o[c].z * inv, o[c].w * inv));
+                } else {
+                    *reinterpret_cast<float4*>(static_cast<float*>(p.out) + (size_t)done * (G * HD) + col) = make_float4(o[c].x * inv, o[c].y * inv, o[c].z * inv, o[c].w * inv);
+                }
+            }
+            if (lane < G) {  // member 0's lanes
+                if (!last) __stcg(reinterpret_cast<float2*>(p.part_ml + slot_of(i) * (2 * G) + 2 * lane), make_float2(mx, lsum));
+                else if (p.scores) *reinterpret_cast<float2*>(p.score_ml + 2 * ((size_t)done * G + lane)) = make_float2(m_safe, inv_lane);
+            }
+            if (last) break;
         }
-        if (lane == 0) p.counters[wf] = 0;  // for the next launch
     }
 }
 

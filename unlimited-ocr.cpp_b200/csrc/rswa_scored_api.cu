@@ -143,7 +143,9 @@ int run_scored(const uocr_b200_paged_kv* kv, const uocr_b200_score* score, const
     p.rs = ws->score_rs;
     p.part_acc = ws->part_acc;
     p.part_ml = ws->part_ml;
-    p.counters = ws->counters;
+    static_assert(kScoreJoin == kScoreJoinWidth, "the workspace holds the counters of this tree");
+    p.counters = ws->score_counters;
+    p.pieces = ws->pieces_max;
     p.status = ws->status;
     p.wait_limit = ws->wait_limit;
 

@@ -43,6 +43,7 @@ constexpr int kPartElems = 512;  // accumulator elements of one partial: a head,
 
 constexpr int kScoreMaxGroup = 4;  // query heads of a group that share one pass over a KV tile
 constexpr size_t kScoreRowBytes = 32;
+constexpr int kScoreJoinWidth = 8, kScoreJoinLevels = 4;  // partials are joined 8 at a time: 4 levels cover 4096 pieces
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
@@ -70,6 +71,7 @@ struct uocr_b200_workspace {
     uocr_b200::RowInfo* info = nullptr;
     uocr_b200::ScoreRow* score_rows = nullptr;  // [max_rows] plan of the attention with modified scores, when it is made in global memory
     long long* score_rs = nullptr;              // [max_rows + 1]
+    int* score_counters = nullptr;              // [2 kScoreJoinLevels][pieces_max], zero between launches
     float* part_acc = nullptr;
     float* part_ml = nullptr;
     int* counters = nullptr;   // [pieces_max] arrival counters, zero between launches
