@@ -14,6 +14,7 @@ namespace uocr_b200 {
 // equal to it.  The keys of up to kSelectSharedTokens tokens stay in shared memory.
 // -------------------------------------------------------------------------------------------------
 constexpr int kSelectThreads = 1024;
+constexpr int kSelectCopies = 8;
 constexpr int kSelectSharedTokens = 49152;
 
 struct SelectParams {
@@ -35,11 +36,12 @@ __device__ __forceinline__ uint32_t mass_key(float m) {
 
 __global__ void __launch_bounds__(kSelectThreads) rswa_evict_select_kernel(const SelectParams p, int shared_tokens) {
     extern __shared__ uint32_t keys[];
-    __shared__ int hist[256];
+    __shared__ int hist[kSelectCopies][256];  // masses crowd into few bins: every fourth warp has its own counts
     __shared__ int warp_gt[32], warp_eq[32];
     __shared__ uint32_t s_prefix;
     __shared__ int s_need;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the compaction may be set up meanwhile (it waits for this launch)
     const int slot = __ldg(p.d_slots + blockIdx.x);
     const int pfx = max(__ldg(p.d_prefill_len + slot), 0);
     const int n = min(pfx, p.mass_stride);
@@ -64,24 +66,27 @@ __global__ void __launch_bounds__(kSelectThreads) rswa_evict_select_kernel(const
     int need_eq = n;  // everything is kept: no threshold to look for
     if (take < n && take > 0) {
         for (int shift = 24; shift >= 0; shift -= 8) {
-            if (tid < 256) hist[tid] = 0;
+            for (int i = tid; i < kSelectCopies * 256; i += kSelectThreads) (&hist[0][0])[i] = 0;
             __syncthreads();
             const uint32_t prefix = s_prefix, mask = shift == 24 ? 0u : ~0u << (shift + 8);
             for (int s0 = 0; s0 < n; s0 += kSelectThreads) {
                 const int s = s0 + tid;
                 const uint32_t k = s < n ? key(s) : 0u;
-                const bool in = s < n && (k & mask) == prefix;
-                const int bin = in ? (int)((k >> shift) & 255u) : -1;
-                // one atomic per distinct bin of the warp: masses crowd into few bins
-                const unsigned same = __match_any_sync(0xffffffffu, bin);
-                if (in && lane == __ffs(same) - 1) atomicAdd(&hist[bin], __popc(same));
+                if (s < n && (k & mask) == prefix) atomicAdd(&hist[warp % kSelectCopies][(k >> shift) & 255u], 1);
+            }
+            __syncthreads();
+            if (tid < 256) {
+                int sum = 0;
+#pragma unroll
+                for (int i = 0; i < kSelectCopies; ++i) sum += hist[i][tid];
+                hist[0][tid] = sum;
             }
             __syncthreads();
             if (warp == 0) {  // the bin, from the top, in which the running count reaches what is still needed
                 const int need = s_need;
                 int mine = 0;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) mine += hist[255 - lane * 8 - i];
+                for (int i = 0; i < 8; ++i) mine += hist[0][255 - lane * 8 - i];
                 int incl = mine;
 #pragma unroll
                 for (int d = 1; d < 32; d <<= 1) {
@@ -93,12 +98,12 @@ __global__ void __launch_bounds__(kSelectThreads) rswa_evict_select_kernel(const
                     int above = incl - mine;
                     for (int i = 0; i < 8; ++i) {
                         const int bin = 255 - lane * 8 - i;
-                        if (above + hist[bin] >= need) {
+                        if (above + hist[0][bin] >= need) {
                             s_prefix = prefix | ((uint32_t)bin << shift);
                             s_need = need - above;
                             break;
                         }
-                        above += hist[bin];
+                        above += hist[0][bin];
                     }
                 }
             }
@@ -190,10 +195,11 @@ __device__ __forceinline__ long long old_token(const CompactParams& p, int slot,
 
 __global__ void __launch_bounds__(kCompactThreads) rswa_evict_compact_kernel(const __grid_constant__ CompactParams p) {
     __shared__ long long s_src[kBlockTokens];
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // (launched so that its set-up overlaps the launch before it)
     const int i = blockIdx.z, nb = blockIdx.x, tid = threadIdx.x;
     const int layer = blockIdx.y >> 1;
     uint4* pool = reinterpret_cast<uint4*>((blockIdx.y & 1) ? p.pools.v[layer] : p.pools.k[layer]);
-    const int count = min(__ldg(p.d_keep_len + i), p.keep_stride);
+    const int count = min(__ldcg(p.d_keep_len + i), p.keep_stride);
     if (nb * kBlockTokens >= count) return;
     const int dst = nb < p.new_stride ? __ldg(p.d_new_blocks + (size_t)i * p.new_stride + nb) : -1;
     if (dst < 0 || dst >= p.num_blocks) {
@@ -203,7 +209,7 @@ __global__ void __launch_bounds__(kCompactThreads) rswa_evict_compact_kernel(con
     if (tid < kBlockTokens) {
         const int slot = __ldg(p.d_slots + i);
         const int j = nb * kBlockTokens + tid;
-        s_src[tid] = j < count ? old_token(p, slot, __ldg(p.d_keep + (size_t)i * p.keep_stride + j), __ldg(p.d_prefill_len + slot)) : -1;
+        s_src[tid] = j < count ? old_token(p, slot, __ldcg(p.d_keep + (size_t)i * p.keep_stride + j), __ldg(p.d_prefill_len + slot)) : -1;
     }
     __syncthreads();
     uint4* out = pool + (long long)dst * p.kv_heads * kBlockTokens * p.row_chunks;
@@ -231,12 +237,13 @@ __global__ void __launch_bounds__(kCompactThreads) rswa_evict_compact_kernel(con
 // or behind j; one CTA walks a head of a layer in order and reads a batch of rows before it writes it, so nothing is
 // overwritten before it has been read.
 __global__ void __launch_bounds__(kCompactThreads) rswa_evict_compact_in_place_kernel(const __grid_constant__ CompactParams p) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     const int i = blockIdx.z, head = blockIdx.x, tid = threadIdx.x;
     const int layer = blockIdx.y >> 1;
     uint4* pool = reinterpret_cast<uint4*>((blockIdx.y & 1) ? p.pools.v[layer] : p.pools.k[layer]);
     const int slot = __ldg(p.d_slots + i);
     if (slot_seen_before(p.d_slots, i, slot)) return;
-    const int count = min(__ldg(p.d_keep_len + i), p.keep_stride), pfx = __ldg(p.d_prefill_len + slot);
+    const int count = min(__ldcg(p.d_keep_len + i), p.keep_stride), pfx = __ldg(p.d_prefill_len + slot);
     const int* keep = p.d_keep + (size_t)i * p.keep_stride;
     const int rows = kCompactThreads / p.row_chunks;  // head rows of at most 64 chunks
     const int my_row = tid / p.row_chunks, c = tid - my_row * p.row_chunks;
@@ -249,7 +256,7 @@ __global__ void __launch_bounds__(kCompactThreads) rswa_evict_compact_in_place_k
             const int j = j0 + u * rows + my_row;
             dst[u] = -1;
             if (my_row < rows && j < count) {
-                const int at = __ldg(keep + j);
+                const int at = __ldcg(keep + j);
                 const long long src = at >= j ? old_token(p, slot, at, pfx) : -1;
                 if (src >= 0 && at != j) {
                     dst[u] = old_token(p, slot, j, pfx);
@@ -301,7 +308,7 @@ __device__ __forceinline__ void compact_tokens(T* x, int stride, const int* keep
         const int j = j0 + tid;
         T t = fill;
         if (j < count) {
-            const int at = __ldg(keep + j);
+            const int at = __ldcg(keep + j);
             if (at >= j && at < end) t = x[at];
         }
         __syncthreads();
@@ -315,7 +322,7 @@ __global__ void __launch_bounds__(kPublishThreads) rswa_evict_publish_kernel(con
     const int slot = __ldg(p.d_slots + i);
     if (slot_seen_before(p.d_slots, i, slot)) return;
     const int old = p.d_prefill_len[slot];
-    const int count = min(min(__ldg(p.d_keep_len + i), p.keep_stride), old);
+    const int count = min(min(__ldcg(p.d_keep_len + i), p.keep_stride), old);
     if (count < 0) return;
     const int* keep = p.d_keep + (size_t)i * p.keep_stride;
     const int old_blocks = (old + kBlockTokens - 1) / kBlockTokens, new_blocks = (count + kBlockTokens - 1) / kBlockTokens;

@@ -61,10 +61,8 @@ int uocr_b200_rswa_evict_compact_paged_layers(const uocr_b200_paged_kv* kv_layer
     p.new_stride = new_stride;
     p.status = ws ? ws->status : nullptr;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-    if (d_new_blocks)
-        rswa_evict_compact_kernel<<<dim3((keep_stride + kBlockTokens - 1) / kBlockTokens, 2 * layers, n), kCompactThreads, 0, st>>>(p);
-    else
-        rswa_evict_compact_in_place_kernel<<<dim3(pv.kv_heads, 2 * layers, n), kCompactThreads, 0, st>>>(p);
+    const dim3 grid = d_new_blocks ? dim3((keep_stride + kBlockTokens - 1) / kBlockTokens, 2 * layers, n) : dim3(pv.kv_heads, 2 * layers, n);
+    CHECK_CUDA(launch_after(d_new_blocks ? rswa_evict_compact_kernel : rswa_evict_compact_in_place_kernel, grid, kCompactThreads, 0, st, p), "evict: compact");
     return after_launch("evict: compact");
 }
 

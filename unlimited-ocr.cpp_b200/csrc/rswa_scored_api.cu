@@ -167,7 +167,7 @@ int run_scored(const uocr_b200_paged_kv* kv, const uocr_b200_score* score, const
         mp.stride = mass->stride;
         mp.decay = mass->decay;
         mp.status = ws->status;
-        rswa_mass_kernel<<<dim3((mass->stride + kMassThreads - 1) / kMassThreads, plan.rows), kMassThreads, 0, st>>>(mp);
+        CHECK_CUDA(launch_after(rswa_mass_kernel, dim3((mass->stride + kMassThreads - 1) / kMassThreads, plan.rows), kMassThreads, 0, st, mp), "attention weights");
         return after_launch("attention weights");
     }
     return UOCR_B200_OK;

@@ -38,6 +38,22 @@ struct DeviceInfo {
 // The current device, refused unless it is an sm_100 part.
 int device_info(const DeviceInfo** out);
 
+// Launches a kernel that opens with griddepcontrol.wait: its set-up may overlap the launch before it in the stream.
+template <typename P>
+cudaError_t launch_after(void (*kernel)(P), dim3 grid, int threads, int smem, cudaStream_t st, const P& params) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, params);
+}
+
 constexpr int kMaxHeadDim = 256;
 constexpr int kPartElems = 512;  // accumulator elements of one partial: a head, or the heads of a group that share a KV tile
 
