@@ -536,34 +536,35 @@ def _dtype_of(t):
     raise ValueError(f"rows must be float32 or bfloat16, got {dt}")
 
 
-def _row_stride(t, ref, n):
-    """Elements between the rows of t: a [n, width] matrix of ref's type with contiguous rows."""
-    if t.dtype is not ref.dtype or t.size(0) != n or t.stride(1) != 1:
+def _row_stride(t, dtype, n):
+    """Elements between the rows of t: an [n, width] matrix of the type with contiguous rows."""
+    step, one = t.stride()
+    if one != 1 or t.dtype is not dtype or t.size(0) != n:
         raise ValueError("rows must have one type and count, and contiguous elements")
-    return t.stride(0) if n > 1 else max(t.stride(0), t.size(1))
+    return step if n > 1 else max(step, t.size(1))
 
 
 def _qkv_rows(q, k, v, q_out, heads, n):
     """Packed rows, [n, width] each with its own row stride."""
     ref = q if q is not None else k
-    r = QkvRows()
-    r.dtype, r.heads = _dtype_of(ref), heads
+    dt = ref.dtype
+    qs = ks = vs = os = 0
     if q is not None:
-        r.q, r.q_stride = q.data_ptr(), _row_stride(q, ref, n)
+        qs = _row_stride(q, dt, n)
         if q_out is not None:
-            r.q_out, r.q_out_stride = q_out.data_ptr(), _row_stride(q_out, ref, n)
+            os = qs if q_out is q else _row_stride(q_out, dt, n)
     if k is not None:
-        r.k, r.k_stride = k.data_ptr(), _row_stride(k, ref, n)
+        ks = _row_stride(k, dt, n)
         if v is not None:
-            r.v, r.v_stride = v.data_ptr(), _row_stride(v, ref, n)
-    return r
+            vs = _row_stride(v, dt, n)
+    return QkvRows(_dp(q), _dp(k), _dp(v), _dp(q_out), qs, ks, vs, os, _dtype_of(ref), heads)
 
 
 def rope_rows(rope, q, k, q_out, k_out, d_positions, heads, kv_heads, head_dim, stream=None):
     """Rotates the packed rows of q and k (either may be None with 0 heads; outputs may be the inputs)."""
     n = (q if q is not None else k).size(0)
     rows = _qkv_rows(q, k, None, q_out, heads, n)
-    check(lib().uocr_b200_rswa_rope_rows(rope.h, rows, _dp(k_out), _row_stride(k_out, k, n) if k_out is not None else 0, d_positions.data_ptr(),
+    check(lib().uocr_b200_rswa_rope_rows(rope.h, rows, _dp(k_out), _row_stride(k_out, k.dtype, n) if k_out is not None else 0, d_positions.data_ptr(),
                                          n, kv_heads, head_dim, stream_handle(stream)))
 
 

@@ -101,6 +101,11 @@ __device__ __forceinline__ void score_range(const int* d_lo, const int* d_hi, in
     if (hi <= lo) lo = hi = 0;
 }
 
+__device__ __forceinline__ int score_ring_tiles(const ScoreRow& o) {
+    const int skip = o.text >= 0 ? o.text & 15 : 0;
+    return o.ring > 0 ? (skip + o.ring + kBlockTokens - 1) / kBlockTokens : 0;
+}
+
 __device__ __forceinline__ int score_plan_row(const ScorePlan& p, int r, ScoreRow& o) {
     const int slot = __ldg(p.d_slots + r);
     const int pfx = max(__ldg(p.d_prefill_len + slot), 0);
@@ -134,11 +139,37 @@ __device__ __forceinline__ int score_plan_row(const ScorePlan& p, int r, ScoreRo
         if (p.d_q_pos) o.q_pos = __ldg(p.d_q_pos + r);
     }
     const int fixed_tiles = o.hi > o.lo ? (o.hi + kBlockTokens - 1) / kBlockTokens - o.lo / kBlockTokens : 0;
-    const int ring_tiles = o.ring > 0 ? (skip + o.ring + kBlockTokens - 1) / kBlockTokens : 0;
-    return fixed_tiles + ring_tiles;
+    return fixed_tiles + score_ring_tiles(o);
 }
 
-// Block-wide: info[0..rows) and the prefix sum of the rows' units (rs[0..rows]).  `scratch`: 33 long longs of shared memory.
+__device__ __forceinline__ void score_zero_row(const ScorePlan& p, int r) {
+    for (int i = 0; i < p.out_row_words; ++i) p.out[(size_t)r * p.out_row_words + i] = 0u;
+}
+
+__device__ __forceinline__ long long warp_inclusive_sum(long long v, int lane) {
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+        const long long t = __shfl_up_sync(0xffffffffu, v, d);
+        if (lane >= d) v += t;
+    }
+    return v;
+}
+
+// info[0..rows) and the prefix sum of the rows' units (rs[0..rows]), by one warp for up to 32 rows.
+__device__ __forceinline__ void score_plan_warp(const ScorePlan& p, ScoreRow* info, long long* rs, bool zero_rows, int lane) {
+    long long units = 0;
+    if (lane < p.rows) {
+        ScoreRow o;
+        units = (long long)score_plan_row(p, lane, o) * p.items_per_row;
+        info[lane] = o;
+        if (units == 0 && zero_rows) score_zero_row(p, lane);
+    }
+    const long long incl = warp_inclusive_sum(units, lane);
+    if (lane < p.rows) rs[lane + 1] = incl;
+    if (lane == 0) rs[0] = 0;
+}
+
+// The same for any number of rows, block-wide.  `scratch`: 32 long longs of shared memory.
 __device__ __forceinline__ void score_plan_rows(const ScorePlan& p, ScoreRow* info, long long* rs, long long* scratch, bool zero_rows) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nthreads = blockDim.x;
     long long carry = 0;
@@ -149,30 +180,40 @@ __device__ __forceinline__ void score_plan_rows(const ScorePlan& p, ScoreRow* in
             ScoreRow o;
             units = (long long)score_plan_row(p, r, o) * p.items_per_row;
             info[r] = o;
-            if (units == 0 && zero_rows)
-                for (int i = 0; i < p.out_row_words; ++i) p.out[(size_t)r * p.out_row_words + i] = 0u;
+            if (units == 0 && zero_rows) score_zero_row(p, r);
         }
-        long long incl = units;
-#pragma unroll
-        for (int d = 1; d < 32; d <<= 1) {
-            const long long t = __shfl_up_sync(0xffffffffu, incl, d);
-            if (lane >= d) incl += t;
-        }
+        const long long incl = warp_inclusive_sum(units, lane);
         if (lane == 31) scratch[warp] = incl;
         __syncthreads();
-        long long before = carry;
-        for (int w = 0; w < warp; ++w) before += scratch[w];
-        if (r < p.rows) rs[r] = before + incl - units;
-        long long all = 0;
-        for (int w = 0; w < (nthreads >> 5); ++w) all += scratch[w];
-        carry += all;
+        const long long sums = warp_inclusive_sum(lane < (nthreads >> 5) ? scratch[lane] : 0, lane);
+        const long long before = warp > 0 ? __shfl_sync(0xffffffffu, sums, warp - 1) : 0;
+        if (r < p.rows) rs[r] = carry + before + incl - units;
+        carry += __shfl_sync(0xffffffffu, sums, 31);
         __syncthreads();
     }
     if (tid == 0) rs[p.rows] = carry;
 }
 
+// 64-bit divisions cost hundreds of cycles and are taken only where 32 bits do not hold the operands.
+__device__ __forceinline__ long long div_units(long long a, long long b) {
+    return ((unsigned long long)a | (unsigned long long)b) >> 32 ? a / b : (long long)((uint32_t)a / (uint32_t)b);
+}
+// The unit line [0, total) cut into ns pieces of equal length, but for one unit: piece k begins at floor(k total / ns).
+struct ScorePieces {
+    long long total, each;
+    int ns, rest;  // total = each * ns + rest
+    __device__ __forceinline__ ScorePieces(long long n, int total_warps) {
+        total = n;
+        ns = (int)min((long long)total_warps, total);
+        each = div_units(total, ns);
+        rest = (int)(total - each * ns);
+    }
+    __device__ __forceinline__ long long start(int k) const { return k * each + (uint32_t)(k * rest) / (uint32_t)ns; }  // (at most 4096 pieces)
+    __device__ __forceinline__ int of(long long u) const { return (int)div_units((u + 1) * ns - 1, total); }
+};
+
 __global__ void __launch_bounds__(1024) rswa_scored_plan_kernel(ScorePlan p, ScoreRow* info, long long* rs) {
-    __shared__ long long scratch[33];
+    __shared__ long long scratch[32];
     score_plan_rows(p, info, rs, scratch, true);
 }
 
@@ -323,21 +364,22 @@ struct ScoreFma {
             for (int e = 0; e < PPL; ++e) acc2[h][e] = mul2(acc2[h][e], alpha2);
         }
     }
-    __device__ __forceinline__ void values(const uint8_t* vtile, int nskip, int nvalid, int) {
-        const bool all = nvalid == kBlockTokens && nskip == 0;
+    template <bool ALL>
+    __device__ __forceinline__ void add_values(const uint8_t* vtile, int nskip, int nvalid) {
 #pragma unroll
         for (int i = 0; i < ITER; ++i) {
             const int t = i * RPW + rg;
             float2 pi2[G];
 #pragma unroll
             for (int h = 0; h < G; ++h) {
-                const float pi = (LPR >= 2) ? __shfl_sync(0xffffffffu, pr[h], rg * LPR + 2 * i) : pr[h];
+                float pi = (LPR >= 2) ? __shfl_sync(0xffffffffu, pr[h], rg * LPR + 2 * i) : pr[h];
+                if (ALL && RPW > kBlockTokens && rg >= kBlockTokens) pi = 0.f;
                 pi2[h] = make_float2(pi, pi);
             }
-            if (all ? (RPW <= kBlockTokens || t < kBlockTokens) : (t >= nskip && t < nvalid)) {  // rows outside may hold anything
+            if (ALL || (t >= nskip && t < nvalid)) {  // rows outside may hold anything
 #pragma unroll
                 for (int cp = 0; cp < CPL; ++cp) {
-                    const uint4 w = *reinterpret_cast<const uint4*>(vtile + t * ROWB + (g + 32 * cp) * 16);
+                    const uint4 w = *reinterpret_cast<const uint4*>(vtile + (ALL ? t & (kBlockTokens - 1) : t) * ROWB + (g + 32 * cp) * 16);
                     float2 f[PPC];
                     unpack2<KV>(w, f);
 #pragma unroll
@@ -347,6 +389,11 @@ struct ScoreFma {
                 }
             }
         }
+    }
+    __device__ __forceinline__ void values(const uint8_t* vtile, int nskip, int nvalid, int) {
+        // (two loops: a condition inside the loop keeps the loads of its iterations apart)
+        if (nvalid == kBlockTokens && nskip == 0) add_values<true>(vtile, nskip, nvalid);
+        else add_values<false>(vtile, nskip, nvalid);
     }
     // the item's result, or this segment's partial into slot my_slot
     __device__ __forceinline__ void emit(const ScoreParams& p, const ScoreItem& it, bool whole, int my_slot, int lane) {
@@ -634,36 +681,40 @@ __global__ void __launch_bounds__(C::kThreads, 1) rswa_scored_kernel(const __gri
     uint8_t* my_tiles = smem + bar_bytes + (size_t)warp * (kScoreRing * TILE);
     const uint32_t bar0 = smem_addr(smem) + warp * (kScoreRing * 8);
     const uint32_t tile0 = smem_addr(my_tiles);
-    if (lane == 0) {
+    auto init_barriers = [&]() {
+        if (lane == 0) {
 #pragma unroll
-        for (int s = 0; s < kScoreRing; ++s) mbar_init(bar0 + 8 * s, 1);
-        mbar_init_fence();
-    }
-    __syncwarp();
+            for (int s = 0; s < kScoreRing; ++s) mbar_init(bar0 + 8 * s, 1);
+            mbar_init_fence();
+        }
+        __syncwarp();
+    };
 
-    // ---- the plan -------------------------------------------------------------------------------------
+    // ---- the plan: up to 32 rows by warp 0 while the others set up their barriers, more by the whole CTA, many in global memory ----
     const ScoreRow* info = p.info;
     const long long* rs = p.rs;
     if (p.rows <= kScoreSharedRows) {
         uint8_t* plan_base = smem + bar_bytes + (size_t)warps * (kScoreRing * TILE);
         ScoreRow* info_s = reinterpret_cast<ScoreRow*>(plan_base);
         long long* rs_s = reinterpret_cast<long long*>(plan_base + sizeof(ScoreRow) * p.rows);
-        score_plan_rows(p.plan, info_s, rs_s, rs_s + p.rows + 1, blockIdx.x == 0);
+        if (p.rows > 32) score_plan_rows(p.plan, info_s, rs_s, rs_s + p.rows + 1, blockIdx.x == 0);
+        else if (warp == 0) score_plan_warp(p.plan, info_s, rs_s, blockIdx.x == 0, lane);
+        init_barriers();
         __syncthreads();
         info = info_s;
         rs = rs_s;
+    } else {
+        init_barriers();
     }
     const int items_per_row = p.plan.items_per_row;
     const long long total = rs[p.rows];
     if (total == 0) return;
-    const PieceMap pm = make_piece_map(total, p.total_warps, warps);
+    const ScorePieces pm(total, p.total_warps);
     // fewer pieces than warps are spread over the SMs
-    const int gw = (int)blockIdx.x * warps + warp;
-    const int gw_spread = warp * (int)gridDim.x + (int)blockIdx.x;
-    const int piece = pm.ns == p.total_warps ? gw : (gw_spread < pm.ns ? gw_spread : -1);
-    if (piece < 0) return;
+    const int piece = pm.ns == p.total_warps ? (int)blockIdx.x * warps + warp : warp * (int)gridDim.x + (int)blockIdx.x;
+    if (piece >= pm.ns) return;
     const long long u0 = pm.start(piece);
-    const long long n_units = pm.end(piece) - u0;
+    const int n_units = (int)(pm.start(piece + 1) - u0);
 
     if (p.scores) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the kernel that turns scores into weights
     C work;
@@ -672,8 +723,8 @@ __global__ void __launch_bounds__(C::kThreads, 1) rswa_scored_kernel(const __gri
     // ---- unit descriptors: lane l describes unit desc_base + l of this piece ----------------------------
     uint32_t d_tile = 0, d_meta = 0, d_item = 0;
     int d_tok = 0;  // fixed region: index of the tile's token 0; ring / text: its distance from the query
-    long long desc_base = 0;
-    auto build_desc = [&](long long base) {
+    int desc_base = 0;
+    auto build_desc = [&](int base) {
         desc_base = base;
         d_tile = d_meta = d_item = 0;
         d_tok = 0;
@@ -685,12 +736,12 @@ __global__ void __launch_bounds__(C::kThreads, 1) rswa_scored_kernel(const __gri
                 if (rs[mid] <= u) lo = mid; else hi = mid;
             }
             const ScoreRow o = info[lo];
-            const int per_item = (int)((rs[lo + 1] - rs[lo]) / items_per_row);
-            const long long rem = u - rs[lo];
-            const int it = (int)(rem / per_item), j = (int)(rem - (long long)it * per_item);
-            const int kvh = it * G / p.group;
             const int first = o.lo / kBlockTokens;
             const int fixed_tiles = o.hi > o.lo ? (o.hi + kBlockTokens - 1) / kBlockTokens - first : 0;
+            const int per_item = fixed_tiles + score_ring_tiles(o);
+            const long long rem = u - rs[lo];
+            const int it = (int)div_units(rem, per_item), j = (int)(rem - (long long)it * per_item);
+            const int kvh = (int)((uint32_t)(it * G) / (uint32_t)p.group);
             uint32_t m = 0;
             int valid, skip = 0, blk = -1;
             if (j < fixed_tiles) {
@@ -731,11 +782,11 @@ __global__ void __launch_bounds__(C::kThreads, 1) rswa_scored_kernel(const __gri
     // ---- producer: tiles K(0) V(0) K(1) V(1) ... rotate through the slots ------------------------------
     const uint64_t pol_stream = l2_policy_evict_first(), pol_keep = l2_policy_evict_last();
     int issue_slot = 0, use_slot = 0;
-    long long issue_seq = 0, consumed = 0;
+    int issue_seq = 0, consumed = 0;
     uint32_t phases = 0;
     auto issue_next = [&]() {
         if (issue_seq >= 2 * n_units) return;
-        const int src = (int)((issue_seq >> 1) - desc_base);
+        const int src = (issue_seq >> 1) - desc_base;
         const bool is_v = (issue_seq & 1) != 0;
         const uint32_t tile = __shfl_sync(FULL, d_tile, src);
         const uint32_t meta = __shfl_sync(FULL, d_meta, src);
@@ -779,10 +830,10 @@ __global__ void __launch_bounds__(C::kThreads, 1) rswa_scored_kernel(const __gri
     bool first_segment = true, gave_up = false;
     bool from_start = (__shfl_sync(FULL, d_meta, 0) & kSuFirst) != 0;
 
-    for (long long it = 0; it < n_units; ++it) {
+    for (int it = 0; it < n_units; ++it) {
         if (it - desc_base >= 32 - 2) build_desc(it);  // the producer looks two units ahead
-        const uint32_t meta = __shfl_sync(FULL, d_meta, (int)(it - desc_base));
-        const int tok0 = __shfl_sync(FULL, d_tok, (int)(it - desc_base));
+        const uint32_t meta = __shfl_sync(FULL, d_meta, it - desc_base);
+        const int tok0 = __shfl_sync(FULL, d_tok, it - desc_base);
         const int nvalid = (int)(meta & kSuValid), nskip = (int)((meta >> kSuSkipShift) & 15);
 
         const uint8_t* ktile = wait_tile();
@@ -805,7 +856,7 @@ __global__ void __launch_bounds__(C::kThreads, 1) rswa_scored_kernel(const __gri
             if (!whole) pend[pend_n++ & 1] = item.index;
             first_segment = false;
             if (!piece_done) {
-                start_item(__shfl_sync(FULL, d_item, (int)(it + 1 - desc_base)));
+                start_item(__shfl_sync(FULL, d_item, it + 1 - desc_base));
                 from_start = true;
             }
         }
@@ -829,7 +880,7 @@ __global__ void __launch_bounds__(C::kThreads, 1) rswa_scored_kernel(const __gri
     for (int k = 0; k < pend_n; ++k) {
         const uint32_t done = pend[k];
         const int r = (int)(done / (uint32_t)items_per_row);
-        const int n = (int)((rs[r + 1] - rs[r]) / items_per_row);
+        const int n = (int)div_units(rs[r + 1] - rs[r], items_per_row);
         const long long s0 = rs[r] + (long long)(done - (uint32_t)r * (uint32_t)items_per_row) * n;
         const int wf = pm.of(s0), n_part = pm.of(s0 + n - 1) - wf + 1;
         const bool wf_second = pm.start(wf) < s0;  // the item is piece wf's second segment

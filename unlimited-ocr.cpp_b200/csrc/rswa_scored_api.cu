@@ -11,7 +11,7 @@ namespace {
 template <typename C, int HD>
 int launch_scored(ScoreParams& p, const DeviceInfo& di, const uocr_b200_workspace* ws, cudaStream_t st) {
     constexpr int per_warp = kScoreRing * C::kTile;
-    const int plan_bytes = p.rows <= kScoreSharedRows ? (int)(sizeof(ScoreRow) * p.rows + sizeof(long long) * (p.rows + 1 + 33)) : 0;
+    const int plan_bytes = p.rows <= kScoreSharedRows ? (int)(sizeof(ScoreRow) * p.rows + sizeof(long long) * (p.rows + 1 + 32)) : 0;
     int warps = ((di.smem_optin < 200 * 1024 ? di.smem_optin : 200 * 1024) - 1024 - plan_bytes) / per_warp;
     if (warps > C::kThreads / 32) warps = C::kThreads / 32;
     if (warps < 1) return fail(UOCR_B200_ERR_UNSUPPORTED, "attention_scored: tile does not fit in shared memory");
