@@ -514,7 +514,7 @@ UOCR_B200_API int uocr_b200_rswa_rope_append_decode_batch_paged(
  * ============================================================================================= */
 typedef struct {
     float scale;         /* 0: 1/sqrt(head_dim)                                                        */
-    float softcap;       /* 0: none                                                                    */
+    float softcap;       /* 0: none; otherwise at least 1e-6                                           */
     const float* slopes; /* device [heads], or null: no bias                                           */
     const int* d_q_pos;  /* device [rows], position of each query row; needed with slopes (ragged vision
                             rows default to d_pos)                                                     */
@@ -574,8 +574,8 @@ UOCR_B200_API int uocr_b200_rswa_prefill_text_scored_paged(
  * results, the probabilities are rounded to bf16 (half a step, as the result itself).  K and V outside
  * the span of keys that the rows of a query tile see -- from the first to the last -- may hold anything; inside it
  * they must be finite, since the rows that do not see a key multiply its value by zero. A query row that holds a NaN or an
- * infinity gives NaN (0 if it sees no key).  d_key_pos is not supported (UNSUPPORTED): keys
- * stand at their own index. */
+ * infinity gives NaN (0 if it sees no key).  Not supported
+ * (UNSUPPORTED): d_key_pos, keys stand at their own index; a softcap above 256, the tanh is off by 2^-21 of the cap. */
 UOCR_B200_API int uocr_b200_rswa_prefill_attention_scored_tc(
     const uocr_b200_paged_kv* kv, const void* text_k_pool, const void* text_v_pool, int text_blocks,
     const uocr_b200_score* score, const void* q, int q_dtype, const int* d_prefill_len,

@@ -263,3 +263,44 @@ def test_run_of_the_operators(b, pool):
             for l in range(layers):
                 fixed[s][l] = tuple(x[kept] for x in fixed[s][l])
     assert ws.status() == 0
+
+
+def test_captured_eviction(b):
+    """The three calls in one captured graph, replayed on new weights."""
+    import torch
+    rng = np.random.default_rng(3)
+    W, keep, layers = 16, 40, 2
+    lens = [100, 77]
+    lay, table, free, st = build(b, torch, rng, lens, [4, 9], W, layers, 2, 32, b.F32, extra=8)
+    arr, ds = b.layer_array(lay), ints(torch, [1, 0])
+    new = torch.tensor(free[:6].reshape(2, 3).copy(), device="cuda")
+    mass = torch.rand(2, 112, device="cuda")
+    d_keep, d_n = torch.empty((2, keep), dtype=torch.int32, device="cuda"), torch.empty(2, dtype=torch.int32, device="cuda")
+    ws = b.Workspace(1)
+    start = [x.clone() for x in (table, st["d_len"], st["d_prefill"])]
+    old = [(x.k.clone(), x.v.clone()) for x in lay]
+
+    def step():
+        b.evict_select(mass, st["d_prefill"], ds, 2, keep, 1, 1, d_keep, d_n, ws)
+        b.evict_compact_paged_layers(arr, st["d_prefill"], ds, 2, d_keep, d_n, new, ws)
+        b.evict_publish(table, ds, 2, d_keep, d_n, st["d_len"], st["d_prefill"], W, new, None, None, ws)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(s):
+        with torch.cuda.graph(g, stream=s):
+            step()
+    torch.cuda.current_stream().wait_stream(s)
+    for _ in range(3):
+        for x, y in zip((table, st["d_len"], st["d_prefill"]), start):
+            x.copy_(y)
+        mass.uniform_()
+        g.replay()
+        torch.cuda.synchronize()
+        assert ws.status() == 0 and st["d_prefill"].tolist() == [40, 40] and st["d_len"][1].tolist() == [44, 49]
+        for i, slot in enumerate((1, 0)):
+            kept = torch.tensor(choose(mass[slot].cpu().numpy(), lens[slot], keep, 1, 1), device="cuda")
+            assert torch.equal(d_keep[i].long(), kept)
+            for x, (k, v) in zip(lay, old):
+                assert torch.equal(rows(x.k, table[slot, :3], keep), rows(k, start[0][slot, :7], lens[slot])[kept])
+                assert torch.equal(rows(x.v, table[slot, :3], keep), rows(v, start[0][slot, :7], lens[slot])[kept])

@@ -303,7 +303,7 @@ def test_refusals(b):
 
     def call(score, layer=w.layer, text=w.text, heads=2, window=8, q=w.q):
         b.prefill_attention_scored_tc(layer, *text, w.text_blocks, score, q, w.d_prefill, w.tiles, window, heads, out, ws)
-    bad = [dict(score=b.Score(softcap=-1.0)), dict(score=b.Score(softcap=float("nan"))), dict(score=b.Score(scale=float("inf"))),
+    bad = [dict(score=b.Score(softcap=300.0)), dict(score=b.Score(softcap=1e-7)), dict(score=b.Score(softcap=-1.0)), dict(score=b.Score(softcap=float("nan"))), dict(score=b.Score(scale=float("inf"))),
            dict(score=b.Score(d_key_pos=pos.reshape(2, 12).contiguous())), dict(score=b.Score(slopes=slopes_of(torch, 2))),  # text rows need their positions
            dict(score=b.Score(), text=(None, None)), dict(score=b.Score(), heads=3), dict(score=b.Score(), window=0)]
     for kw in bad:
@@ -318,7 +318,7 @@ def test_refusals(b):
     ints = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")
     small = b.Workspace(2)
     o = torch.empty(4, 256, device="cuda")
-    for kw in (dict(score=b.Score(softcap=-2.0)), dict(score=b.Score(scale=float("nan"))), dict(score=b.Score(slopes=slopes_of(torch, 2))), dict(heads=3), dict(batch=3)):
+    for kw in (dict(score=b.Score(softcap=1e-9)), dict(score=b.Score(softcap=-2.0)), dict(score=b.Score(scale=float("nan"))), dict(score=b.Score(slopes=slopes_of(torch, 2))), dict(heads=3), dict(batch=3)):
         a = dict(score=b.Score(), heads=2, batch=1) | kw
         with pytest.raises(b.Error):
             b.attention_scored_batch_paged(w.layer, a["score"], w.q, ints(20, 20), ints(0, 0), w.d_prefill, ints(0, 0, 0), a["batch"], 16, a["heads"], o, small)

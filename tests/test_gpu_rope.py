@@ -95,6 +95,7 @@ def positions(torch, rng, rows, far):
     (5, 3, 1, 80, 40, 300000),         # half layout: the halves are not whole chunks
     (9, 2, 2, 10, 6, 5000),            # rows that are not a multiple of 16 bytes
     (3, 1, 1, 2, 2, 100), (7, 1, 0, 256, 256, 65536), (4, 0, 3, 16, 2, 65536), (2500, 2, 1, 32, 32, 65536),
+    (3, 2, 1, 512, 256, 65536), (2, 1, 2, 1024, 64, 65536), (2400, 3, 1, 264, 128, 4000),  # heads wider than a warp's 32 chunks
 ])
 def test_rope_rows(b, scaling, layout, dtype, rows, heads, kvh, hd, r, far):
     import torch
@@ -266,3 +267,10 @@ def test_rope_in_a_captured_graph(b):
         b.rope_rows(rope, x, None, want, None, pos, 10, 0, 128)
         torch.cuda.synchronize()
         assert torch.equal(out, want)
+
+
+def test_rope_wants_tensors_of_the_current_device(b):
+    import torch
+    x, pos = torch.zeros(2, 64), torch.zeros(2, dtype=torch.int32)
+    with pytest.raises(ValueError):
+        b.rope_rows(b.Rope(rotary_dim=64), x, None, x, None, pos, 1, 0, 64)

@@ -342,3 +342,14 @@ def test_captured_and_on_another_stream(b):
         call(want, mass2)
         torch.cuda.synchronize()
         assert torch.equal(out, want) and torch.equal(m, m2)
+
+
+def test_text_blocks_outside_the_pool_are_reported(b):
+    import torch
+    c = Caches([(5, 0, 0)], 1, 64, b.F32, 16, seed=1)
+    (kt, vt), _, block0, blocks = text_pools(b, torch, np.random.default_rng(0), [20], 1, 64, b.F32)
+    q, ws = torch.randn(1, 64, device="cuda"), b.Workspace(1)
+    out = torch.empty(1, 64, device="cuda")
+    for at, bad in ((block0[0], False), (-1, True), (-(1 << 31), True), (blocks, True), ((1 << 31) - 1, True), (1 << 27, True)):
+        b.prefill_text_scored_paged(c.layer, kt, vt, blocks, b.Score(), q, c.d_prefill, ints(torch, [0]), ints(torch, [19]), ints(torch, [at]), 1, 64, 1, out, ws)
+        assert ws.status() == (b.STATUS_BAD_BLOCK if bad else 0), at

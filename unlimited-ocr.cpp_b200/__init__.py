@@ -521,6 +521,14 @@ class Rope:
             pass
 
 
+def _stream_of(t, stream):
+    """The stream of a call on t's device, which has to be the current one (launches go there)."""
+    import torch
+    if t.get_device() != torch.cuda.current_device():
+        raise ValueError(f"tensors must be on the current device, got {t.device}")
+    return stream_handle(stream)
+
+
 def _dp(t):
     """Device address of a tensor / None (the light form of _p for calls that are short themselves)."""
     return None if t is None else t.data_ptr()
@@ -565,7 +573,7 @@ def rope_rows(rope, q, k, q_out, k_out, d_positions, heads, kv_heads, head_dim, 
     n = (q if q is not None else k).size(0)
     rows = _qkv_rows(q, k, None, q_out, heads, n)
     check(lib().uocr_b200_rswa_rope_rows(rope.h, rows, _dp(k_out), _row_stride(k_out, k.dtype, n) if k_out is not None else 0, d_positions.data_ptr(),
-                                         n, kv_heads, head_dim, stream_handle(stream)))
+                                         n, kv_heads, head_dim, _stream_of(d_positions, stream)))
 
 
 def rope_write_prefill_paged(layer, rope, q, k, v, q_out, d_positions, d_slots, d_pos, heads, ws=None, stream=None):
@@ -573,7 +581,7 @@ def rope_write_prefill_paged(layer, rope, q, k, v, q_out, d_positions, d_slots, 
     n = k.size(0)
     check(lib().uocr_b200_rswa_rope_write_prefill_paged(
         layer.desc, rope.h, _qkv_rows(q, k, v, q_out, heads, n), d_positions.data_ptr(), d_slots.data_ptr(), d_pos.data_ptr(), n,
-        ws.h if ws else None, stream_handle(stream)))
+        ws.h if ws else None, _stream_of(k, stream)))
 
 
 def rope_append_decode_batch_paged(layer, rope, q, k, v, q_out, d_positions, d_len, d_ring, d_prefill, d_slots, window, heads, ws=None,
@@ -582,7 +590,7 @@ def rope_append_decode_batch_paged(layer, rope, q, k, v, q_out, d_positions, d_l
     n = k.size(0)
     check(lib().uocr_b200_rswa_rope_append_decode_batch_paged(
         layer.desc, rope.h, _qkv_rows(q, k, v, q_out, heads, n), d_positions.data_ptr(), d_len.data_ptr(), d_ring.data_ptr(), d_prefill.data_ptr(),
-        d_slots.data_ptr(), n, window, ws.h if ws else None, stream_handle(stream)))
+        d_slots.data_ptr(), n, window, ws.h if ws else None, _stream_of(k, stream)))
 
 
 # ---- attention with modified scores --------------------------------------------------------------------
@@ -619,13 +627,13 @@ def attention_scored_batch_paged(layer, score, q, d_len, d_ring, d_prefill, d_sl
     """Decode attention with modified scores; `mass` also accumulates the attention weights."""
     check(lib().uocr_b200_rswa_attention_scored_batch_paged(
         layer.desc, score.desc, _dp(q), _dtype_of(q), _dp(d_len), _dp(d_ring), _dp(d_prefill), _dp(d_slots), batch, window, heads,
-        _dp(out), C.addressof(mass.desc) if mass is not None else None, ws.h, stream_handle(stream)))
+        _dp(out), C.addressof(mass.desc) if mass is not None else None, ws.h, _stream_of(q, stream)))
 
 
 def attention_scored_ragged_paged(layer, score, q, d_prefill, d_slots, d_pos, total, heads, out, ws, stream=None):
     """Packed vision rows with modified scores, any geometry."""
     check(lib().uocr_b200_rswa_attention_scored_ragged_paged(layer.desc, score.desc, _dp(q), _dtype_of(q), _dp(d_prefill), _dp(d_slots),
-                                                             _dp(d_pos), total, heads, _dp(out), ws.h, stream_handle(stream)))
+                                                             _dp(d_pos), total, heads, _dp(out), ws.h, _stream_of(q, stream)))
 
 
 def prefill_text_scored_paged(layer, text_k, text_v, text_blocks, score, q, d_prefill, d_slots, d_pos, d_block0, total, window, heads, out, ws,
@@ -633,14 +641,14 @@ def prefill_text_scored_paged(layer, text_k, text_v, text_blocks, score, q, d_pr
     """Packed text rows over prefix + text window with modified scores, any geometry (K and V already in the text pool)."""
     check(lib().uocr_b200_rswa_prefill_text_scored_paged(layer.desc, _dp(text_k), _dp(text_v), text_blocks, score.desc, _dp(q),
                                                          _dtype_of(q), _dp(d_prefill), _dp(d_slots), _dp(d_pos), _dp(d_block0), total, window,
-                                                         heads, _dp(out), ws.h, stream_handle(stream)))
+                                                         heads, _dp(out), ws.h, _stream_of(q, stream)))
 
 
 def prefill_plan_scored_tc(score, tiles, d_prefill, window, ws, stream=None):
     """Uploads and orders the query tiles for the score's visible ranges; later calls with reuse_plan=True share the plan."""
     import numpy as np
     t = np.ascontiguousarray(tiles, dtype=np.int32)
-    check(lib().uocr_b200_rswa_prefill_plan_scored_tc(score.desc, t.ctypes.data, t.shape[0], _dp(d_prefill), window, ws.h, stream_handle(stream)))
+    check(lib().uocr_b200_rswa_prefill_plan_scored_tc(score.desc, t.ctypes.data, t.shape[0], _dp(d_prefill), window, ws.h, _stream_of(d_prefill, stream)))
 
 
 def prefill_attention_scored_tc(layer, text_k, text_v, text_blocks, score, q, d_prefill, tiles, window, heads, out, ws, stream=None, reuse_plan=False):
@@ -649,7 +657,7 @@ def prefill_attention_scored_tc(layer, text_k, text_v, text_blocks, score, q, d_
     t = np.ascontiguousarray(tiles, dtype=np.int32)
     check(lib().uocr_b200_rswa_prefill_attention_scored_tc(
         layer.desc, _dp(text_k), _dp(text_v), text_blocks, score.desc, _dp(q), _dtype_of(q), _dp(d_prefill),
-        None if reuse_plan else t.ctypes.data, t.shape[0], window, heads, _dp(out), ws.h, stream_handle(stream)))
+        None if reuse_plan else t.ctypes.data, t.shape[0], window, heads, _dp(out), ws.h, _stream_of(q, stream)))
 
 
 # ---- eviction from the fixed region ----------------------------------------------------------------------
@@ -657,7 +665,7 @@ def prefill_attention_scored_tc(layer, text_k, text_v, text_blocks, score, q, d_
 def evict_select(mass, d_prefill, d_slots, n, keep, sinks, recent, d_keep, d_keep_len, ws=None, stream=None):
     """The `keep` heaviest tokens of each slot's fixed region, ascending: d_keep int32 [n, keep], d_keep_len int32 [n]."""
     check(lib().uocr_b200_rswa_evict_select(_dp(mass), mass.size(1), _dp(d_prefill), _dp(d_slots), n, keep, sinks, recent, _dp(d_keep),
-                                            _dp(d_keep_len), ws.h if ws else None, stream_handle(stream)))
+                                            _dp(d_keep_len), ws.h if ws else None, _stream_of(mass, stream)))
 
 
 def evict_compact_paged_layers(layers, d_prefill, d_slots, n, d_keep, d_keep_len, d_new_blocks=None, ws=None, stream=None):
@@ -665,7 +673,7 @@ def evict_compact_paged_layers(layers, d_prefill, d_slots, n, d_keep, d_keep_len
     arr = layers if isinstance(layers, C.Array) else layer_array(layers)
     check(lib().uocr_b200_rswa_evict_compact_paged_layers(
         arr, len(arr), _dp(d_prefill), _dp(d_slots), n, _dp(d_keep), d_keep.size(1), _dp(d_keep_len), _dp(d_new_blocks),
-        d_new_blocks.shape[1] if d_new_blocks is not None else 0, ws.h if ws else None, stream_handle(stream)))
+        d_new_blocks.shape[1] if d_new_blocks is not None else 0, ws.h if ws else None, _stream_of(d_keep, stream)))
 
 
 def evict_publish(table, d_slots, n, d_keep, d_keep_len, d_len, d_prefill, window, d_new_blocks=None, mass=None, d_key_pos=None, ws=None,
@@ -675,4 +683,4 @@ def evict_publish(table, d_slots, n, d_keep, d_keep_len, d_len, d_prefill, windo
     check(lib().uocr_b200_rswa_evict_publish(
         _dp(table), table.shape[1], _dp(d_slots), n, _dp(d_keep), d_keep.size(1), _dp(d_keep_len), _dp(d_new_blocks), width(d_new_blocks), _dp(d_len),
         d_len.stride(0), d_len.shape[0], _dp(d_prefill), window, _dp(mass), width(mass), _dp(d_key_pos), width(d_key_pos),
-        ws.h if ws else None, stream_handle(stream)))
+        ws.h if ws else None, _stream_of(table, stream)))

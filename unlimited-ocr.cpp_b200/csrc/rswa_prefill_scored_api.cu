@@ -33,7 +33,9 @@ int launch_types(bool pair_q, bool pair_p, const PrefillParams& pp, const Prefil
 int check_score(const uocr_b200_score* score, const char* who) {
     auto bad = [&](const char* what) { return fail(UOCR_B200_ERR_INVALID, std::string(who) + ": " + what); };
     if (!score) return bad("null pointer");
-    if (!(score->softcap >= 0.f) || !std::isfinite(score->softcap)) return bad("softcap must be 0 (none) or positive");
+    if (!(score->softcap == 0.f || score->softcap >= 1e-6f) || !std::isfinite(score->softcap)) return bad("softcap must be 0 (none) or at least 1e-6");
+    // the kernel's tanh is off by 2^-21 of the cap: a cap far above the scores would drown them
+    if (score->softcap > 256.f) return fail(UOCR_B200_ERR_UNSUPPORTED, std::string(who) + ": softcap above 256 (use the calls for any geometry)");
     if (!std::isfinite(score->scale)) return bad("scale must be finite (0: 1/sqrt(head_dim))");
     if (score->d_key_pos) return fail(UOCR_B200_ERR_UNSUPPORTED, std::string(who) + ": keys stand at their own index here (d_key_pos: use the calls for any geometry)");
     return UOCR_B200_OK;

@@ -91,6 +91,7 @@ struct ScoreParams {
 };
 
 constexpr int kScoreJoin = 8;  // partials joined at a time
+constexpr int kScoreTextBlocks = (1 << 27) - 1;  // more blocks than a text pool may have
 
 constexpr int kScoreSharedRows = 512;  // rows a CTA plans in its own shared memory
 
@@ -134,7 +135,8 @@ __device__ __forceinline__ int score_plan_row(const ScorePlan& p, int r, ScoreRo
         const int first = max(0, pos - p.window + 1);
         skip = first & (kBlockTokens - 1);
         o.ring = max(pos - first + 1, 0);
-        o.text = ((__ldg(p.d_text_block0 + r) + first / kBlockTokens) << 4) | skip;
+        const long long blk = (long long)__ldg(p.d_text_block0 + r) + first / kBlockTokens;
+        o.text = (int)(blk < 0 || blk >= kScoreTextBlocks ? kScoreTextBlocks : blk) << 4 | skip;  // (a block outside the pool is reported when it is read)
         o.age0 = pos - (first - skip);
         if (p.d_q_pos) o.q_pos = __ldg(p.d_q_pos + r);
     }

@@ -74,13 +74,13 @@ int run_scored(const uocr_b200_paged_kv* kv, const uocr_b200_score* score, const
     if (q_dtype != UOCR_B200_F32 && q_dtype != UOCR_B200_BF16) return fail(UOCR_B200_ERR_UNSUPPORTED, std::string(who) + ": q must be fp32 or bf16");
     if (heads <= 0 || heads % kv->kv_heads != 0) return bad("heads must be a positive multiple of kv_heads");
     if (!aligned16(q) || !aligned16(out)) return bad("q/out must be 16-byte aligned");
-    if (!(score->softcap >= 0.f) || !std::isfinite(score->softcap)) return bad("softcap must be 0 (none) or positive");
+    if (!(score->softcap == 0.f || score->softcap >= 1e-6f) || !std::isfinite(score->softcap)) return bad("softcap must be 0 (none) or at least 1e-6");
     if (!std::isfinite(score->scale)) return bad("scale must be finite (0: 1/sqrt(head_dim))");
     if (score->d_key_pos && score->key_pos_stride <= 0) return bad("key_pos_stride must be positive");
     if (score->slopes && plan.mode != kScoreRagged && !score->d_q_pos) return bad("a distance bias needs d_q_pos");
     if (plan.rows > ws->max_rows) return fail(UOCR_B200_ERR_WORKSPACE, std::string(who) + ": more rows than the workspace was created for");
     if ((long long)plan.rows * heads >= (1ll << 31) || (long long)kv->num_blocks * kv->kv_heads >= (1ll << 32) ||
-        (long long)text.blocks * kv->kv_heads >= (1ll << 32) || text.blocks >= (1 << 27))
+        (long long)text.blocks * kv->kv_heads >= (1ll << 32) || text.blocks > kScoreTextBlocks)
         return fail(UOCR_B200_ERR_UNSUPPORTED, std::string(who) + ": rows * heads or a pool is too large");
     size_t score_bytes = 0;
     if (mass) {
