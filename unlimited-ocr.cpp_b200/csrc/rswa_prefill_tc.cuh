@@ -526,6 +526,8 @@ __device__ __forceinline__ void tc_tile_steps(const PrefillTile& t, int pfx, int
 // items in this order, heads innermost: CTA c starts with item c, the counter (zero at launch) gives the rest.
 constexpr int kTcOrderBins = 256;
 
+__device__ __forceinline__ int tc_block_start(int token) { return token & ~(kBlockTokens - 1); }
+
 // What row r (packed row t.row0 + r) of a tile sees of the fixed region: tokens [lo, hi), hi <= lo if none.
 __device__ __forceinline__ void tc_row_range(const PrefillParams& p, const PrefillTile& t, int r, int pfx, int& lo, int& hi) {
     lo = p.d_lo ? max(__ldg(p.d_lo + t.row0 + r), 0) : 0;
@@ -556,10 +558,14 @@ __global__ void __launch_bounds__(SCORED ? 1024 : 256) rswa_prefill_order_kernel
             }
             w.fixed_lo = __reduce_min_sync(0xffffffffu, ulo);
             w.fixed_hi = __reduce_max_sync(0xffffffffu, uhi);
-            const int text_tiles = w.n_steps - w.n_prefix_tiles;
             if (w.fixed_hi == 0) w.fixed_lo = 0;
-            w.n_prefix_tiles = (w.fixed_hi + kTcTile - 1) / kTcTile - w.fixed_lo / kTcTile;
-            w.n_steps = w.n_prefix_tiles + text_tiles;
+            // key tiles begin at the block of the first key that is seen, not at a multiple of the tile
+            w.n_prefix_tiles = (w.fixed_hi - tc_block_start(w.fixed_lo) + kTcTile - 1) / kTcTile;
+            w.n_steps = w.n_prefix_tiles;
+            if (w.t.kind == 1) {
+                w.text_tile0 = tc_block_start(max(0, w.t.pos0 - p.window + 1));  // here: the first token of the first text tile
+                w.n_steps += (w.t.pos0 + w.t.rows - w.text_tile0 + kTcTile - 1) / kTcTile;
+            }
         }
         return w;
     };
@@ -641,9 +647,9 @@ rswa_prefill_tc_kernel(const PrefillParams p, const __grid_constant__ PrefillMap
         return (lo > 0 && (lo & (kBlockTokens - 1))) || (hi < kTcTile && (hi & (kBlockTokens - 1)));
     };
     auto first_token = [&](const TcItem& it, int n) {  // of key tile n
-        if (n >= it.n_prefix_tiles) return (it.text_tile0 + n - it.n_prefix_tiles) * kTcTile;
-        if constexpr (Mode::kScored) return (it.fixed_lo / kTcTile + n) * kTcTile;
-        else return n * kTcTile;
+        const bool text = n >= it.n_prefix_tiles;
+        if constexpr (Mode::kScored) return text ? it.text_tile0 + (n - it.n_prefix_tiles) * kTcTile : tc_block_start(it.fixed_lo) + n * kTcTile;
+        else return (text ? it.text_tile0 + n - it.n_prefix_tiles : n) * kTcTile;
     };
     constexpr uint32_t kItemReaders = 8 + 4 + 1 + 1 + 1;
     auto read_slot = [&](uint32_t sl) {
