@@ -537,15 +537,23 @@ struct ScoreMma {
             hi[i] = *reinterpret_cast<const uint4*>(ktile + (g + 8) * ROWB + (c + 4 * i) * 16);
         }
         released();
-        float s0[4] = {0.f, 0.f, 0.f, 0.f}, s1[4] = {0.f, 0.f, 0.f, 0.f};  // two chains
+        float s[2 * NT][4];  // chains of products that do not wait for one another
+#pragma unroll
+        for (int k = 0; k < 2 * NT; ++k)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[k][e] = 0.f;
 #pragma unroll
         for (int i = 0; i < CH; ++i)
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-                mma_16816(s0, lo[i].x, hi[i].x, lo[i].y, hi[i].y, qf[nt][i].x, qf[nt][i].y);
-                mma_16816(s1, lo[i].z, hi[i].z, lo[i].w, hi[i].w, qf[nt][i].z, qf[nt][i].w);
+                mma_16816(s[2 * nt], lo[i].x, hi[i].x, lo[i].y, hi[i].y, qf[nt][i].x, qf[nt][i].y);
+                mma_16816(s[2 * nt + 1], lo[i].z, hi[i].z, lo[i].w, hi[i].w, qf[nt][i].z, qf[nt][i].w);
             }
-        float x0 = (s0[0] + s1[0]) + (s0[1] + s1[1]), x1 = (s0[2] + s1[2]) + (s0[3] + s1[3]);
+        float x0 = (s[0][0] + s[1][0]) + (s[0][1] + s[1][1]), x1 = (s[0][2] + s[1][2]) + (s[0][3] + s[1][3]);
+        if constexpr (NT == 2) {
+            x0 += (s[2][0] + s[3][0]) + (s[2][1] + s[3][1]);
+            x1 += (s[2][2] + s[3][2]) + (s[2][3] + s[3][3]);
+        }
         if constexpr (G == 2) {  // the third part is in the neighbour's columns
             x0 += __shfl_xor_sync(0xffffffffu, x0, 1);
             x1 += __shfl_xor_sync(0xffffffffu, x1, 1);
@@ -605,14 +613,24 @@ struct ScoreMma {
         // element e of chunk k, as (token 2c, token 2c + 1) and (2c + 8, 2c + 9) pairs
         auto word = [](const uint4& w, int e) { return e < 2 ? w.x : e < 4 ? w.y : e < 6 ? w.z : w.w; };
         auto pair = [&](int k, int e, int t) { return __byte_perm(word(v[k][t], e), word(v[k][t + 1], e), (e & 1) ? 0x7632 : 0x5410); };
+        // four 16-dim tiles at a time, so that a tile's second product does not wait for its first
 #pragma unroll
-        for (int m = 0; m < MT; ++m) {
-            // rows g and g + 8 of the 16-dim tile: with 128 dims element m of chunks g and g + 8, with 64 elements m and m + 4 of chunk g
-            constexpr bool kTwo = VC == 2;
-            const int k1 = kTwo ? 1 : 0, e1 = kTwo ? m : m + 4;
-            const uint32_t a0 = pair(0, m, 0), a1 = pair(k1, e1, 0), a2 = pair(0, m, 2), a3 = pair(k1, e1, 2);
+        for (int m0 = 0; m0 < MT; m0 += 4) {
+            uint32_t a[4][4];
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) mma_16816(acc[m], a0, a1, a2, a3, b[nt][0], b[nt][1]);
+            for (int i = 0; i < 4; ++i) {
+                // rows g and g + 8 of the tile: with 128 dims element m of chunks g and g + 8, with 64 elements m and m + 4 of chunk g
+                constexpr bool kTwo = VC == 2;
+                const int m = m0 + i, k1 = kTwo ? 1 : 0, e1 = kTwo ? m : m + 4;
+                a[i][0] = pair(0, m, 0);
+                a[i][1] = pair(k1, e1, 0);
+                a[i][2] = pair(0, m, 2);
+                a[i][3] = pair(k1, e1, 2);
+            }
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) mma_16816(acc[m0 + i], a[i][0], a[i][1], a[i][2], a[i][3], b[nt][0], b[nt][1]);
         }
     }
     __device__ __forceinline__ void emit(const ScoreParams& p, const ScoreItem& it, bool whole, int my_slot, int) {
