@@ -999,19 +999,20 @@ __global__ void __launch_bounds__(kMassThreads) rswa_mass_kernel(const __grid_co
     asm volatile("griddepcontrol.wait;" ::: "memory");  // (launched so that its set-up overlaps the attention)
     const int b = blockIdx.y, tid = threadIdx.x;
     const int slot = __ldg(p.plan.d_slots + b);
+    const int pfx = max(__ldg(p.plan.d_prefill_len + slot), 0);  // (on their way while the batch is looked through)
+    const int len = __ldg(p.plan.d_len + slot);
     int others = 0;  // rows that name the slot too: 1 earlier, 2 later ones
     for (int j = tid; j < p.plan.rows; j += kMassThreads)
         if (j != b && __ldg(p.plan.d_slots + j) == slot) others |= j < b ? 1 : 2;
     if (__syncthreads_or(others & 1)) return;
     const int last = __syncthreads_or(others & 2) ? p.plan.rows : b + 1;
-    const int pfx = max(__ldg(p.plan.d_prefill_len + slot), 0);
     const int n = min(pfx, p.stride);
     if (pfx > p.stride && tid == 0 && blockIdx.x == 0) atomicOr(p.status, kStatusBadSlot);
     const int s = blockIdx.x * kMassThreads + tid;
     if ((int)blockIdx.x * kMassThreads >= n) return;
     const size_t at = (size_t)slot * p.stride + s;
     float sum = (s < n && p.mass_in && p.decay != 0.f) ? p.decay * p.mass_in[at] : 0.f;
-    const int fixed = min(max(__ldg(p.plan.d_len + slot), 0), pfx);
+    const int fixed = min(max(len, 0), pfx);
     for (int r = b; r < last; ++r) {
         if (__ldg(p.plan.d_slots + r) != slot) continue;
         int lo, hi;
@@ -1019,7 +1020,7 @@ __global__ void __launch_bounds__(kMassThreads) rswa_mass_kernel(const __grid_co
         if (s < lo || s >= hi || s >= n) continue;
         const float* sc = p.scores + (size_t)r * p.heads * p.stride + s;
         const float2* ml = reinterpret_cast<const float2*>(p.score_ml) + (size_t)r * p.heads;
-#pragma unroll 8
+#pragma unroll 10
         for (int h = 0; h < p.heads; ++h) {
             const float2 w = __ldcg(ml + h);
             sum += fast_exp2(__ldcs(sc + (size_t)h * p.stride) - w.x) * w.y;
