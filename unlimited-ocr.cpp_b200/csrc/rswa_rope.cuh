@@ -14,6 +14,8 @@
 // before anything else, the warp's table of the row's angles (one entry per pair of one head) is filled meanwhile.  In the half
 // layout a lane owns a chunk and its partner rotary_dim / 2 further on, in the interleaved layout a chunk holds whole pairs; every
 // element is read and written by one lane, so a call may work in place.
+// Measured: 16384 rows of 10 + 10 + 10 heads of 128, bf16 (252 MB) in 51 us, 4.9 TB/s, where a plain copy of the bytes takes 40;
+// four rows around one table and a CTA barrier took 61-64 us, chunks dealt out one by one (twice the instructions) 74.
 #pragma once
 
 #include "rswa_paged.cuh"
