@@ -283,14 +283,47 @@ __device__ __forceinline__ float2 tc_exp2_poly(float2 x) {
 // away what half-hidden tiles allow.)
 constexpr int kTcChunk = 32;
 
-// Scores of a chunk of keys modified in place, into the log2 domain.  tanh(x) = 1 - 2 / (1 + e^2x), right at both ends.  Special
-// functions are the scarce resource (16 results a cycle and SM), so four reciprocals are taken as one, of the product of the four
-// denominators (e^2x is cut at 2^30, where the tanh is 1 already: the product stays below 2^121), and with bf16 results half of
-// the powers go to the polynomial.  The cut also turns the NaN of a key that the row does not see into a number, so it cannot
-// reach the three others through the product; a NaN in the query is reported by the helpers.  d0: the query's position minus that
-// of key 0.
+// tanh(x) / x as a polynomial in x^2 of least maximum relative error (3.9e-9) for |x| <= kTcTanhSmall.
+constexpr float kTcTanhSmall = 0.625f;
+__device__ __forceinline__ float2 tc_tanh_over_x(float2 t) {
+    auto horner = [&](float2 acc, float c) { return __ffma2_rn(acc, t, make_float2(c, c)); };
+    float2 y = horner(make_float2(-0.005659989081323147f, -0.005659989081323147f), 0.02059098891913891f);
+    y = horner(horner(y, -0.05372106656432152f), 0.13331127166748047f);
+    return horner(horner(y, -0.3333325982093811f), 1.f);
+}
+
+// Scores of a chunk of keys modified in place, into the log2 domain.  With a cap, mul makes s the power 2x in e^2x, and
+// tanh(x) = 1 - 2 / (1 + e^2x), right at both ends and off by 2^-21 at most.  Special functions are the scarce resource (16 results
+// a cycle and SM), so four reciprocals are taken as one, of the product of the four denominators (e^2x is cut at 2^30, where the
+// tanh is 1 already: the product stays below 2^121), and with bf16 results half of the powers are a polynomial.  The cut also turns the
+// NaN of a key that the row does not see into a number, so it cannot reach the three others through the product; a NaN in the
+// query is reported by the helpers.  For fp32 results an error of 2^-21 of the cap is much beside scores far below it: a
+// row whose chunk stays below 5/8 of the cap takes a polynomial that is right to 2^-23 of each score.  (The choice is the row's own:
+// its bits depend neither on its neighbours nor on hidden keys, whose scores are zero by then.)  With bf16 results the
+// polynomial gained nothing (60 us became 65 on pages with half-hidden chunks), and a hidden key's score stays in the product of
+// its four, where it can move the last bit of the others' fp32 scores.  d0: the query's position minus that of key 0.
 template <typename Mode>
 __device__ __forceinline__ void tc_modify(uint32_t* s, float mul, float cap_log2, float slope_log2, float d0) {
+    if constexpr (Mode::kCap && Mode::kPairP) {
+        float top = 0.f;
+#pragma unroll
+        for (int j = 0; j < kTcChunk; ++j) top = fmaxf(top, fabsf(__uint_as_float(s[j])));
+        const float to_x = mul * 0.34657359027997264f;  // mul / (2 log2(e))
+        if (top * fabsf(to_x) <= kTcTanhSmall) {
+#pragma unroll
+            for (int j = 0; j < kTcChunk; j += 2) {
+                const float2 x = __fmul2_rn(make_float2(__uint_as_float(s[j]), __uint_as_float(s[j + 1])), make_float2(to_x, to_x));
+                float2 y = __fmul2_rn(__fmul2_rn(x, make_float2(cap_log2, cap_log2)), tc_tanh_over_x(__fmul2_rn(x, x)));
+                if constexpr (Mode::kBias) {
+                    y.x = fmaf(-slope_log2, fabsf(d0 - (float)j), y.x);
+                    y.y = fmaf(-slope_log2, fabsf(d0 - (float)(j + 1)), y.y);
+                }
+                s[j] = __float_as_uint(y.x);
+                s[j + 1] = __float_as_uint(y.y);
+            }
+            return;
+        }
+    }
 #pragma unroll
     for (int j = 0; j < kTcChunk; j += 4) {
         float2 x[2];
@@ -405,7 +438,7 @@ __device__ __forceinline__ bool tc_softmax_half(bool full, uint32_t tS, int h, i
 // probabilities are zero), the scores of hidden keys are only looked for in chunks that some row does not see whole.  lo / hi: what
 // this row sees of this thread's 64 keys; w: what the warp's rows see of them.
 // Measured, cycles per key tile and SM: 3 300 without a cap and 4 900 with one for bf16 rows of 2184 keys (the products take
-// 1 024), 4 100 and 5 500 in fp32 (2 048); pages of 273 in four documents, cap, bf16: 60 us.
+// 1 024), 4 100 and 6 000 in fp32 (2 048); pages of 273 in four documents, cap, bf16: 60 us.
 template <typename Mode>
 __device__ __forceinline__ bool tc_softmax_half_scored(uint32_t tS, int h, int lo, int hi, const TcSpan& w, float* my_max, const float* other_max,
                                                        uint32_t pair_bar, uint32_t pair_parity, int* status, uint32_t wait_limit, float& m_ref,
@@ -417,6 +450,13 @@ __device__ __forceinline__ bool tc_softmax_half_scored(uint32_t tS, int h, int l
 #pragma unroll
     for (int c = 0; c < 64; c += kTcChunk) {
         if (!some_see(c)) continue;
+        if constexpr (Mode::kCap && Mode::kPairP) {  // what the row does not see must not decide how the rest is computed
+            if (c + kTcChunk > w.hi_min || c < w.lo_max) {
+#pragma unroll
+                for (int j = c; j < c + kTcChunk; ++j)
+                    if (j < lo || j >= hi) s[j] = 0u;
+            }
+        }
         tc_modify<Mode>(s + c, mul, cap_log2, slope_log2, d0 - (float)c);
         if (c + kTcChunk > w.hi_min || c < w.lo_max) {
 #pragma unroll
