@@ -921,6 +921,7 @@ __global__ void __launch_bounds__(C::kThreads, 1) rswa_scored_kernel(const __gri
                 asm volatile("atom.add.acq_rel.gpu.global.s32 %0, [%1], 1;" : "=r"(old) : "l"(counter) : "memory");
             old = __shfl_sync(FULL, old, 0);
             if (old != members - 1) break;
+            __syncwarp();  // the arriving lane's acquire covers the loads the whole warp issues next
             if (lane == 0) *counter = 0;  // for the next launch
             const bool last = entries <= kScoreJoin;
             // lane 4 m + h holds (max, sum) of member m, head h; the accumulators follow in 16-byte columns, 128 floats a round
