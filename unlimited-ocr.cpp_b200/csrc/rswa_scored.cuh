@@ -457,9 +457,10 @@ struct ScoreFma {
 //   values   out^T[HD][8] = V^T[HD x 16 tokens] P: lane (g, c) reads chunk(s) g of tokens 2c, 2c + 1, 2c + 8, 2c + 9 and pairs
 //            the tokens' elements with byte permutes; P comes from the lanes that hold the scores by four shuffles.
 // Column n of a product is part n % (8 / G) of head n / (8 / G); with four heads the third parts are a second product into the same
-// accumulators (the columns of a head are summed in the end, whatever they hold).  Two-way (K) and four-way (V) bank conflicts
-// of the unswizzled tiles are left: they stay below the time the tile takes to arrive.  Measured: 16 + 4 heads of 128 over six
-// caches of 24096 tokens (282 MB) 72 us, bound by the latency of a tile's chain with 12 warps an SM; 155 us on the CUDA cores.
+// accumulators (the columns of a head are summed in the end, whatever they hold).  Measured: 16 + 4 heads of 128 over six caches
+// of 24096 tokens (282 MB) 72 us, 155 us on the CUDA cores; bound by the instructions and latency of a tile's chain.  The
+// two-way (K) and four-way (V) bank conflicts of the unswizzled tiles are left: rows fetched one by one into padded slots have none,
+// but sixteen copies a tile cost more (84 us), and 16 warps with the Q fragments in shared memory were slower too (77 us).
 // -------------------------------------------------------------------------------------------------
 __device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
