@@ -10,9 +10,9 @@ using namespace uocr_b200;
 
 namespace {
 
-template <bool CAP, bool BIAS, bool PAIR_Q, bool PAIR_P>
+template <bool CAP, bool BIAS, bool PAIR_Q, bool FINE_CAP>
 int launch(const PrefillParams& pp, const PrefillMaps& maps, int grid, int device, cudaStream_t st) {
-    auto kern = rswa_prefill_tc_kernel<TcMode<true, CAP, BIAS, PAIR_Q, PAIR_P>>;
+    auto kern = rswa_prefill_tc_kernel<TcMode<true, CAP, BIAS, PAIR_Q, FINE_CAP>>;
     static bool configured[64] = {false};  // one per instantiation
     if (!configured[device & 63]) {
         CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kTcSmemBytes), "prefill smem attribute");
@@ -23,11 +23,10 @@ int launch(const PrefillParams& pp, const PrefillMaps& maps, int grid, int devic
 }
 
 template <bool CAP, bool BIAS>
-int launch_types(bool pair_q, bool pair_p, const PrefillParams& pp, const PrefillMaps& maps, int grid, int device, cudaStream_t st) {
-    if (pair_q && pair_p) return launch<CAP, BIAS, true, true>(pp, maps, grid, device, st);
-    if (pair_q) return launch<CAP, BIAS, true, false>(pp, maps, grid, device, st);
-    if (pair_p) return launch<CAP, BIAS, false, true>(pp, maps, grid, device, st);
-    return launch<CAP, BIAS, false, false>(pp, maps, grid, device, st);
+int launch_types(bool pair_q, bool fine_cap, const PrefillParams& pp, const PrefillMaps& maps, int grid, int device, cudaStream_t st) {
+    if (!CAP || fine_cap)  // (without a cap the last argument says nothing)
+        return pair_q ? launch<CAP, BIAS, true, true>(pp, maps, grid, device, st) : launch<CAP, BIAS, false, true>(pp, maps, grid, device, st);
+    return pair_q ? launch<CAP, BIAS, true, !CAP>(pp, maps, grid, device, st) : launch<CAP, BIAS, false, !CAP>(pp, maps, grid, device, st);
 }
 
 int check_score(const uocr_b200_score* score, const char* who) {
@@ -125,12 +124,12 @@ int uocr_b200_rswa_prefill_attention_scored_tc(const uocr_b200_paged_kv* kv, con
         maps.tv = maps.v;
     }
     const int grid = (int)std::min<long long>((long long)n_tiles * heads, di->sms);
-    const bool pair_q = q_dtype == UOCR_B200_F32, pair_p = !ws->out_bf16;
+    const bool pair_q = q_dtype == UOCR_B200_F32, fine_cap = !ws->out_bf16;
     const bool cap = score->softcap > 0.f, bias = score->slopes != nullptr;
-    if (cap && bias) return launch_types<true, true>(pair_q, pair_p, pp, maps, grid, dev, st);
-    if (cap) return launch_types<true, false>(pair_q, pair_p, pp, maps, grid, dev, st);
-    if (bias) return launch_types<false, true>(pair_q, pair_p, pp, maps, grid, dev, st);
-    return launch_types<false, false>(pair_q, pair_p, pp, maps, grid, dev, st);
+    if (cap && bias) return launch_types<true, true>(pair_q, fine_cap, pp, maps, grid, dev, st);
+    if (cap) return launch_types<true, false>(pair_q, fine_cap, pp, maps, grid, dev, st);
+    if (bias) return launch_types<false, true>(pair_q, fine_cap, pp, maps, grid, dev, st);
+    return launch_types<false, false>(pair_q, fine_cap, pp, maps, grid, dev, st);
 }
 
 }  // extern "C"

@@ -63,11 +63,13 @@ struct PrefillTile {
 };
 
 // What a kernel instantiation computes.  SCORED: scores modified as uocr_b200_score says (CAP: tanh cap, BIAS: distance
-// bias) and visible ranges per row; PAIR_Q / PAIR_P: Q / P go to the tensor cores as bf16 pairs (fp32 queries / fp32
-// results) instead of as one bf16 each (bf16 queries, which are exact, / bf16 results, whose own rounding is no finer).
-template <bool SCORED, bool CAP, bool BIAS, bool PAIR_Q, bool PAIR_P>
+// bias) and visible ranges per row; PAIR_Q: Q goes to the tensor cores as bf16 pairs (fp32 queries) instead of as one bf16 each
+// (bf16 queries, which are exact); FINE_CAP: the cap's tanh as exact as fp32 results want it.  P always goes as bf16 pairs: one
+// bf16 would take less (pages of 273 in four documents with a cap: 60 us for 67) but add a rounding as large as that of a bf16
+// result itself (rms error against 64 bits 2.25e-3 for 1.66e-3).
+template <bool SCORED, bool CAP, bool BIAS, bool PAIR_Q, bool FINE_CAP>
 struct TcMode {
-    static constexpr bool kScored = SCORED, kCap = CAP, kBias = BIAS, kPairQ = PAIR_Q, kPairP = PAIR_P;
+    static constexpr bool kScored = SCORED, kCap = CAP, kBias = BIAS, kPairQ = PAIR_Q, kFineCap = FINE_CAP;
 };
 using TcPlain = TcMode<false, false, false, true, true>;
 
@@ -300,11 +302,11 @@ __device__ __forceinline__ float2 tc_tanh_over_x(float2 t) {
 // query is reported by the helpers.  For fp32 results an error of 2^-21 of the cap is much beside scores far below it: a
 // row whose chunk stays below 5/8 of the cap takes a polynomial that is right to 2^-23 of each score.  (The choice is the row's own:
 // its bits depend neither on its neighbours nor on hidden keys, whose scores are zero by then.)  With bf16 results the
-// polynomial gained nothing (60 us became 65 on pages with half-hidden chunks), and a hidden key's score stays in the product of
+// polynomial would cost 8 us on pages with half-hidden chunks (75 for 67), and a hidden key's score stays in the product of
 // its four, where it can move the last bit of the others' fp32 scores.  d0: the query's position minus that of key 0.
 template <typename Mode>
 __device__ __forceinline__ void tc_modify(uint32_t* s, float mul, float cap_log2, float slope_log2, float d0) {
-    if constexpr (Mode::kCap && Mode::kPairP) {
+    if constexpr (Mode::kCap && Mode::kFineCap) {
         float top = 0.f;
 #pragma unroll
         for (int j = 0; j < kTcChunk; ++j) top = fmaxf(top, fabsf(__uint_as_float(s[j])));
@@ -335,7 +337,7 @@ __device__ __forceinline__ void tc_modify(uint32_t* s, float mul, float cap_log2
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 const float2 t = make_float2(fminf(x[i].x, 30.f), fminf(x[i].y, 30.f));
-                if (i == 1 && !Mode::kPairP) e[i] = tc_exp2_poly(make_float2(fmaxf(t.x, -126.f), fmaxf(t.y, -126.f)));
+                if (i == 1 && !Mode::kFineCap) e[i] = tc_exp2_poly(make_float2(fmaxf(t.x, -126.f), fmaxf(t.y, -126.f)));
                 else e[i] = make_float2(tc_exp2(t.x), tc_exp2(t.y));
                 e[i] = __fadd2_rn(e[i], make_float2(1.f, 1.f));
             }
@@ -437,8 +439,8 @@ __device__ __forceinline__ bool tc_softmax_half(bool full, uint32_t tS, int h, i
 // The same with modified scores.  Chunks of keys that no row of the warp sees are left out of everything (their
 // probabilities are zero), the scores of hidden keys are only looked for in chunks that some row does not see whole.  lo / hi: what
 // this row sees of this thread's 64 keys; w: what the warp's rows see of them.
-// Measured, cycles per key tile and SM: 3 300 without a cap and 4 900 with one for bf16 rows of 2184 keys (the products take
-// 1 024), 4 100 and 6 000 in fp32 (2 048); pages of 273 in four documents, cap, bf16: 60 us.
+// Measured, cycles per key tile and SM: 3 700 without a cap and 5 500 with one for bf16 rows of 2184 keys (the products take
+// 1 536), 4 100 and 6 000 in fp32 (2 048); pages of 273 in four documents, cap, bf16: 67 us.
 template <typename Mode>
 __device__ __forceinline__ bool tc_softmax_half_scored(uint32_t tS, int h, int lo, int hi, const TcSpan& w, float* my_max, const float* other_max,
                                                        uint32_t pair_bar, uint32_t pair_parity, int* status, uint32_t wait_limit, float& m_ref,
@@ -450,7 +452,7 @@ __device__ __forceinline__ bool tc_softmax_half_scored(uint32_t tS, int h, int l
 #pragma unroll
     for (int c = 0; c < 64; c += kTcChunk) {
         if (!some_see(c)) continue;
-        if constexpr (Mode::kCap && Mode::kPairP) {  // what the row does not see must not decide how the rest is computed
+        if constexpr (Mode::kCap && Mode::kFineCap) {  // what the row does not see must not decide how the rest is computed
             if (c + kTcChunk > w.hi_min || c < w.lo_max) {
 #pragma unroll
                 for (int j = c; j < c + kTcChunk; ++j)
@@ -485,29 +487,25 @@ __device__ __forceinline__ bool tc_softmax_half_scored(uint32_t tS, int h, int l
     uint32_t pk[32];
 #pragma unroll
     for (int c = 0; c < 64; c += kTcChunk) {
-        // pairs: the chunk's 16 hi words, then its 16 lo words, over its own columns; single bf16: 64 keys in the first 32 of
-        // this thread's columns
-        const int at = Mode::kPairP ? 0 : c / 2;
+        // the chunk's 16 hi words, then its 16 lo words, over its own columns
         if (some_see(c)) {
 #pragma unroll
             for (int e = 0; e < kTcChunk / 2; ++e) {
                 const float2 x = __fadd2_rn(make_float2(__uint_as_float(s[c + 2 * e]), __uint_as_float(s[c + 2 * e + 1])), make_float2(-m_safe, -m_safe));
                 const float2 pr = make_float2(tc_exp2(x.x), tc_exp2(x.y));
                 l2 = __fadd2_rn(l2, pr);
-                if constexpr (Mode::kPairP) tc_split2_rn(pr.x, pr.y, pk[at + e], pk[16 + at + e]);
-                else pk[at + e] = rn_bf16x2(pr.x, pr.y);
+                tc_split2_rn(pr.x, pr.y, pk[e], pk[16 + e]);
             }
         } else {
 #pragma unroll
             for (int e = 0; e < kTcChunk / 2; ++e) {
-                pk[at + e] = 0u;
-                if constexpr (Mode::kPairP) pk[16 + at + e] = 0u;
+                pk[e] = 0u;
+                pk[16 + e] = 0u;
             }
         }
-        if constexpr (Mode::kPairP) tc_st32(tS + h * 64 + c, pk);
+        tc_st32(tS + h * 64 + c, pk);
     }
     static_assert(kTcChunk == 32, "the layout of a pair of words above");
-    if constexpr (!Mode::kPairP) tc_st32(tS + h * 64, pk);
     asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
     l_run = l_run * alpha + l2.x + l2.y;
     return true;
@@ -1198,15 +1196,10 @@ rswa_prefill_tc_kernel(const PrefillParams p, const __grid_constant__ PrefillMap
                     // P: 16 keys = 8 TMEM columns per MMA; every 32 keys hold their 16 hi words, then their 16 lo words.
                     // The accumulator carries over from tile to tile (the item's first product overwrites it).
                     tc_mma_ts(tO, tP, dV[0] + stage, idesc_o, (uint32_t)n);
-                    if constexpr (Mode::kPairP) {
 #pragma unroll
-                        for (int u = 1; u < 16; ++u) {
-                            const int hp = u >> 3, j = u & 7;
-                            tc_mma_ts(tO, tP + (j >> 1) * 32 + hp * 16 + (j & 1) * 8, dV[j] + stage, idesc_o, 1u);
-                        }
-                    } else {  // every 64 keys hold 32 words, then 32 unused columns
-#pragma unroll
-                        for (int j = 1; j < 8; ++j) tc_mma_ts(tO, tP + (j >> 2) * 64 + (j & 3) * 8, dV[j] + stage, idesc_o, 1u);
+                    for (int u = 1; u < 16; ++u) {
+                        const int hp = u >> 3, j = u & 7;
+                        tc_mma_ts(tO, tP + (j >> 1) * 32 + hp * 16 + (j & 1) * 8, dV[j] + stage, idesc_o, 1u);
                     }
                     tc_commit(o_full(b));
                     tc_commit(v_free(b));
