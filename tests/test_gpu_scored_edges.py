@@ -1,0 +1,45 @@
+"""Attention with modified scores where values or ranges are extreme."""
+import pytest
+
+from paged_fixture import load_b200
+from test_gpu_prefill_scored import MODES, Wave, slopes_of
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def b():
+    import torch
+    if not torch.cuda.is_available():
+        pytest.skip("needs a CUDA device")
+    return load_b200()
+
+
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+@pytest.mark.parametrize("cap,bias,q_dtype,out", MODES)
+def test_prefill_infinite_query_of_either_sign(b, cap, bias, q_dtype, out, sign):
+    """An infinity in a query makes its scores +inf or -inf, by the sign of the key's element; either way the row is NaN, unless it sees nothing."""
+    import torch
+    w = Wave(b, torch, [(140, 0, 140, 0), (0, 0, 3, 1), (20, 0, 4, 0)], 2, 2, seed=41)
+    one = w.layer.k.nan_to_num(0)  # every key has the same sign in dim 7
+    one[..., 7] = 1.0
+    w.layer.k.copy_(torch.where(torch.isnan(w.layer.k), w.layer.k, one))
+    tk = w.text[0]
+    tk.copy_(torch.where(torch.isnan(tk), tk, torch.where(torch.arange(128, device="cuda") == 7, torch.ones_like(tk), tk)))
+    q = w.q.clone()
+    bad = [0, 1, 127, 128, 139, 140, 142, 143, 146]
+    q[bad, 7] = sign * float("inf")  # head 0
+    q = q.to(getattr(torch, q_dtype))
+    hi = torch.cat([torch.arange(1, 141), torch.zeros(3), torch.zeros(4)]).to(torch.int32).cuda()  # the last request's rows see nothing
+    pos = torch.arange(w.total, dtype=torch.int32, device="cuda")
+    ws = b.Workspace(64)
+    ws.set_out_dtype(b.BF16 if out == "bfloat16" else b.F32)
+    got = torch.full((w.total, 256), 7.0, dtype=getattr(torch, out), device="cuda")
+    score = b.Score(softcap=cap, slopes=slopes_of(torch, 2) if bias else None, d_q_pos=pos, d_hi=hi)
+    b.prefill_attention_scored_tc(w.layer, *w.text, w.text_blocks, score, q, w.d_prefill, w.tiles, 9, 2, got, ws)
+    assert ws.status() == 0
+    hurt = torch.zeros(w.total, dtype=torch.bool, device="cuda")
+    hurt[bad] = True
+    hurt[143:] = False
+    assert torch.isnan(got[hurt][:, :128]).all() and torch.isfinite(got[~hurt]).all() and torch.isfinite(got[:, 128:]).all()
+    assert not got[143:].any()
