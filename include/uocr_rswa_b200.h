@@ -569,7 +569,9 @@ UOCR_B200_API int uocr_b200_rswa_prefill_text_scored_paged(
  * uocr_b200_rswa_prefill_attention_tc with modified scores, tiles and plans as there.  d_lo / d_hi / d_q_pos are
  * per packed row.  A plan (made by the plan call, or by the attention call when h_tiles is given) covers the
  * keys that some row of a tile sees and so belongs to the ranges it was made with: it is reused by calls whose d_lo,
- * d_hi and prefix lengths still hold the same values, and never by the call without modified scores.  fp32
+ * d_hi and prefix lengths still hold the same values, and never by the call without modified scores.  Ranges that have become
+ * narrower are right with it too; a row that sees a key which no row of its tile saw when the plan was made sets status bit 4,
+ * and its result is void.  fp32
  * queries and the probabilities go through the tensor cores as bf16 pairs, bf16 queries are taken as they are.  K and V outside
  * the span of keys that the rows of a query tile see -- from the first to the last -- may hold anything; inside it
  * they must be finite, since the rows that do not see a key multiply its value by zero. A query row that holds a NaN or an

@@ -43,3 +43,43 @@ def test_prefill_infinite_query_of_either_sign(b, cap, bias, q_dtype, out, sign)
     hurt[143:] = False
     assert torch.isnan(got[hurt][:, :128]).all() and torch.isfinite(got[~hurt]).all() and torch.isfinite(got[:, 128:]).all()
     assert not got[143:].any()
+
+
+@pytest.mark.parametrize("change", ["hi", "lo", "default", "prefix", "empty"])
+def test_plan_that_no_longer_covers_the_ranges_is_reported(b, change):
+    """A plan is reused with other ranges or prefix lengths than it was made for: reported where a row sees a key that no row of its tile saw then."""
+    import torch
+    w = Wave(b, torch, [(300, 0, 200, 0), (300, 0, 60, 1)], 2, 2, seed=5)
+    full = lambda v: torch.full((w.total,), v, dtype=torch.int32, device="cuda")
+    ws = b.Workspace(64)
+    out = torch.empty(w.total, 256, device="cuda")
+    plan = lambda score: b.prefill_plan_scored_tc(score, w.tiles, w.d_prefill, 16, ws)
+
+    def status(score):
+        b.prefill_attention_scored_tc(w.layer, *w.text, w.text_blocks, score, w.q, w.d_prefill, w.tiles, 16, 2, out, ws, reuse_plan=True)
+        return ws.status()
+    narrow, wide = {
+        "hi": (b.Score(d_hi=full(100)), b.Score(d_hi=full(101))),
+        "lo": (b.Score(d_lo=full(40), d_hi=full(290)), b.Score(d_lo=full(39), d_hi=full(290))),
+        "default": (b.Score(d_hi=full(16)), b.Score()),
+        "prefix": (b.Score(d_hi=full(400)),) * 2,
+        "empty": (b.Score(d_hi=full(0)), b.Score(d_lo=full(299), d_hi=full(300))),
+    }[change]
+    if change == "prefix":
+        w.d_prefill.fill_(100)
+    plan(narrow)
+    assert status(narrow) == 0
+    if change == "prefix":
+        w.d_prefill.fill_(300)
+    assert status(wide) == b.STATUS_BAD_SLOT
+    plan(wide)
+    assert status(wide) == 0
+    want = out.clone()
+    if change == "prefix":
+        return
+    # the other way round the plan covers more than is seen, and the result is that of a plan of its own
+    plan(narrow)
+    assert status(narrow) == 0
+    own = out.clone()
+    plan(wide)
+    assert status(narrow) == 0 and torch.equal(out, own) and not torch.equal(out, want)

@@ -791,7 +791,12 @@ rswa_prefill_tc_kernel(const PrefillParams p, const __grid_constant__ PrefillMap
             float slope_log2 = 0.f;
             TcSpan fixed_span = {}, text_span = {};
             if constexpr (Mode::kScored) {
-                if (live) tc_row_range(p, t, r, cur.pfx, plo, phi);
+                if (live) {
+                    // The plan fixed the keys that the tile's rows may see; ranges and prefix lengths are those of now.  A row that has
+                    // come to see others would lose them: it is reported.
+                    tc_row_range(p, t, r, max(__ldg(p.d_prefill_len + t.slot), 0), plo, phi);
+                    if (plo < phi && (plo < cur.fixed_lo || phi > cur.fixed_hi)) atomicOr(p.status, kStatusBadSlot);
+                }
                 fixed_span = tc_span(live, plo, phi);
                 if (t.kind == 1) text_span = tc_span(live, tlo, thi);
                 if constexpr (Mode::kBias) {
