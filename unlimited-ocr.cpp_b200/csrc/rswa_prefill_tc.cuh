@@ -848,7 +848,8 @@ rswa_prefill_tc_kernel(const PrefillParams p, const __grid_constant__ PrefillMap
             }
             if (!ok) break;
             // the row's sum over this thread's key half goes to the helper that writes the row out
-            xsum[((itc & 1u) * 2 + h) * 128 + r] = l_run;
+            // (modified scores: -1 for a row that sees no key)
+            xsum[((itc & 1u) * 2 + h) * 128 + r] = Mode::kScored && t.kind == 0 && phi <= plo ? -1.f : l_run;
             mbar_arrive(l_ready(itc));
             g += cur.n_steps;
         }
@@ -946,12 +947,8 @@ rswa_prefill_tc_kernel(const PrefillParams p, const __grid_constant__ PrefillMap
             if (!__all_sync(0xffffffffu, mbar_wait_bounded(l_ready(um), (um >> 1) & 1u, p.status, p.wait_limit))) { ok = false; break; }
             const float l_tot = xsum[((um & 1u) * 2 + 0) * 128 + r] + xsum[((um & 1u) * 2 + 1) * 128 + r];
             float inv = l_tot > 0.f ? 1.f / l_tot : 0.f;
-            if (Mode::kScored && (nxt.valid ? q_bad : next_bad) && r < cur.t.rows) {  // (convert_q has moved on to the next item's row)
-                // NaN if the row sees a key.  (Its sum does not tell: an infinity can make every score -inf and the sum 0.)
-                int lo = 0, hi = 1;
-                if (cur.t.kind == 0) tc_row_range(p, cur.t, r, cur.pfx, lo, hi);
-                if (lo < hi) inv = __uint_as_float(0x7fffffffu);
-            }
+            // (convert_q has moved on to the next item's row; a sum of 0 may be that of a row whose scores are all -inf)
+            if (Mode::kScored && (nxt.valid ? q_bad : next_bad) && !(l_tot < 0.f)) inv = __uint_as_float(0x7fffffffu);
             if (!__all_sync(0xffffffffu, mbar_wait_bounded(o_done, um & 1u, p.status, p.wait_limit))) { ok = false; break; }
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll 1
