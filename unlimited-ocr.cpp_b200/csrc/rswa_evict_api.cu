@@ -16,11 +16,8 @@ int uocr_b200_rswa_evict_select(const float* mass, int mass_stride, const int* d
     int dev = 0;
     CHECK_CUDA(cudaGetDevice(&dev), "cudaGetDevice");
     const int tokens = mass_stride < kSelectSharedTokens ? mass_stride : kSelectSharedTokens;
-    static bool configured[64] = {false};
-    if (!configured[dev & 63]) {
-        CHECK_CUDA(cudaFuncSetAttribute(rswa_evict_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSelectSharedTokens * (int)sizeof(uint32_t)), "smem attribute");
-        configured[dev & 63] = true;
-    }
+    static SmemLimit limit;
+    CHECK_CUDA(limit.allow(rswa_evict_select_kernel, dev, kSelectSharedTokens * (int)sizeof(uint32_t)), "smem attribute");
     SelectParams p{};
     p.mass = mass;
     p.mass_stride = mass_stride;

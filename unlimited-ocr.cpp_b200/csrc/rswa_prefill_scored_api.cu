@@ -13,11 +13,8 @@ namespace {
 template <bool CAP, bool BIAS, bool PAIR_Q, bool FINE_CAP>
 int launch(const PrefillParams& pp, const PrefillMaps& maps, int grid, int device, cudaStream_t st) {
     auto kern = rswa_prefill_tc_kernel<TcMode<true, CAP, BIAS, PAIR_Q, FINE_CAP>>;
-    static bool configured[64] = {false};  // one per instantiation
-    if (!configured[device & 63]) {
-        CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kTcSmemBytes), "prefill smem attribute");
-        configured[device & 63] = true;
-    }
+    static SmemLimit limit;  // one per instantiation
+    CHECK_CUDA(limit.allow(kern, device, kTcSmemBytes), "prefill smem attribute");
     kern<<<grid, kTcThreads, kTcSmemBytes, st>>>(pp, maps);
     return after_launch("tensor-core prefill attention (modified scores)");
 }

@@ -12,18 +12,16 @@ template <typename C, int HD>
 int launch_scored(ScoreParams& p, const DeviceInfo& di, const uocr_b200_workspace* ws, cudaStream_t st) {
     constexpr int per_warp = kScoreRing * C::kTile;
     const int plan_bytes = p.rows <= kScoreSharedRows ? (int)(sizeof(ScoreRow) * p.rows + sizeof(long long) * (p.rows + 1 + 32)) : 0;
-    int warps = ((di.smem_optin < 200 * 1024 ? di.smem_optin : 200 * 1024) - 1024 - plan_bytes) / per_warp;
+    const int budget = di.smem_optin < 200 * 1024 ? di.smem_optin : 200 * 1024;
+    int warps = (budget - 1024 - plan_bytes) / per_warp;
     if (warps > C::kThreads / 32) warps = C::kThreads / 32;
     if (warps < 1) return fail(UOCR_B200_ERR_UNSUPPORTED, "attention_scored: tile does not fit in shared memory");
     p.total_warps = di.sms * warps;
     if (p.total_warps > ws->total_warps_max) return fail(UOCR_B200_ERR_WORKSPACE, "attention_scored: workspace built for a smaller device");
     const int smem = ((warps * kScoreRing * 8 + 127) & ~127) + warps * per_warp + plan_bytes;
     auto kern = rswa_scored_kernel<C, HD>;
-    static int configured[64] = {0};  // one per instantiation
-    if (configured[ws->device & 63] < smem) {
-        CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), "smem attribute");
-        configured[ws->device & 63] = smem;
-    }
+    static SmemLimit limit;  // one per instantiation
+    CHECK_CUDA(limit.allow(kern, ws->device, budget), "smem attribute");
     kern<<<di.sms, warps * 32, smem, st>>>(p);
     return after_launch("attention with modified scores");
 }

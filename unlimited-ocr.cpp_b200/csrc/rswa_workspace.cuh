@@ -5,6 +5,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
 #include <string>
 
 #include "rswa_device.cuh"
@@ -37,6 +38,19 @@ struct DeviceInfo {
 };
 // The current device, refused unless it is an sm_100 part.
 int device_info(const DeviceInfo** out);
+
+// Dynamic shared memory of a kernel (one object per instantiation), allowed once per device.  `bytes` is the most that any call
+// asks for, not what this one does: threads that raised the limit to sizes of their own could lower one another's.
+struct SmemLimit {
+    std::atomic<bool> set[64] = {};
+    template <typename Kernel>
+    cudaError_t allow(Kernel kernel, int device, int bytes) {
+        if (set[device & 63].load(std::memory_order_acquire)) return cudaSuccess;
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+        if (e == cudaSuccess) set[device & 63].store(true, std::memory_order_release);
+        return e;
+    }
+};
 
 // Launches a kernel that opens with griddepcontrol.wait: its set-up may overlap the launch before it in the stream.
 template <typename P>
