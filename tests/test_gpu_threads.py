@@ -9,7 +9,7 @@ pytestmark = pytest.mark.gpu
 HERE = os.path.dirname(os.path.abspath(__file__))
 
 
-@pytest.mark.parametrize("what", ["scored"])
+@pytest.mark.parametrize("what", ["scored", "fused"])
 def test_first_calls_of_several_threads(what):
     """Threads with batches of different sizes set the same kernel up at the same time: no launch is refused then or later."""
     import torch

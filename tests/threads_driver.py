@@ -1,7 +1,8 @@
 """Several host threads make their first calls of the same kernels at a time, each with a batch size, a workspace and a stream of
 its own (run as a program of its own: only first calls set a kernel up).  Prints the calls that were refused.
 
-  threads_driver.py scored     attention with modified scores, every instantiation"""
+  threads_driver.py scored     attention with modified scores, every instantiation
+  threads_driver.py fused      append and attention of a decode step in one launch"""
 import ctypes as C
 import sys
 import threading
@@ -60,8 +61,14 @@ def scored(b, L, layer, score, q, kv, d_len, d_ring, d_prefill, slots, rows, gro
         group, out.data_ptr(), None, ws.h, stream.cuda_stream)
 
 
-CALL = {"scored": scored}
-GROUPS = {"scored": (1, 2, 4)}
+def fused(b, L, layer, score, q, kv, d_len, d_ring, d_prefill, slots, rows, group, out, ws, stream):
+    return L.uocr_b200_rswa_decode_step_paged(
+        C.byref(layer.desc), q.data_ptr(), kv.data_ptr(), kv.data_ptr(), d_len.data_ptr(), d_ring.data_ptr(), d_prefill.data_ptr(), slots.data_ptr(), rows, 16,
+        group, out.data_ptr(), ws.h, stream.cuda_stream)
+
+
+CALL = {"scored": scored, "fused": fused}
+GROUPS = {"scored": (1, 2, 4), "fused": (1,)}
 
 if __name__ == "__main__":
     sys.exit(main(sys.argv[1]))

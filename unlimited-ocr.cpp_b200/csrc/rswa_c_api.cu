@@ -301,8 +301,8 @@ int launch_partial(const AttnParams& ap, const DeviceInfo& di, int* warps_used, 
     using M = TileMap<KV, HD>;
     constexpr int per_warp = kRing * M::kTileBytes;
     const int plan_bytes = FUSED ? (int)(sizeof(RowInfo) * ap.rows + sizeof(int) * (3 * ap.rows + 1 + 33) + 128) : 0;
-    const int budget = (di.smem_optin < 200 * 1024 ? di.smem_optin : 200 * 1024) - 1024 - plan_bytes -
-                       kMaxWarpsPerCta * kPendMax * (int)sizeof(int);
+    const int most = di.smem_optin < 200 * 1024 ? di.smem_optin : 200 * 1024;
+    const int budget = most - 1024 - plan_bytes - kMaxWarpsPerCta * kPendMax * (int)sizeof(int);
     int warps = budget / per_warp;
     if (warps > kMaxWarpsPerCta) warps = kMaxWarpsPerCta;
     if (warps < 1) return fail(UOCR_B200_ERR_UNSUPPORTED, "tile does not fit in shared memory");
@@ -312,13 +312,10 @@ int launch_partial(const AttnParams& ap, const DeviceInfo& di, int* warps_used, 
     const int bar_bytes = (warps * kRing * 8 + 127) & ~127;
     const int smem = bar_bytes + warps * per_warp + warps * kPendMax * (int)sizeof(int) + plan_bytes;
     auto kern = rswa_attn_kernel<KV, HD, PAGED, FUSED, ROPE>;
-    static int configured_smem[64] = {0};  // one per instantiation of this template
+    static SmemLimit limit;  // one per instantiation of this template
     int dev = 0;
     cudaGetDevice(&dev);
-    if (configured_smem[dev] < smem) {
-        CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), "smem attribute");
-        configured_smem[dev] = smem;
-    }
+    CHECK_CUDA(limit.allow(kern, dev, most), "smem attribute");
     if (FUSED && overlap) {
         // programmatic dependent launch: this grid may become resident while the previous kernel in the
         // stream is still draining; the kernel itself waits for it before consuming inputs or scratch
