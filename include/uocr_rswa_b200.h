@@ -513,8 +513,8 @@ UOCR_B200_API int uocr_b200_rswa_rope_append_decode_batch_paged(
  * own rule).  Everything is computed in fp32; `out` is fp32 or bf16 as the workspace says.
  * ============================================================================================= */
 typedef struct {
-    float scale;         /* 0: 1/sqrt(head_dim)                                                        */
-    float softcap;       /* 0: none; otherwise at least 1e-6                                           */
+    float scale;         /* 0: 1/sqrt(head_dim); 3 * scale / min(softcap, 1) must be finite in fp32    */
+    float softcap;       /* 0: none; otherwise 1e-6 to 1e30                                            */
     const float* slopes; /* device [heads], or null: no bias                                           */
     const int* d_q_pos;  /* device [rows], position of each query row; needed with slopes (ragged vision
                             rows default to d_pos)                                                     */

@@ -83,3 +83,20 @@ def test_plan_that_no_longer_covers_the_ranges_is_reported(b, change):
     own = out.clone()
     plan(wide)
     assert status(narrow) == 0 and torch.equal(out, own) and not torch.equal(out, want)
+
+
+@pytest.mark.parametrize("cap", [1e6, 1e20, 1e30])
+@pytest.mark.parametrize("heads,kvh,hd,pool", [(2, 2, 128, "bf16"), (8, 2, 128, "bf16"), (3, 1, 32, "f32")])
+def test_caps_far_above_the_scores_say_nothing(b, heads, kvh, hd, pool, cap):
+    """Up to the largest cap: the result is the one without, within the bound of that (20 roundings of a score) plus the tanh's 2 ulp
+    (4 roundings of the score, so 24 / 20 of it)."""
+    import torch
+    from score_fixture import Caches, attend, check_out
+    c = Caches([(90, 20, 0)], kvh, hd, b.BF16 if pool == "bf16" else b.F32, 24, seed=7)
+    ints = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")
+    q = torch.randn(1, heads * hd, device="cuda") * 2
+    ws, out = b.Workspace(1), torch.empty(1, heads * hd, device="cuda")
+    b.attention_scored_batch_paged(c.layer, b.Score(softcap=cap), q, c.d_len, c.d_ring, c.d_prefill, ints(0), 1, 24, heads, out, ws)
+    assert ws.status() == 0
+    want, _, tol, _ = attend(q[0].double().cpu().numpy(), c.k[0], c.v[0], 0.0, heads, kvh, hd)
+    check_out(torch, out[0], want, 1.2 * tol)

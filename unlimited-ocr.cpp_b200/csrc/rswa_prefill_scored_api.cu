@@ -26,13 +26,11 @@ int launch_types(bool pair_q, bool fine_cap, const PrefillParams& pp, const Pref
     return pair_q ? launch<CAP, BIAS, true, !CAP>(pp, maps, grid, device, st) : launch<CAP, BIAS, false, !CAP>(pp, maps, grid, device, st);
 }
 
-int check_score(const uocr_b200_score* score, const char* who) {
-    auto bad = [&](const char* what) { return fail(UOCR_B200_ERR_INVALID, std::string(who) + ": " + what); };
-    if (!score) return bad("null pointer");
-    if (!(score->softcap == 0.f || score->softcap >= 1e-6f) || !std::isfinite(score->softcap)) return bad("softcap must be 0 (none) or at least 1e-6");
+// What this call takes of the modified scores.
+int check_tc_score(const uocr_b200_score* score, const char* who) {
+    if (int rc = check_score(score, kTcTile, who)) return rc;
     // the kernel's tanh is off by 2^-21 of the cap: a cap far above the scores would drown them
     if (score->softcap > 256.f) return fail(UOCR_B200_ERR_UNSUPPORTED, std::string(who) + ": softcap above 256 (use the calls for any geometry)");
-    if (!std::isfinite(score->scale)) return bad("scale must be finite (0: 1/sqrt(head_dim))");
     if (score->d_key_pos) return fail(UOCR_B200_ERR_UNSUPPORTED, std::string(who) + ": keys stand at their own index here (d_key_pos: use the calls for any geometry)");
     return UOCR_B200_OK;
 }
@@ -43,7 +41,7 @@ extern "C" {
 
 int uocr_b200_rswa_prefill_plan_scored_tc(const uocr_b200_score* score, const uocr_b200_prefill_tile* h_tiles, int n_tiles,
                                           const int* d_prefill_len, int window, uocr_b200_workspace* ws, uocr_b200_stream_t stream) {
-    if (int rc = check_score(score, "prefill_plan_scored_tc")) return rc;
+    if (int rc = check_tc_score(score, "prefill_plan_scored_tc")) return rc;
     return prefill_plan(h_tiles, n_tiles, d_prefill_len, window, score, ws, reinterpret_cast<cudaStream_t>(stream), "prefill_plan_scored_tc");
 }
 
@@ -57,7 +55,7 @@ int uocr_b200_rswa_prefill_attention_scored_tc(const uocr_b200_paged_kv* kv, con
     PagedView pv;
     if (int rc = paged_view(kv, &pv)) return rc;
     if (kv->dtype != UOCR_B200_BF16 || kv->head_dim != kTcTile) return fail(UOCR_B200_ERR_UNSUPPORTED, std::string(who) + ": needs bf16 KV and head_dim 128");
-    if (int rc = check_score(score, who)) return rc;
+    if (int rc = check_tc_score(score, who)) return rc;
     if (!q || !out || !d_prefill_len || !ws) return bad("null pointer");
     if (q_dtype != UOCR_B200_F32 && q_dtype != UOCR_B200_BF16) return fail(UOCR_B200_ERR_UNSUPPORTED, std::string(who) + ": q must be fp32 or bf16");
     if (!aligned16(q) || !aligned16(out)) return bad("q/out must be 16-byte aligned");

@@ -68,12 +68,11 @@ int run_scored(const uocr_b200_paged_kv* kv, const uocr_b200_score* score, const
     auto bad = [&](const char* what) { return fail(UOCR_B200_ERR_INVALID, std::string(who) + ": " + what); };
     PagedView pv;
     if (int rc = paged_view(kv, &pv)) return rc;
-    if (!score || !q || !out || !ws || !plan.d_slots || !plan.d_prefill_len) return bad("null pointer");
+    if (int rc = check_score(score, kv->head_dim, who)) return rc;
+    if (!q || !out || !ws || !plan.d_slots || !plan.d_prefill_len) return bad("null pointer");
     if (q_dtype != UOCR_B200_F32 && q_dtype != UOCR_B200_BF16) return fail(UOCR_B200_ERR_UNSUPPORTED, std::string(who) + ": q must be fp32 or bf16");
     if (heads <= 0 || heads % kv->kv_heads != 0) return bad("heads must be a positive multiple of kv_heads");
     if (!aligned16(q) || !aligned16(out)) return bad("q/out must be 16-byte aligned");
-    if (!(score->softcap == 0.f || score->softcap >= 1e-6f) || !std::isfinite(score->softcap)) return bad("softcap must be 0 (none) or at least 1e-6");
-    if (!std::isfinite(score->scale)) return bad("scale must be finite (0: 1/sqrt(head_dim))");
     if (score->d_key_pos && score->key_pos_stride <= 0) return bad("key_pos_stride must be positive");
     if (score->slopes && plan.mode != kScoreRagged && !score->d_q_pos) return bad("a distance bias needs d_q_pos");
     if (plan.rows > ws->max_rows) return fail(UOCR_B200_ERR_WORKSPACE, std::string(who) + ": more rows than the workspace was created for");
@@ -172,6 +171,21 @@ int run_scored(const uocr_b200_paged_kv* kv, const uocr_b200_score* score, const
 }
 
 }  // namespace
+
+namespace uocr_b200 {
+
+int check_score(const uocr_b200_score* score, int head_dim, const char* who) {
+    auto bad = [&](const char* what) { return fail(UOCR_B200_ERR_INVALID, std::string(who) + ": " + what); };
+    if (!score) return bad("null pointer");
+    if (!(score->softcap == 0.f || (score->softcap >= 1e-6f && score->softcap <= 1e30f))) return bad("softcap must be 0 (none) or in [1e-6, 1e30]");
+    if (!std::isfinite(score->scale)) return bad("scale must be finite (0: 1/sqrt(head_dim))");
+    // what q is multiplied by on the way into the log2 domain, twice of it at most
+    const double scale = score->scale != 0.f ? (double)score->scale : 1.0 / std::sqrt((double)head_dim);
+    if (!std::isfinite((float)(2 * 1.4426950408889634 * scale / (score->softcap > 0.f ? std::fmin(score->softcap, 1.f) : 1.f)))) return bad("scale (over softcap) overflows fp32");
+    return UOCR_B200_OK;
+}
+
+}  // namespace uocr_b200
 
 extern "C" {
 

@@ -82,6 +82,9 @@ inline bool head_dim_ok(int hd, int dtype) {
     return (hd & (hd - 1)) == 0;
 }
 
+// The cap and the scale of modified scores.
+int check_score(const uocr_b200_score* score, int head_dim, const char* who);
+
 struct PagedView;
 struct LayerPools;
 // Checked views of one layer, and of several layers of one geometry behind one block table.
