@@ -100,3 +100,21 @@ def test_caps_far_above_the_scores_say_nothing(b, heads, kvh, hd, pool, cap):
     assert ws.status() == 0
     want, _, tol, _ = attend(q[0].double().cpu().numpy(), c.k[0], c.v[0], 0.0, heads, kvh, hd)
     check_out(torch, out[0], want, 1.2 * tol)
+
+
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+@pytest.mark.parametrize("heads,hd,pool,prefix", [(1, 64, "bf16", 20), (2, 128, "bf16", 20), (4, 64, "bf16", 20), (3, 16, "f32", 20), (1, 64, "f32", 3000), (4, 128, "bf16", 3000)])
+def test_decode_infinite_query_of_either_sign(b, heads, hd, pool, prefix, sign):
+    """Scores that are all +inf or all -inf leave inf - inf in the softmax: NaN, as a whole item and joined from pieces."""
+    import torch
+    from score_fixture import Caches
+    c = Caches([(prefix, 5, 0)], 1, hd, b.BF16 if pool == "bf16" else b.F32, 16, seed=2)
+    k = c.layer.k
+    k[..., 3] = torch.where(torch.isnan(k[..., 3]), k[..., 3], torch.ones_like(k[..., 3]))
+    ints = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")
+    q = torch.randn(2, heads * hd, device="cuda")
+    q[0, 3] = sign * float("inf")  # row 0, head 0
+    ws, out = b.Workspace(2), torch.zeros(2, heads * hd, device="cuda")
+    b.attention_scored_batch_paged(c.layer, b.Score(), q, c.d_len, c.d_ring, c.d_prefill, ints(0, 0), 2, 16, heads, out, ws)
+    assert ws.status() == 0
+    assert torch.isnan(out[0, :hd]).all() and torch.isfinite(out[0, hd:]).all() and torch.isfinite(out[1]).all()

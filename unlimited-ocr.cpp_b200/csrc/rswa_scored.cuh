@@ -422,7 +422,7 @@ struct ScoreFma {
             for (int e = 0; e < EPL; ++e)
 #pragma unroll
                 for (int d = LPR; d < 32; d <<= 1) acc[e] += __shfl_xor_sync(0xffffffffu, acc[e], d);
-            const float inv = lsum == 0.f ? 0.f : 1.f / lsum;
+            const float inv = 1.f / lsum;  // (0 only where every score is -inf: 0/0, NaN)
             if (lane < LPR) {
                 float* dst = p.part_acc + (size_t)my_slot * (G * HD) + h * HD;
                 const size_t at = ((size_t)it.index * G + h) * HD;
@@ -642,7 +642,7 @@ struct ScoreMma {
         float lsum = l_run;
 #pragma unroll
         for (int d = 4; d <= 16; d <<= 1) lsum += __shfl_xor_sync(0xffffffffu, lsum, d);
-        const float inv = lsum == 0.f ? 0.f : 1.f / lsum;
+        const float inv = 1.f / lsum;
         float lo[MT], hi[MT];  // rows g, g + 8 of the tiles
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
@@ -957,7 +957,7 @@ __global__ void __launch_bounds__(C::kThreads, 1) rswa_scored_kernel(const __gri
                     o[c].w = fmaf(t[m].w, w, o[c].w);
                 }
             }
-            const float inv_lane = lsum == 0.f ? 0.f : 1.f / lsum;
+            const float inv_lane = 1.f / lsum;
 #pragma unroll
             for (int c = 0; c < kRounds; ++c) {
                 const int col = c * 128 + lane * 4;
