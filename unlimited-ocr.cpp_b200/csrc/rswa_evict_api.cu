@@ -13,6 +13,7 @@ int uocr_b200_rswa_evict_select(const float* mass, int mass_stride, const int* d
     if (mass_stride <= 0 || keep <= 0 || sinks < 0 || recent < 0) return fail(UOCR_B200_ERR_INVALID, "evict_select: mass_stride and keep must be positive, sinks and recent not negative");
     const DeviceInfo* di = nullptr;
     if (int rc = device_info(&di)) return rc;
+    if (int rc = check_workspace_device(ws, "evict_select")) return rc;
     int dev = 0;
     CHECK_CUDA(cudaGetDevice(&dev), "cudaGetDevice");
     const int tokens = mass_stride < kSelectSharedTokens ? mass_stride : kSelectSharedTokens;
@@ -44,6 +45,9 @@ int uocr_b200_rswa_evict_compact_paged_layers(const uocr_b200_paged_kv* kv_layer
     if (!d_prefill_len || !d_slots || !d_keep || !d_keep_len) return fail(UOCR_B200_ERR_INVALID, "evict_compact_paged_layers: null pointer");
     if (keep_stride <= 0 || (d_new_blocks && new_stride <= 0)) return fail(UOCR_B200_ERR_INVALID, "evict_compact_paged_layers: strides must be positive");
     if (n > 65535) return fail(UOCR_B200_ERR_UNSUPPORTED, "evict_compact_paged_layers: at most 65535 slots per call");
+    const DeviceInfo* di = nullptr;
+    if (int rc = device_info(&di)) return rc;
+    if (int rc = check_workspace_device(ws, "evict_compact_paged_layers")) return rc;
     p.table = pv.table;
     p.table_stride = pv.table_stride;
     p.num_blocks = pv.num_blocks;
@@ -72,6 +76,9 @@ int uocr_b200_rswa_evict_publish(int32_t* block_table, int table_stride, const i
     if (table_stride <= 0 || keep_stride <= 0 || layers <= 0 || window <= 0 || (d_new_blocks && new_stride <= 0) || (mass && mass_stride <= 0) ||
         (d_key_pos && key_pos_stride <= 0))
         return fail(UOCR_B200_ERR_INVALID, "evict_publish: bad geometry");
+    const DeviceInfo* di = nullptr;
+    if (int rc = device_info(&di)) return rc;
+    if (int rc = check_workspace_device(ws, "evict_publish")) return rc;
     EvictPublishParams p{};
     p.table = block_table;
     p.table_stride = table_stride;

@@ -42,6 +42,11 @@ extern "C" {
 int uocr_b200_rswa_prefill_plan_scored_tc(const uocr_b200_score* score, const uocr_b200_prefill_tile* h_tiles, int n_tiles,
                                           const int* d_prefill_len, int window, uocr_b200_workspace* ws, uocr_b200_stream_t stream) {
     if (int rc = check_tc_score(score, "prefill_plan_scored_tc")) return rc;
+    const DeviceInfo* di = nullptr;
+    if (ws) {
+        if (int rc = device_info(&di)) return rc;
+        if (int rc = check_workspace_device(ws, "prefill_plan_scored_tc")) return rc;
+    }
     return prefill_plan(h_tiles, n_tiles, d_prefill_len, window, score, ws, reinterpret_cast<cudaStream_t>(stream), "prefill_plan_scored_tc");
 }
 
@@ -64,9 +69,7 @@ int uocr_b200_rswa_prefill_attention_scored_tc(const uocr_b200_paged_kv* kv, con
     if (text_k_pool && (!aligned16(text_k_pool) || !aligned16(text_v_pool))) return bad("the text pools must be 16-byte aligned");
     const DeviceInfo* di = nullptr;
     if (int rc = device_info(&di)) return rc;
-    int dev = 0;
-    CHECK_CUDA(cudaGetDevice(&dev), "cudaGetDevice");
-    if (dev != ws->device) return bad("the workspace belongs to another device");
+    if (int rc = check_workspace_device(ws, who)) return rc;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     if (h_tiles) {
         if (int rc = prefill_plan(h_tiles, n_tiles, d_prefill_len, window, score, ws, st, who)) return rc;
@@ -121,10 +124,10 @@ int uocr_b200_rswa_prefill_attention_scored_tc(const uocr_b200_paged_kv* kv, con
     const int grid = (int)std::min<long long>((long long)n_tiles * heads, di->sms);
     const bool pair_q = q_dtype == UOCR_B200_F32, fine_cap = !ws->out_bf16;
     const bool cap = score->softcap > 0.f, bias = score->slopes != nullptr;
-    if (cap && bias) return launch_types<true, true>(pair_q, fine_cap, pp, maps, grid, dev, st);
-    if (cap) return launch_types<true, false>(pair_q, fine_cap, pp, maps, grid, dev, st);
-    if (bias) return launch_types<false, true>(pair_q, fine_cap, pp, maps, grid, dev, st);
-    return launch_types<false, false>(pair_q, fine_cap, pp, maps, grid, dev, st);
+    if (cap && bias) return launch_types<true, true>(pair_q, fine_cap, pp, maps, grid, ws->device, st);
+    if (cap) return launch_types<true, false>(pair_q, fine_cap, pp, maps, grid, ws->device, st);
+    if (bias) return launch_types<false, true>(pair_q, fine_cap, pp, maps, grid, ws->device, st);
+    return launch_types<false, false>(pair_q, fine_cap, pp, maps, grid, ws->device, st);
 }
 
 }  // extern "C"

@@ -71,7 +71,7 @@ void launch_rope(RopeParams& p, bool interleaved, bool vec, int sms, cudaStream_
 
 // Checks the rows, fills what every mode shares and launches.
 template <int MODE>
-int run_rope(RopeParams& p, const uocr_b200_rope* rope, const uocr_b200_qkv_rows* rows, int kv_dtype, cudaStream_t st, const char* who) {
+int run_rope(RopeParams& p, const uocr_b200_rope* rope, const uocr_b200_qkv_rows* rows, int kv_dtype, const uocr_b200_workspace* ws, cudaStream_t st, const char* who) {
     auto bad = [&](const char* what) { return fail(UOCR_B200_ERR_INVALID, std::string(who) + ": " + what); };
     if (!rope || !rows || !p.d_positions) return bad("null pointer");
     if (rows->dtype != UOCR_B200_F32 && rows->dtype != UOCR_B200_BF16) return fail(UOCR_B200_ERR_UNSUPPORTED, std::string(who) + ": rows must be fp32 or bf16");
@@ -86,6 +86,8 @@ int run_rope(RopeParams& p, const uocr_b200_rope* rope, const uocr_b200_qkv_rows
     if (MODE == kRopeRows && p.kv_heads > 0 && rows->k == p.k_out && rows->k_stride != p.k_out_stride) return bad("in place, the strides must be equal");
     const DeviceInfo* di = nullptr;
     if (int rc = device_info(&di)) return rc;
+    if (int rc = check_workspace_device(ws, who)) return rc;
+    p.status = ws ? ws->status : nullptr;
 
     for (int i = 0; i < kRopeMaxPairs; ++i) p.turn[i] = rope->turn[i];
     p.amplitude = rope->amplitude;
@@ -175,7 +177,7 @@ int uocr_b200_rswa_rope_rows(const uocr_b200_rope* rope, const uocr_b200_qkv_row
     p.k_out = k_out;
     p.k_out_stride = k_out_stride;
     p.d_positions = d_positions;
-    return run_rope<kRopeRows>(p, rope, rows, UOCR_B200_F32, reinterpret_cast<cudaStream_t>(stream), "rope_rows");
+    return run_rope<kRopeRows>(p, rope, rows, UOCR_B200_F32, nullptr, reinterpret_cast<cudaStream_t>(stream), "rope_rows");
 }
 
 int uocr_b200_rswa_rope_write_prefill_paged(const uocr_b200_paged_kv* kv, const uocr_b200_rope* rope, const uocr_b200_qkv_rows* rows,
@@ -191,8 +193,7 @@ int uocr_b200_rswa_rope_write_prefill_paged(const uocr_b200_paged_kv* kv, const 
     p.d_positions = d_positions;
     p.d_slots = d_slots;
     p.d_pos = d_pos;
-    p.status = ws ? ws->status : nullptr;
-    return run_rope<kRopeWrite>(p, rope, rows, kv->dtype, reinterpret_cast<cudaStream_t>(stream), "rope_write_prefill_paged");
+    return run_rope<kRopeWrite>(p, rope, rows, kv->dtype, ws, reinterpret_cast<cudaStream_t>(stream), "rope_write_prefill_paged");
 }
 
 int uocr_b200_rswa_rope_append_decode_batch_paged(const uocr_b200_paged_kv* kv, const uocr_b200_rope* rope, const uocr_b200_qkv_rows* rows,
@@ -213,8 +214,7 @@ int uocr_b200_rswa_rope_append_decode_batch_paged(const uocr_b200_paged_kv* kv, 
     p.d_ring_pos = d_ring_pos;
     p.d_prefill_len = d_prefill_len;
     p.window = window;
-    p.status = ws ? ws->status : nullptr;
-    return run_rope<kRopeAppend>(p, rope, rows, kv->dtype, reinterpret_cast<cudaStream_t>(stream), "rope_append_decode_batch_paged");
+    return run_rope<kRopeAppend>(p, rope, rows, kv->dtype, ws, reinterpret_cast<cudaStream_t>(stream), "rope_append_decode_batch_paged");
 }
 
 }  // extern "C"

@@ -91,9 +91,7 @@ int run_scored(const uocr_b200_paged_kv* kv, const uocr_b200_score* score, const
     }
     const DeviceInfo* di = nullptr;
     if (int rc = device_info(&di)) return rc;
-    int dev = 0;
-    CHECK_CUDA(cudaGetDevice(&dev), "cudaGetDevice");
-    if (dev != ws->device) return bad("the workspace belongs to another device");
+    if (int rc = check_workspace_device(ws, who)) return rc;
 
     const int group = heads / kv->kv_heads;
     int g = group % 4 == 0 ? 4 : group % 2 == 0 ? 2 : 1;

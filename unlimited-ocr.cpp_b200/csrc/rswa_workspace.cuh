@@ -125,3 +125,14 @@ struct uocr_b200_workspace {
     bool overlap = false;  // fused decode step may start its prologue before the preceding kernel ends
     cudaEvent_t ev0 = nullptr, ev1 = nullptr;
 };
+
+namespace uocr_b200 {
+
+// A workspace (null: none) serves the device that it was made on; kernels of another one must not get its memory.
+inline int check_workspace_device(const uocr_b200_workspace* ws, const char* who) {
+    int dev = 0;
+    CHECK_CUDA(cudaGetDevice(&dev), "cudaGetDevice");
+    return ws && ws->device != dev ? fail(UOCR_B200_ERR_INVALID, std::string(who) + ": the workspace belongs to another device") : UOCR_B200_OK;
+}
+
+}  // namespace uocr_b200
