@@ -14,6 +14,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 import subprocess
 
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -82,6 +83,13 @@ class Error(RuntimeError):
         self.status = status
 
 
+class ArgumentError(Error, ValueError):
+    """Tensors a call would misread (type, layout, size, device): the library gets bare addresses, so they are refused before it is called."""
+
+    def __init__(self, msg):
+        super().__init__(1, msg)
+
+
 _LIB = None
 
 _vp, _i, _i64 = C.c_void_p, C.c_int, C.c_int64
@@ -141,9 +149,9 @@ _SIGS = {
     "uocr_b200_rswa_evict_publish": (_i, [_vp, _i, _vp, _i, _vp, _i, _vp, _vp, _i, _vp, C.c_longlong, _i, _vp, _i, _vp, _i, _vp, _i, _vp, _vp]),
     "uocr_b200_rope_create": (_i, [C.POINTER(RopeDesc), C.POINTER(_vp)]),
     "uocr_b200_rope_destroy": (_i, [_vp]),
-    "uocr_b200_rswa_rope_rows": (_i, [_vp, C.POINTER(QkvRows), _vp, _i64, _vp, _i, _i, _i, _vp]),
-    "uocr_b200_rswa_rope_write_prefill_paged": (_i, [C.POINTER(PagedKV), _vp, C.POINTER(QkvRows)] + [_vp] * 3 + [_i, _vp, _vp]),
-    "uocr_b200_rswa_rope_append_decode_batch_paged": (_i, [C.POINTER(PagedKV), _vp, C.POINTER(QkvRows)] + [_vp] * 5 + [_i, _i, _vp, _vp]),
+    "uocr_b200_rswa_rope_rows": (_i, [_vp, _vp, _vp, _i64, _vp, _i, _i, _i, _vp]),
+    "uocr_b200_rswa_rope_write_prefill_paged": (_i, [C.POINTER(PagedKV), _vp, _vp] + [_vp] * 3 + [_i, _vp, _vp]),
+    "uocr_b200_rswa_rope_append_decode_batch_paged": (_i, [C.POINTER(PagedKV), _vp, _vp] + [_vp] * 5 + [_i, _i, _vp, _vp]),
 }
 
 
@@ -209,14 +217,14 @@ def _p(t):
 _current_raw_stream = None  # torch's raw handle of a device's current stream, without building a Stream object
 
 
-def stream_handle(stream=None):
+def stream_handle(stream=None, device=None):
     if stream is not None:
         return stream.cuda_stream
     global _current_raw_stream
-    import torch
     if _current_raw_stream is None:
+        import torch
         _current_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda d: torch.cuda.current_stream(d).cuda_stream)
-    return _current_raw_stream(torch.cuda.current_device())
+    return _current_raw_stream(_current_device() if device is None else device)
 
 
 class Workspace:
@@ -224,6 +232,8 @@ class Workspace:
         h = _vp()
         check(lib().uocr_b200_workspace_create(max_rows, C.byref(h)))
         self.h = h
+        self.out_dtype = F32
+        self.plan_rows = None  # packed rows of the tile plan with modified scores
 
     def status(self, stream=None) -> int:
         v = _i(0)
@@ -236,6 +246,7 @@ class Workspace:
     def set_out_dtype(self, dtype: int) -> None:
         """F32 (default) or BF16: type of the `out` tensor of every attention call using this workspace."""
         check(lib().uocr_b200_workspace_set_out_dtype(self.h, dtype))
+        self.out_dtype = dtype
 
     def set_overlap(self, enabled: bool) -> None:
         check(lib().uocr_b200_workspace_set_overlap(self.h, 1 if enabled else 0))
@@ -521,12 +532,22 @@ class Rope:
             pass
 
 
-def _stream_of(t, stream):
-    """The stream of a call on t's device, which has to be the current one (launches go there)."""
+_I32 = _FLOAT = _HALF = None  # torch.int32, torch.float32, torch.bfloat16, once torch has been asked for
+_device_index = None
+
+
+def _current_device():
+    """Index of the current device: launches go there, so the tensors of a call must be there."""
+    if _device_index is None:
+        _load_torch()
+    return _device_index()
+
+
+def _load_torch():
+    global _I32, _FLOAT, _HALF, _device_index
     import torch
-    if t.get_device() != torch.cuda.current_device():
-        raise ValueError(f"tensors must be on the current device, got {t.device}")
-    return stream_handle(stream)
+    _I32, _FLOAT, _HALF = torch.int32, torch.float32, torch.bfloat16
+    _device_index = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
 def _dp(t):
@@ -535,62 +556,124 @@ def _dp(t):
 
 
 def _dtype_of(t):
-    import torch
     dt = t.dtype
-    if dt is torch.float32:
+    if dt is _FLOAT:
         return F32
-    if dt is torch.bfloat16:
+    if dt is _HALF:
         return BF16
-    raise ValueError(f"rows must be float32 or bfloat16, got {dt}")
+    raise ArgumentError(f"rows must be float32 or bfloat16, got {dt}")
 
 
-def _row_stride(t, dtype, n):
-    """Elements between the rows of t: an [n, width] matrix of the type with contiguous rows."""
-    step, one = t.stride()
-    if one != 1 or t.dtype is not dtype or t.size(0) != n:
-        raise ValueError("rows must have one type and count, and contiguous elements")
-    return step if n > 1 else max(step, t.size(1))
+def _refuse(t, dtype, n, dev, name):
+    """The error for a tensor that is not what `_array` or `_ints` wants."""
+    return ArgumentError(f"{name}: wanted at least {n} contiguous {dtype} on cuda:{dev}, got {t.numel()} {t.dtype} {'contiguous' if t.is_contiguous() else 'strided'} on {t.device}")
 
 
-def _qkv_rows(q, k, v, q_out, heads, n):
-    """Packed rows, [n, width] each with its own row stride."""
+def _array(t, dtype, n, dev, name):
+    """Address of a contiguous tensor of at least n elements of the type (None passes: the library says where it wants one)."""
+    if t is None:
+        return None
+    if t.dtype is not dtype or t.numel() < n or not t.is_contiguous() or t.get_device() != dev:
+        raise _refuse(t, dtype, n, dev, name)
+    return t.data_ptr()
+
+
+def _ints(t, n, dev, name):
+    if t is None:
+        return None
+    if t.dtype is not _I32 or t.numel() < n or not t.is_contiguous() or t.get_device() != dev:
+        raise _refuse(t, _I32, n, dev, name)
+    return t.data_ptr()
+
+
+def _slot_ints(t, dev, name):
+    """The same for one integer per slot, however many slots there are (an empty tensor has no address, which the library refuses)."""
+    if t is None:
+        return None
+    if t.dtype is not _I32 or not t.is_contiguous() or t.get_device() != dev:
+        raise _refuse(t, _I32, 1, dev, name)
+    return t.data_ptr()
+
+
+def _grid(t, dtype, rows, dev, name):
+    """(address, width) of a contiguous [at least `rows`][width] matrix of the type; (None, 0) for None."""
+    if t is None:
+        return None, 0
+    shape = t.shape
+    if len(shape) != 2 or shape[0] < rows:
+        raise ArgumentError(f"{name}: wanted a matrix of at least {rows} rows, got {tuple(shape)}")
+    if t.dtype is not dtype or not t.is_contiguous() or t.get_device() != dev:
+        raise _refuse(t, dtype, 0, dev, name)
+    return t.data_ptr(), shape[1]
+
+
+def _row_stride(t, dtype, n, width, dev):
+    """Elements between the rows of t: an [n, width or more] matrix of the type on the device with contiguous rows."""
+    shape, stride = t.shape, t.stride()
+    if len(shape) != 2 or shape[0] != n or shape[1] < width or stride[1] != 1 or t.dtype is not dtype or t.get_device() != dev:
+        raise ArgumentError(f"rows must be [{n}, at least {width}] {dtype} on cuda:{dev} with contiguous elements, got {tuple(shape)} {t.dtype} on {t.device}, strides {stride}")
+    return stride[0] if n > 1 else width
+
+
+_QKV_ROWS = struct.Struct("PPPPqqqqii")  # QkvRows (packing is a fifth of the time that filling a ctypes structure takes)
+
+
+def _addr(t):
+    return 0 if t is None else t.data_ptr()
+
+
+def _qkv_rows(q, k, v, q_out, heads, kv_heads, head_dim, n, dev):
+    """Packed rows, [n, width] each with its own row stride, as the bytes of a QkvRows; and the stride of k."""
     ref = q if q is not None else k
     dt = ref.dtype
+    q_width, kv_width = heads * head_dim, kv_heads * head_dim
     qs = ks = vs = os = 0
     if q is not None:
-        qs = _row_stride(q, dt, n)
+        qs = _row_stride(q, dt, n, q_width, dev)
         if q_out is not None:
-            os = qs if q_out is q else _row_stride(q_out, dt, n)
+            os = qs if q_out is q else _row_stride(q_out, dt, n, q_width, dev)
     if k is not None:
-        ks = _row_stride(k, dt, n)
+        ks = _row_stride(k, dt, n, kv_width, dev)
         if v is not None:
-            vs = _row_stride(v, dt, n)
-    return QkvRows(_dp(q), _dp(k), _dp(v), _dp(q_out), qs, ks, vs, os, _dtype_of(ref), heads)
+            vs = _row_stride(v, dt, n, kv_width, dev)
+    return _QKV_ROWS.pack(_addr(q), _addr(k), _addr(v), _addr(q_out), qs, ks, vs, os, _dtype_of(ref), heads), ks
 
 
 def rope_rows(rope, q, k, q_out, k_out, d_positions, heads, kv_heads, head_dim, stream=None):
     """Rotates the packed rows of q and k (either may be None with 0 heads; outputs may be the inputs)."""
-    n = (q if q is not None else k).size(0)
-    rows = _qkv_rows(q, k, None, q_out, heads, n)
-    check(lib().uocr_b200_rswa_rope_rows(rope.h, rows, _dp(k_out), _row_stride(k_out, k.dtype, n) if k_out is not None else 0, d_positions.data_ptr(),
-                                         n, kv_heads, head_dim, _stream_of(d_positions, stream)))
+    n, dev = (q if q is not None else k).shape[0], _current_device()
+    rows, k_stride = _qkv_rows(q, k, None, q_out, heads, kv_heads, head_dim, n, dev)
+    if k_out is not None and k_out is not k:
+        k_stride = _row_stride(k_out, (k if k is not None else k_out).dtype, n, kv_heads * head_dim, dev)
+    check(lib().uocr_b200_rswa_rope_rows(rope.h, rows, _dp(k_out), k_stride, _ints(d_positions, n, dev, "d_positions"), n, kv_heads, head_dim,
+                                         stream_handle(stream, dev)))
+
+
+def _kv_rows(layer, q, k, v, q_out, heads, dev):
+    """The rows of a call that writes K and V to the layer, and their count."""
+    d, n = layer.desc, k.shape[0]
+    if layer.k.get_device() != dev:
+        raise ArgumentError(f"the layer is on {layer.k.device}, the current device is cuda:{dev}")
+    return _qkv_rows(q, k, v, q_out, heads, d.kv_heads, d.head_dim, n, dev)[0], n
 
 
 def rope_write_prefill_paged(layer, rope, q, k, v, q_out, d_positions, d_slots, d_pos, heads, ws=None, stream=None):
     """rope + write_prefill_ragged_paged in one pass."""
-    n = k.size(0)
+    dev = _current_device()
+    rows, n = _kv_rows(layer, q, k, v, q_out, heads, dev)
     check(lib().uocr_b200_rswa_rope_write_prefill_paged(
-        layer.desc, rope.h, _qkv_rows(q, k, v, q_out, heads, n), d_positions.data_ptr(), d_slots.data_ptr(), d_pos.data_ptr(), n,
-        ws.h if ws else None, _stream_of(k, stream)))
+        layer.desc, rope.h, rows, _ints(d_positions, n, dev, "d_positions"), _ints(d_slots, n, dev, "d_slots"), _ints(d_pos, n, dev, "d_pos"), n,
+        ws.h if ws else None, stream_handle(stream, dev)))
 
 
 def rope_append_decode_batch_paged(layer, rope, q, k, v, q_out, d_positions, d_len, d_ring, d_prefill, d_slots, window, heads, ws=None,
                                    stream=None):
     """rope + append_decode_batch_paged in one pass."""
-    n = k.size(0)
+    dev = _current_device()
+    rows, n = _kv_rows(layer, q, k, v, q_out, heads, dev)
     check(lib().uocr_b200_rswa_rope_append_decode_batch_paged(
-        layer.desc, rope.h, _qkv_rows(q, k, v, q_out, heads, n), d_positions.data_ptr(), d_len.data_ptr(), d_ring.data_ptr(), d_prefill.data_ptr(),
-        d_slots.data_ptr(), n, window, ws.h if ws else None, _stream_of(k, stream)))
+        layer.desc, rope.h, rows, _ints(d_positions, n, dev, "d_positions"), _slot_ints(d_len, dev, "d_len"), _slot_ints(d_ring, dev, "d_ring"),
+        _slot_ints(d_prefill, dev, "d_prefill"), _ints(d_slots, n, dev, "d_slots"), n, window, ws.h if ws else None, stream_handle(stream, dev)))
 
 
 # ---- attention with modified scores --------------------------------------------------------------------
@@ -602,10 +685,22 @@ class Score:
         import torch
         for t, dt in ((slopes, torch.float32), (d_q_pos, torch.int32), (d_key_pos, torch.int32), (d_lo, torch.int32), (d_hi, torch.int32)):
             if t is not None and (t.dtype != dt or not t.is_contiguous()):
-                raise ValueError(f"expected a contiguous {dt} tensor")
+                raise ArgumentError(f"expected a contiguous {dt} tensor")
         self.keep = (slopes, d_q_pos, d_key_pos, d_lo, d_hi)
         self.desc = ScoreDesc(scale, softcap, _p(slopes), _p(d_q_pos), _p(d_key_pos), d_key_pos.shape[1] if d_key_pos is not None else 0,
                               _p(d_lo), _p(d_hi))
+        # what a call may read: rows and heads its tensors reach (None: no limit), and their device
+        self.rows = min((t.numel() for t in (d_q_pos if slopes is not None else None, d_lo, d_hi) if t is not None), default=None)
+        self.heads = slopes.numel() if slopes is not None else None
+        self.device = _one_device(self.keep)
+
+
+def _one_device(tensors):
+    """Index of the device all of them are on; None for none."""
+    found = {t.get_device() for t in tensors if t is not None}
+    if len(found) > 1:
+        raise ArgumentError("the tensors are on different devices")
+    return found.pop() if found else None
 
 
 class Mass:
@@ -615,72 +710,133 @@ class Mass:
         import torch
         for t in (mass_in, mass_out):
             if t is not None and (t.dtype != torch.float32 or not t.is_contiguous() or t.shape != mass_out.shape):
-                raise ValueError("the mass must be contiguous float32, [slots, stride]")
+                raise ArgumentError("the mass must be contiguous float32, [slots, stride]")
         stride = mass_out.shape[1]
         n = lib().uocr_b200_rswa_mass_scratch_bytes(batch, heads, stride)
         self.scratch = torch.empty(n, dtype=torch.uint8, device=mass_out.device)
         self.keep = (mass_in, mass_out)
         self.desc = MassDesc(_p(mass_in), _p(mass_out), stride, decay, _p(self.scratch), n)
+        self.device = _one_device(self.keep)
+
+
+def _scored(layer, score, q, rows, heads, out, ws, dev):
+    """Addresses of q and out and q's type, for a call of `rows` rows."""
+    if (score.rows is not None and rows > score.rows) or (score.heads is not None and heads > score.heads):
+        raise ArgumentError(f"the score's tensors are for {score.rows} rows and {score.heads} heads, the call has {rows} and {heads}")
+    if (score.device is not None and score.device != dev) or layer.k.get_device() != dev:
+        raise ArgumentError(f"score and layer must be on the current device, cuda:{dev}")
+    dt, n = _dtype_of(q), rows * heads * layer.desc.head_dim
+    return _array(q, q.dtype, n, dev, "q"), dt, _array(out, _HALF if ws.out_dtype == BF16 else _FLOAT, n, dev, "out")
 
 
 def attention_scored_batch_paged(layer, score, q, d_len, d_ring, d_prefill, d_slots, batch, window, heads, out, ws, mass=None, stream=None):
     """Decode attention with modified scores; `mass` also accumulates the attention weights."""
+    dev = _current_device()
+    q, dt, out = _scored(layer, score, q, batch, heads, out, ws, dev)
+    if mass is not None and mass.device != dev:
+        raise ArgumentError(f"the mass must be on the current device, cuda:{dev}")
     check(lib().uocr_b200_rswa_attention_scored_batch_paged(
-        layer.desc, score.desc, _dp(q), _dtype_of(q), _dp(d_len), _dp(d_ring), _dp(d_prefill), _dp(d_slots), batch, window, heads,
-        _dp(out), C.addressof(mass.desc) if mass is not None else None, ws.h, _stream_of(q, stream)))
+        layer.desc, score.desc, q, dt, _slot_ints(d_len, dev, "d_len"), _slot_ints(d_ring, dev, "d_ring"), _slot_ints(d_prefill, dev, "d_prefill"),
+        _ints(d_slots, batch, dev, "d_slots"), batch, window, heads, out, C.addressof(mass.desc) if mass is not None else None, ws.h, stream_handle(stream, dev)))
 
 
 def attention_scored_ragged_paged(layer, score, q, d_prefill, d_slots, d_pos, total, heads, out, ws, stream=None):
     """Packed vision rows with modified scores, any geometry."""
-    check(lib().uocr_b200_rswa_attention_scored_ragged_paged(layer.desc, score.desc, _dp(q), _dtype_of(q), _dp(d_prefill), _dp(d_slots),
-                                                             _dp(d_pos), total, heads, _dp(out), ws.h, _stream_of(q, stream)))
+    dev = _current_device()
+    q, dt, out = _scored(layer, score, q, total, heads, out, ws, dev)
+    check(lib().uocr_b200_rswa_attention_scored_ragged_paged(
+        layer.desc, score.desc, q, dt, _slot_ints(d_prefill, dev, "d_prefill"), _ints(d_slots, total, dev, "d_slots"), _ints(d_pos, total, dev, "d_pos"), total,
+        heads, out, ws.h, stream_handle(stream, dev)))
+
+
+def _text_pools(layer, text_k, text_v, text_blocks, dev):
+    n = max(text_blocks, 0) * layer.desc.kv_heads * BLOCK_TOKENS * layer.desc.head_dim
+    return _array(text_k, layer.k.dtype, n, dev, "text_k"), _array(text_v, layer.k.dtype, n, dev, "text_v")
 
 
 def prefill_text_scored_paged(layer, text_k, text_v, text_blocks, score, q, d_prefill, d_slots, d_pos, d_block0, total, window, heads, out, ws,
                               stream=None):
     """Packed text rows over prefix + text window with modified scores, any geometry (K and V already in the text pool)."""
-    check(lib().uocr_b200_rswa_prefill_text_scored_paged(layer.desc, _dp(text_k), _dp(text_v), text_blocks, score.desc, _dp(q),
-                                                         _dtype_of(q), _dp(d_prefill), _dp(d_slots), _dp(d_pos), _dp(d_block0), total, window,
-                                                         heads, _dp(out), ws.h, _stream_of(q, stream)))
+    dev = _current_device()
+    q, dt, out = _scored(layer, score, q, total, heads, out, ws, dev)
+    text_k, text_v = _text_pools(layer, text_k, text_v, text_blocks, dev)
+    check(lib().uocr_b200_rswa_prefill_text_scored_paged(
+        layer.desc, text_k, text_v, text_blocks, score.desc, q, dt, _slot_ints(d_prefill, dev, "d_prefill"), _ints(d_slots, total, dev, "d_slots"),
+        _ints(d_pos, total, dev, "d_pos"), _ints(d_block0, total, dev, "d_block0"), total, window, heads, out, ws.h, stream_handle(stream, dev)))
+
+
+def _tiles(tiles):
+    """The query tiles as the library takes them, and the packed rows they reach."""
+    import numpy as np
+    t = np.ascontiguousarray(tiles, dtype=np.int32)
+    if t.ndim != 2 or t.shape[1] != 6:
+        raise ArgumentError(f"tiles must be [n, 6], got {t.shape}")
+    return t, int((t[:, 0].astype(np.int64) + t[:, 1]).max(initial=0))
 
 
 def prefill_plan_scored_tc(score, tiles, d_prefill, window, ws, stream=None):
     """Uploads and orders the query tiles for the score's visible ranges; later calls with reuse_plan=True share the plan."""
-    import numpy as np
-    t = np.ascontiguousarray(tiles, dtype=np.int32)
-    check(lib().uocr_b200_rswa_prefill_plan_scored_tc(score.desc, t.ctypes.data, t.shape[0], _dp(d_prefill), window, ws.h, _stream_of(d_prefill, stream)))
+    dev = _current_device()
+    t, rows = _tiles(tiles)
+    if (score.rows is not None and rows > score.rows) or (score.device is not None and score.device != dev):
+        raise ArgumentError(f"the score's tensors are for {score.rows} rows on device {score.device}, the tiles reach {rows} on cuda:{dev}")
+    check(lib().uocr_b200_rswa_prefill_plan_scored_tc(score.desc, t.ctypes.data, t.shape[0], _slot_ints(d_prefill, dev, "d_prefill"), window, ws.h,
+                                                      stream_handle(stream, dev)))
+    ws.plan_rows = rows
 
 
 def prefill_attention_scored_tc(layer, text_k, text_v, text_blocks, score, q, d_prefill, tiles, window, heads, out, ws, stream=None, reuse_plan=False):
     """prefill_attention_tc with modified scores; q fp32 or bf16."""
-    import numpy as np
-    t = np.ascontiguousarray(tiles, dtype=np.int32)
+    dev = _current_device()
+    t, rows = (tiles, ws.plan_rows) if reuse_plan and ws.plan_rows is not None else _tiles(tiles)  # the rows of a reused plan are the plan's
+    q, dt, out = _scored(layer, score, q, rows, heads, out, ws, dev)
+    text_k, text_v = _text_pools(layer, text_k, text_v, text_blocks, dev)
     check(lib().uocr_b200_rswa_prefill_attention_scored_tc(
-        layer.desc, _dp(text_k), _dp(text_v), text_blocks, score.desc, _dp(q), _dtype_of(q), _dp(d_prefill),
-        None if reuse_plan else t.ctypes.data, t.shape[0], window, heads, _dp(out), ws.h, _stream_of(q, stream)))
+        layer.desc, text_k, text_v, text_blocks, score.desc, q, dt, _slot_ints(d_prefill, dev, "d_prefill"), None if reuse_plan else t.ctypes.data, len(t),
+        window, heads, out, ws.h, stream_handle(stream, dev)))
+    if not reuse_plan:
+        ws.plan_rows = rows
 
 
 # ---- eviction from the fixed region ----------------------------------------------------------------------
 
 def evict_select(mass, d_prefill, d_slots, n, keep, sinks, recent, d_keep, d_keep_len, ws=None, stream=None):
     """The `keep` heaviest tokens of each slot's fixed region, ascending: d_keep int32 [n, keep], d_keep_len int32 [n]."""
-    check(lib().uocr_b200_rswa_evict_select(_dp(mass), mass.size(1), _dp(d_prefill), _dp(d_slots), n, keep, sinks, recent, _dp(d_keep),
-                                            _dp(d_keep_len), ws.h if ws else None, _stream_of(mass, stream)))
+    dev = _current_device()
+    mass, stride = _grid(mass, _FLOAT, 1, dev, "mass")
+    check(lib().uocr_b200_rswa_evict_select(
+        mass, stride, _slot_ints(d_prefill, dev, "d_prefill"), _ints(d_slots, n, dev, "d_slots"), n, keep, sinks, recent,
+        _ints(d_keep, n * keep, dev, "d_keep"), _ints(d_keep_len, n, dev, "d_keep_len"), ws.h if ws else None, stream_handle(stream, dev)))
 
 
 def evict_compact_paged_layers(layers, d_prefill, d_slots, n, d_keep, d_keep_len, d_new_blocks=None, ws=None, stream=None):
     """Moves the kept rows of every layer to the new blocks (None: in place).  layers: PagedLayers, or their layer_array."""
-    arr = layers if isinstance(layers, C.Array) else layer_array(layers)
+    dev = _current_device()
+    if isinstance(layers, C.Array):
+        arr = layers
+    else:
+        arr = layer_array(layers)
+        if any(lay.k.get_device() != dev for lay in layers):
+            raise ArgumentError(f"the layers must be on the current device, cuda:{dev}")
+    keep, width = _grid(d_keep, _I32, n, dev, "d_keep")
+    new, new_width = _grid(d_new_blocks, _I32, n, dev, "d_new_blocks")
     check(lib().uocr_b200_rswa_evict_compact_paged_layers(
-        arr, len(arr), _dp(d_prefill), _dp(d_slots), n, _dp(d_keep), d_keep.size(1), _dp(d_keep_len), _dp(d_new_blocks),
-        d_new_blocks.shape[1] if d_new_blocks is not None else 0, ws.h if ws else None, _stream_of(d_keep, stream)))
+        arr, len(arr), _slot_ints(d_prefill, dev, "d_prefill"), _ints(d_slots, n, dev, "d_slots"), n, keep, width, _ints(d_keep_len, n, dev, "d_keep_len"), new,
+        new_width, ws.h if ws else None, stream_handle(stream, dev)))
 
 
 def evict_publish(table, d_slots, n, d_keep, d_keep_len, d_len, d_prefill, window, d_new_blocks=None, mass=None, d_key_pos=None, ws=None,
                   stream=None):
     """Puts the new regions in force: table rows, d_len [layers, slots], d_prefill, and the per-token arrays."""
-    width = lambda t: t.shape[1] if t is not None else 0
+    dev = _current_device()
+    table, table_width = _grid(table, _I32, 1, dev, "table")
+    keep, width = _grid(d_keep, _I32, n, dev, "d_keep")
+    new, new_width = _grid(d_new_blocks, _I32, n, dev, "d_new_blocks")
+    mass, mass_width = _grid(mass, _FLOAT, 1, dev, "mass")
+    key_pos, pos_width = _grid(d_key_pos, _I32, 1, dev, "d_key_pos")
+    if d_len.dim() != 2 or (d_len.size(1) > 1 and d_len.stride(1) != 1) or d_len.dtype is not _I32 or d_len.get_device() != dev:
+        raise ArgumentError(f"d_len must be [layers, slots] int32 on cuda:{dev} with contiguous rows, got {tuple(d_len.shape)} {d_len.dtype} on {d_len.device}")
     check(lib().uocr_b200_rswa_evict_publish(
-        _dp(table), table.shape[1], _dp(d_slots), n, _dp(d_keep), d_keep.size(1), _dp(d_keep_len), _dp(d_new_blocks), width(d_new_blocks), _dp(d_len),
-        d_len.stride(0), d_len.shape[0], _dp(d_prefill), window, _dp(mass), width(mass), _dp(d_key_pos), width(d_key_pos),
-        ws.h if ws else None, _stream_of(table, stream)))
+        table, table_width, _ints(d_slots, n, dev, "d_slots"), n, keep, width, _ints(d_keep_len, n, dev, "d_keep_len"), new, new_width, d_len.data_ptr(),
+        d_len.stride(0), d_len.size(0), _slot_ints(d_prefill, dev, "d_prefill"), window, mass, mass_width, key_pos, pos_width, ws.h if ws else None,
+        stream_handle(stream, dev)))
