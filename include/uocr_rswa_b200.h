@@ -428,8 +428,9 @@ UOCR_B200_API int uocr_b200_rswa_gather_heads_paged(
  * The reference rotates whole heads in the half layout without scaling (src/kernels/cuda/rope_fused.cu:
  * 12-40), which uocr_b200_rswa_decode_step_rope_paged folds into the fused step with that kernel's own
  * fp32 angles.  The calls below turn pair i of every head by angle = d_positions[row] * freq_i and
- * scale it by `amplitude`: (x0, x1) -> amplitude * (x0 cos - x1 sin, x0 sin + x1 cos).  Angles are exact
- * to 2^-33 turns for every 32-bit position (the fused step's fp32 angles are off by up to
+ * scale it by `amplitude`: (x0, x1) -> amplitude * (x0 cos - x1 sin, x0 sin + x1 cos).  Angles are
+ * exact to 2^-32 turns for every 32-bit position (frequencies above 1: times the frequency) until they are
+ * reduced to an eighth of a turn in fp32, 2^-28 turns (the fused step's fp32 angles are off by up to
  * position * 2^-24 radians); the rotation is done in fp32 and rounded once.
  *   layout HALF: pair i is (i, i + rotary_dim/2); INTERLEAVED: (2i, 2i + 1).  Dims at and beyond
  *     rotary_dim are copied.
@@ -576,7 +577,8 @@ UOCR_B200_API int uocr_b200_rswa_prefill_text_scored_paged(
  * the span of keys that the rows of a query tile see -- from the first to the last -- may hold anything; inside it
  * they must be finite, since the rows that do not see a key multiply its value by zero. A query row that holds a NaN or an
  * infinity gives NaN (0 if it sees no key).  Not supported
- * (UNSUPPORTED): d_key_pos, keys stand at their own index; a softcap above 256, the tanh is off by 2^-21 of the cap. */
+ * (UNSUPPORTED): d_key_pos, keys stand at their own index; a softcap above 256, the tanh is off by 2^-20 of the cap
+ * (2^-19 for bf16 results) at most. */
 UOCR_B200_API int uocr_b200_rswa_prefill_attention_scored_tc(
     const uocr_b200_paged_kv* kv, const void* text_k_pool, const void* text_v_pool, int text_blocks,
     const uocr_b200_score* score, const void* q, int q_dtype, const int* d_prefill_len,

@@ -29,7 +29,7 @@ int launch_types(bool pair_q, bool fine_cap, const PrefillParams& pp, const Pref
 // What this call takes of the modified scores.
 int check_tc_score(const uocr_b200_score* score, const char* who) {
     if (int rc = check_score(score, kTcTile, who)) return rc;
-    // the kernel's tanh is off by 2^-21 of the cap: a cap far above the scores would drown them
+    // the kernel's tanh is off by 2^-20 of the cap (2^-19 for bf16 results): a cap far above the scores would drown them
     if (score->softcap > 256.f) return fail(UOCR_B200_ERR_UNSUPPORTED, std::string(who) + ": softcap above 256 (use the calls for any geometry)");
     if (score->d_key_pos) return fail(UOCR_B200_ERR_UNSUPPORTED, std::string(who) + ": keys stand at their own index here (d_key_pos: use the calls for any geometry)");
     return UOCR_B200_OK;

@@ -285,7 +285,7 @@ __device__ __forceinline__ float2 tc_exp2_poly(float2 x) {
 // away what half-hidden tiles allow.)
 constexpr int kTcChunk = 32;
 
-// tanh(x) / x as a polynomial in x^2 of least maximum relative error (3.9e-9) for |x| <= kTcTanhSmall.
+// tanh(x) / x as a polynomial in x^2 of small maximum relative error for |x| <= kTcTanhSmall: 1.1e-8 with its coefficients in fp32.
 constexpr float kTcTanhSmall = 0.625f;
 __device__ __forceinline__ float2 tc_tanh_over_x(float2 t) {
     auto horner = [&](float2 acc, float c) { return __ffma2_rn(acc, t, make_float2(c, c)); };
@@ -295,12 +295,13 @@ __device__ __forceinline__ float2 tc_tanh_over_x(float2 t) {
 }
 
 // Scores of a chunk of keys modified in place, into the log2 domain.  With a cap, mul makes s the power 2x in e^2x, and
-// tanh(x) = 1 - 2 / (1 + e^2x), right at both ends and off by 2^-21 at most.  Special functions are the scarce resource (16 results
+// tanh(x) = 1 - 2 / (1 + e^2x), right at both ends and off by 2^-20 at most (2^-20.4 emulated with the worst ex2 and reciprocal; 2^-19
+// and 2^-19.3 where the power is the polynomial).  Special functions are the scarce resource (16 results
 // a cycle and SM), so four reciprocals are taken as one, of the product of the four denominators (e^2x is cut at 2^30, where the
 // tanh is 1 already: the product stays below 2^121), and with bf16 results half of the powers are a polynomial.  The cut also turns the
 // NaN of a key that the row does not see into a number, so it cannot reach the three others through the product; a NaN in the
-// query is reported by the helpers.  For fp32 results an error of 2^-21 of the cap is much beside scores far below it: a
-// row whose chunk stays below 5/8 of the cap takes a polynomial that is right to 2^-23 of each score.  (The choice is the row's own:
+// query is reported by the helpers.  For fp32 results an error of 2^-20 of the cap is much beside scores far below it: a
+// row whose chunk stays below 5/8 of the cap takes a polynomial that is right to 2^-22 of each score.  (The choice is the row's own:
 // its bits depend neither on its neighbours nor on hidden keys, whose scores are zero by then.)  With bf16 results the
 // polynomial would cost 8 us on pages with half-hidden chunks (75 for 67), and a hidden key's score stays in the product of
 // its four, where it can move the last bit of the others' fp32 scores.  d0: the query's position minus that of key 0.

@@ -5,8 +5,9 @@
 // amplitude.  Angles of far positions lose everything in fp32 (position 10^6 times freq 1 is only known to
 // 0.06 rad), so they are kept as 64-bit fixed-point fractions of a turn: freq_i / 2 pi is rounded once to
 // 2^-64 turns on the host and position * that, modulo 2^64, is the exact fraction of the product -- one
-// integer multiply, good to 2^-33 turns for any 32-bit position.  What is left after the quadrant is taken
-// off is at most an eighth of a turn and goes to sincospi in fp32.
+// integer multiply.  Rounded to 2^-32 turns that is good to 2^-33, and the frequency's own rounding adds up to 2^-34 at the last
+// 32-bit positions (frequencies above 1, of theta or factor below 1, add more in proportion).  What is left after the quadrant is
+// taken off is at most an eighth of a turn and goes to sincospi in fp32, whose own step of up to 2^-28 turns is the larger error.
 //
 // The kernel moves bytes (q, k, v in; q and the pool rows out) and is bound by HBM, which takes few instructions a chunk and
 // loads in flight with nothing to wait on.  A warp takes a row, or a share of its heads.  A lane keeps one 16-byte chunk position
