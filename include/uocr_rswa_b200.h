@@ -599,7 +599,9 @@ UOCR_B200_API int uocr_b200_rswa_prefill_plan_scored_tc(const uocr_b200_score* s
 /* For each of the n slots the `keep` tokens of its fixed region with the largest mass, as an ascending
  * list in d_keep[i][0 .. count), -1 up to `keep`; count = min(keep, region) goes to d_keep_len[i].  The first
  * `sinks` and the last `recent` tokens count as infinitely heavy; NaN counts as lighter than
- * everything; ties go to the lowest index.  A region longer than mass_stride sets status bit 4 and is
+ * everything; ties go to the lowest index.  So where keep < sinks + recent, or masses are infinite themselves, infinitely heavy
+ * tokens are kept from the front: the sinks, then the others in their order, and the newest tokens are the first to go.  A caller
+ * who wants all protected tokens kept asks for keep >= sinks + recent.  A region longer than mass_stride sets status bit 4 and is
  * treated as mass_stride tokens long.  `ws` may be null. */
 UOCR_B200_API int uocr_b200_rswa_evict_select(const float* mass, int mass_stride, const int* d_prefill_len, const int* d_slots, int n,
                                               int keep, int sinks, int recent, int* d_keep, int* d_keep_len,

@@ -801,7 +801,8 @@ def prefill_attention_scored_tc(layer, text_k, text_v, text_blocks, score, q, d_
 # ---- eviction from the fixed region ----------------------------------------------------------------------
 
 def evict_select(mass, d_prefill, d_slots, n, keep, sinks, recent, d_keep, d_keep_len, ws=None, stream=None):
-    """The `keep` heaviest tokens of each slot's fixed region, ascending: d_keep int32 [n, keep], d_keep_len int32 [n]."""
+    """The `keep` heaviest tokens of each slot's fixed region, ascending: d_keep int32 [n, keep], d_keep_len int32 [n].  Protected tokens
+    that do not all fit (keep < sinks + recent) are kept from the front."""
     dev = _current_device()
     mass, stride = _grid(mass, _FLOAT, 1, dev, "mass")
     check(lib().uocr_b200_rswa_evict_select(
