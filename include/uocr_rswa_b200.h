@@ -77,7 +77,7 @@ UOCR_B200_API int uocr_b200_workspace_status(uocr_b200_workspace* ws, uocr_b200_
                                              int* device_status);
 
 /* Measurement aid: when enabled, every attention call records a CUDA event pair around its
- * partial-attention kernel on the launching stream; last_kernel_ms synchronises on the second
+ * partial-attention kernel on the launching stream (the tensor-core prefill and the calls with modified scores record none); last_kernel_ms synchronises on the second
  * event and returns the elapsed time of the most recent call.  Keep it off inside graph capture. */
 UOCR_B200_API int uocr_b200_workspace_set_timing(uocr_b200_workspace* ws, int enabled);
 UOCR_B200_API int uocr_b200_workspace_last_kernel_ms(uocr_b200_workspace* ws, float* ms);
@@ -511,7 +511,10 @@ UOCR_B200_API int uocr_b200_rswa_rope_append_decode_batch_paged(
  * both directions, a document up to the row itself -- cut to the region; an empty range hides it.
  * Ring and text-window tokens are all visible, as in the plain calls.  Keys and values a row does not
  * see are never multiplied: they may hold anything, NaN included (the tensor-core call below states its
- * own rule).  Everything is computed in fp32; `out` is fp32 or bf16 as the workspace says.
+ * own rule).  Everything is computed in fp32; `out` is fp32 or bf16 as the workspace says.  What a row does see is taken as it is,
+ * NaN and infinities included, and a row whose scores are all -infinity is NaN, as 0/0 is.  One exception: where two or four query
+ * heads share a bf16 KV head of 64 or 128 dims the products take their operands in bf16 parts, and an infinity in a query, or
+ * in a key or value that the row sees, gives NaN.  None of these calls records the event pair of uocr_b200_workspace_set_timing.
  * ============================================================================================= */
 typedef struct {
     float scale;         /* 0: 1/sqrt(head_dim); 3 * scale / min(softcap, 1) must be finite in fp32    */

@@ -118,3 +118,23 @@ def test_decode_infinite_query_of_either_sign(b, heads, hd, pool, prefix, sign):
     b.attention_scored_batch_paged(c.layer, b.Score(), q, c.d_len, c.d_ring, c.d_prefill, ints(0, 0), 2, 16, heads, out, ws)
     assert ws.status() == 0
     assert torch.isnan(out[0, :hd]).all() and torch.isfinite(out[0, hd:]).all() and torch.isfinite(out[1]).all()
+
+
+@pytest.mark.parametrize("heads,hd,pool,parts", [(1, 64, "bf16", False), (3, 128, "bf16", False), (4, 64, "f32", False), (2, 64, "bf16", True), (2, 128, "bf16", True),
+                                                 (4, 128, "bf16", True), (8, 64, "bf16", True)])
+def test_visible_infinities(b, heads, hd, pool, parts):
+    """An infinite value that a row sees is infinite in its result, or NaN where the operands go in bf16 parts; one that it does not see leaves no trace."""
+    import torch
+    from score_fixture import Caches
+    c = Caches([(40, 5, 0)], 1, hd, b.BF16 if pool == "bf16" else b.F32, 16, seed=6)
+    c.layer.v[int(c.table_np[0, 1]), 0, 4, 9] = float("inf")  # token 20
+    ints = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")
+    q = torch.randn(2, heads * hd, device="cuda")
+    ws, out = b.Workspace(2), torch.zeros(2, heads, hd, device="cuda")
+    score = b.Score(d_lo=ints(0, 21))  # both in the same tile: row 1 sees from the next token on
+    b.attention_scored_batch_paged(c.layer, score, q, c.d_len, c.d_ring, c.d_prefill, ints(0, 0), 2, 16, heads, out.view(2, -1), ws)
+    assert ws.status() == 0
+    seen = out[0, :, 9]
+    assert (torch.isnan(seen) if parts else seen == float("inf")).all()
+    out[0, :, 9] = 0
+    assert torch.isfinite(out).all()
