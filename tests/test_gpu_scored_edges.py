@@ -120,7 +120,7 @@ def test_decode_infinite_query_of_either_sign(b, heads, hd, pool, prefix, sign):
     assert torch.isnan(out[0, :hd]).all() and torch.isfinite(out[0, hd:]).all() and torch.isfinite(out[1]).all()
 
 
-@pytest.mark.parametrize("heads,hd,pool,parts", [(1, 64, "bf16", False), (3, 128, "bf16", False), (4, 64, "f32", False), (2, 64, "bf16", True), (2, 128, "bf16", True),
+@pytest.mark.parametrize("heads,hd,pool,parts", [(1, 64, "bf16", False), (3, 128, "bf16", False), (4, 64, "f32", False), (2, 64, "bf16", False), (2, 128, "bf16", False),
                                                  (4, 128, "bf16", True), (8, 64, "bf16", True)])
 def test_visible_infinities(b, heads, hd, pool, parts):
     """An infinite value that a row sees is infinite in its result, or NaN where the operands go in bf16 parts; one that it does not see leaves no trace."""

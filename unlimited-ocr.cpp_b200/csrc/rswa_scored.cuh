@@ -9,8 +9,9 @@
 // sequence and a batch of many short ones load the SMs alike; a warp streams its piece's K and V tiles
 // through a private ring of shared memory with bulk copies, and the partial results (maximum, sum,
 // accumulator) of an item that straddles pieces are joined by the warps that finish last.  What differs:
-//   - an item is a row and up to four query heads of one KV head (G), so grouped heads read a tile once, and where it pays
-//     (bf16, head_dim 64 or 128) their products run on the tensor cores;
+//   - an item is a row and up to four query heads of one KV head (G): a group of two or four reads a tile once, one of eight twice
+//     (115 us where one of four takes 70), an odd one as often as it has heads; four heads of a bf16 cache of head_dim 64 or 128 run
+//     their products on the tensor cores;
 //   - only tiles that hold a visible token are on the line: the cost of a page is the page;
 //   - the line is planned by every CTA in its own shared memory when the rows fit (one launch), else by
 //     rswa_scored_plan_kernel;
@@ -449,14 +450,14 @@ struct ScoreFma {
 };
 
 // -------------------------------------------------------------------------------------------------
-// consumer on the tensor cores (mma.sync m16n8k16), for two or four query heads of a bf16 KV head: a product per head on the CUDA
+// consumer on the tensor cores (mma.sync m16n8k16), for four query heads of a bf16 KV head: a product per head on the CUDA
 // cores costs as many instructions as the memory leaves time for, and here the heads are columns that cost nothing.  fp32 operands
 // (queries, weights) go in as three bf16 whose sum is exact to 24 bits, as columns of their own:
 //   scores   S[16 tokens][8 columns] = K[16 x HD] Q^T: A is the tile's rows, lane (g, c) = (lane / 4, lane % 4) reads chunks
 //            c + 4 i of rows g and g + 8 -- the order of the dims is the same permutation for Q, so no element is moved;
 //   values   out^T[HD][8] = V^T[HD x 16 tokens] P: lane (g, c) reads chunk(s) g of tokens 2c, 2c + 1, 2c + 8, 2c + 9 and pairs
 //            the tokens' elements with byte permutes; P comes from the lanes that hold the scores by four shuffles.
-// Column n of a product is part n % (8 / G) of head n / (8 / G); with four heads the third parts are a second product into the same
+// Column n of a product is part n % 2 of head n / 2; the third parts are a second product into the same
 // accumulators (the columns of a head are summed in the end, whatever they hold).  Measured: 16 + 4 heads of 128 over six caches
 // of 24096 tokens (282 MB) 72 us, 155 us on the CUDA cores; bound by the instructions and latency of a tile's chain.  The
 // two-way (K) and four-way (V) bank conflicts of the unswizzled tiles are left: rows fetched one by one into padded slots have none,
@@ -478,11 +479,11 @@ __device__ __forceinline__ uint32_t split3(float a, float b, int part) {
     return part == 2 ? rn_bf16x2(ra - bf16_lo(mid), rb - bf16_hi(mid)) : 0u;
 }
 
-template <int HD, int G>
+template <int HD>
 struct ScoreMma {
-    static_assert((HD == 64 || HD == 128) && (G == 2 || G == 4), "what the fragments below are laid out for");
-    static constexpr int kGroup = G, kTile = kBlockTokens * HD * 2, kThreads = 384;  // 12 warps: 168 registers a thread
-    static constexpr int NT = G == 4 ? 2 : 1;   // products per K / V fragment
+    static_assert(HD == 64 || HD == 128, "what the fragments below are laid out for");
+    static constexpr int G = 4, kGroup = G, kTile = kBlockTokens * HD * 2, kThreads = 384;  // 12 warps: 168 registers a thread
+    static constexpr int NT = 2;                // products per K / V fragment
     static constexpr int CH = HD / 32;          // chunks of a K row per lane
     static constexpr int MT = HD / 16;          // 16-dim tiles of the accumulator
     static constexpr int VC = HD / 64;          // chunks of a V row per lane
@@ -497,13 +498,13 @@ struct ScoreMma {
     __device__ __forceinline__ void init(int lane) {
         g = lane >> 2;
         c = lane & 3;
-        head = G == 4 ? c : c >> 1;  // whose scores and accumulator columns (2c, 2c + 1) this lane holds
+        head = c;  // whose scores and accumulator columns (2c, 2c + 1) this lane holds
     }
     __device__ __forceinline__ int part_of(int column, int nt) const {
-        return G == 4 ? (nt == 0 ? column & 1 : (column & 1) ? 3 : 2) : column & 3;  // 3: nothing
+        return nt == 0 ? column & 1 : (column & 1) ? 3 : 2;  // 3: nothing
     }
     __device__ __forceinline__ void load(const ScoreParams& p, const ScoreItem& it) {
-        const int col_head = G == 4 ? g >> 1 : g >> 2;  // column g of the B operand
+        const int col_head = g >> 1;  // column g of the B operand
         const size_t at = ((size_t)it.index * G + col_head) * HD;
 #pragma unroll
         for (int i = 0; i < CH; ++i) {
@@ -554,14 +555,8 @@ struct ScoreMma {
                 mma_16816(s[2 * nt + 1], lo[i].z, hi[i].z, lo[i].w, hi[i].w, qf[nt][i].z, qf[nt][i].w);
             }
         float x0 = (s[0][0] + s[1][0]) + (s[0][1] + s[1][1]), x1 = (s[0][2] + s[1][2]) + (s[0][3] + s[1][3]);
-        if constexpr (NT == 2) {
-            x0 += (s[2][0] + s[3][0]) + (s[2][1] + s[3][1]);
-            x1 += (s[2][2] + s[3][2]) + (s[2][3] + s[3][3]);
-        }
-        if constexpr (G == 2) {  // the third part is in the neighbour's columns
-            x0 += __shfl_xor_sync(0xffffffffu, x0, 1);
-            x1 += __shfl_xor_sync(0xffffffffu, x1, 1);
-        }
+        x0 += (s[2][0] + s[3][0]) + (s[2][1] + s[3][1]);
+        x1 += (s[2][2] + s[3][2]) + (s[2][3] + s[3][3]);
         const bool v0 = g >= nskip && g < nvalid, v1 = g + 8 >= nskip && g + 8 < nvalid;
         float d0 = 0.f, d1 = 0.f;
         if (p.slopes) {
@@ -570,7 +565,7 @@ struct ScoreMma {
         }
         x0 = score_modify(p, x0 * p.q_scale, slope, d0);
         x1 = score_modify(p, x1 * p.q_scale, slope, d1);
-        if (p.scores && (meta & kSuFixed) && (G == 4 || !(c & 1))) {
+        if (p.scores && (meta & kSuFixed)) {
             if (v0) score_record(p, (size_t)it.index * G + head, tok0 + g, x0);
             if (v1) score_record(p, (size_t)it.index * G + head, tok0 + g + 8, x1);
         }
@@ -596,7 +591,7 @@ struct ScoreMma {
     }
     __device__ __forceinline__ void values(const uint8_t* vtile, int nskip, int nvalid, int) {
         // weights of tokens 2c, 2c + 1, 2c + 8, 2c + 9 for column g
-        const int col_head = G == 4 ? g >> 1 : (g >> 2) * 2;
+        const int col_head = g >> 1;
         const float w0 = __shfl_sync(0xffffffffu, p0, 8 * c + col_head), w1 = __shfl_sync(0xffffffffu, p0, 8 * c + 4 + col_head);
         const float w2 = __shfl_sync(0xffffffffu, p1, 8 * c + col_head), w3 = __shfl_sync(0xffffffffu, p1, 8 * c + 4 + col_head);
         uint32_t b[NT][2];
@@ -648,10 +643,6 @@ struct ScoreMma {
         for (int m = 0; m < MT; ++m) {
             lo[m] = acc[m][0] + acc[m][1];
             hi[m] = acc[m][2] + acc[m][3];
-            if constexpr (G == 2) {
-                lo[m] += __shfl_xor_sync(0xffffffffu, lo[m], 1);
-                hi[m] += __shfl_xor_sync(0xffffffffu, hi[m], 1);
-            }
         }
         const size_t at = ((size_t)it.index * G + head) * HD;
         float* part = p.part_acc + (size_t)my_slot * (G * HD) + head * HD;
@@ -665,20 +656,15 @@ struct ScoreMma {
                 __stcg(reinterpret_cast<float4*>(part + chunk * 8 + 4), make_float4(f[4], f[5], f[6], f[7]));
             }
         };
+        float f[8];
         if constexpr (VC == 2) {
-            float f[8];
-            if (G == 4 || !(c & 1)) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) f[e] = lo[e];
-                put(g, f);
-            }
-            if (G == 4 || (c & 1)) {
+            for (int e = 0; e < 8; ++e) f[e] = lo[e];
+            put(g, f);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) f[e] = hi[e];
-                put(g + 8, f);
-            }
-        } else if (G == 4 || !(c & 1)) {
-            float f[8];
+            for (int e = 0; e < 8; ++e) f[e] = hi[e];
+            put(g + 8, f);
+        } else {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 f[e] = lo[e];
@@ -686,7 +672,7 @@ struct ScoreMma {
             }
             put(g, f);
         }
-        if (g == 0 && (G == 4 || !(c & 1))) {
+        if (g == 0) {
             if (!whole) __stcg(reinterpret_cast<float2*>(p.part_ml + (size_t)my_slot * (2 * G) + 2 * head), make_float2(m_run, lsum));
             else if (p.scores) *reinterpret_cast<float2*>(p.score_ml + 2 * ((size_t)it.index * G + head)) = make_float2(m_safe, inv);
         }

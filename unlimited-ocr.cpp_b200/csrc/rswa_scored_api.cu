@@ -28,15 +28,15 @@ int launch_scored(ScoreParams& p, const DeviceInfo& di, const uocr_b200_workspac
 
 template <typename KV, int HD>
 int dispatch_group(int g, ScoreParams& p, const DeviceInfo& di, const uocr_b200_workspace* ws, cudaStream_t st) {
-    // Grouped heads of a bf16 cache: the tensor cores (16 + 4 heads of 128 over 144 000 tokens: 155 us on the CUDA cores).
+    // Four heads of a bf16 cache go to the tensor cores: 24 sequences, 4 KV heads, 300 MB of cache take 70 us (head_dim 128) and 83 (64),
+    // 90 and 109 on the CUDA cores; 16 + 4 heads of 128 over 144 000 tokens with a bias 72 and 155.  Two heads do not fill the
+    // columns and stay on the CUDA cores: 66 and 71 us, on the tensor cores 70 and 87.
     if constexpr (KV::kBytes == 2 && (HD == 64 || HD == 128)) {
-        if (g == 4) return launch_scored<ScoreMma<HD, 4>, HD>(p, di, ws, st);
-        if (g == 2) return launch_scored<ScoreMma<HD, 2>, HD>(p, di, ws, st);
-    } else {
-        if constexpr (4 * HD <= kPartElems)
-            if (g == 4) return launch_scored<ScoreFma<KV, HD, 4>, HD>(p, di, ws, st);
-        if (g == 2) return launch_scored<ScoreFma<KV, HD, 2>, HD>(p, di, ws, st);
+        if (g == 4) return launch_scored<ScoreMma<HD>, HD>(p, di, ws, st);
+    } else if constexpr (4 * HD <= kPartElems) {
+        if (g == 4) return launch_scored<ScoreFma<KV, HD, 4>, HD>(p, di, ws, st);
     }
+    if (g == 2) return launch_scored<ScoreFma<KV, HD, 2>, HD>(p, di, ws, st);
     return launch_scored<ScoreFma<KV, HD, 1>, HD>(p, di, ws, st);
 }
 
@@ -94,6 +94,9 @@ int run_scored(const uocr_b200_paged_kv* kv, const uocr_b200_score* score, const
     if (int rc = check_workspace_device(ws, who)) return rc;
 
     const int group = heads / kv->kv_heads;
+    // Heads of a group that share a pass over its tiles: as many of 4, 2, 1 as divide the group and fit a partial.  (Also where the
+    // wider ones spill registers: 24 sequences, 300 MB of cache, a group of four by 4 / 2 / 1: fp32 x 128 86, 95, 169 us; fp32 x 64
+    // 68, 108, 183; fp32 x 32 82, 106, 156; bf16 x 32 160, 195, 297; bf16 x 16 252, 321, 519.)
     int g = group % 4 == 0 ? 4 : group % 2 == 0 ? 2 : 1;
     while (g > 1 && g * kv->head_dim > kPartElems) g /= 2;
 
