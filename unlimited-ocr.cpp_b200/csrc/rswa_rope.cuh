@@ -139,9 +139,11 @@ __device__ __forceinline__ void rope_append_place(const RopeParams& p, int row, 
 // ROW: type of the q / k / v rows, KV: of the pool (ROW again where nothing goes to the pool).  Every chunk of 8 elements is
 // 16-byte aligned and, in the half layout, lies in one half of the rotated dims.  Append: one row per CTA, 8 warps to a row.
 // CTAs of an SM: the half layout takes 3, whose registers let the loads of a batch stay in flight (against 4: 8192 bf16 rows of
-// 20 heads of 128 rotated in 18.5 us, not 21.1; 1537 fp32 rows of 16 + 4 heads of 64 written in 7.0, not 7.6; the one loss is
-// 8192 fp32 rows of 20 heads of 128, 35.5, not 33.6).  Interleaved, 3 would gain on small calls (1537 bf16 rows of 10 + 10
-// heads of 128 written in 6.7, not 7.4) and lose on large ones (8192 rows 30.4, not 28.1; 16384 rows 52.2, not 50.8): 4.
+// 20 heads of 128 rotated in 19.0 us, not 21.5; 16384 / 8192 / 1537 bf16 rows of 10 + 10 + 10 heads written in 60.5 / 34.8 / 8.2,
+// not 67.3 / 37.1 / 10.0, to an fp32 pool 77 for 88, although that one spills 100 bytes and the bf16 one 72; 1537 fp32 rows of 16 + 4
+// heads of 64 written in 6.9, not 7.6; the one loss is 8192 fp32 rows of 20 heads of 128 rotated, 35.6, not 33.4).  Interleaved, 3
+// would gain on small calls (1537 bf16 rows of 10 + 10 heads of 128 written in 6.7, not 7.4) and lose on large ones (8192 rows 30.4,
+// not 28.1; 16384 rows 52.2, not 50.8): 4.
 template <typename ROW, typename KV, int MODE, bool INTERLEAVED>
 __global__ void __launch_bounds__(kRopeThreads, INTERLEAVED ? 4 : 3) rswa_rope_kernel(const __grid_constant__ RopeParams p) {
     constexpr int W = ROW::kBytes / 2;               // 16-byte words of a chunk
