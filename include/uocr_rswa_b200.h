@@ -574,8 +574,9 @@ UOCR_B200_API int uocr_b200_rswa_prefill_text_scored_paged(
  * per packed row.  A plan (made by the plan call, or by the attention call when h_tiles is given) covers the
  * keys that some row of a tile sees and so belongs to the ranges it was made with: it is reused by calls whose d_lo,
  * d_hi and prefix lengths still hold the same values, and never by the call without modified scores.  Ranges that have become
- * narrower are right with it too; a row that sees a key which no row of its tile saw when the plan was made sets status bit 4,
- * and its result is void.  fp32
+ * narrower are right with it too, as long as K and V are finite in all of the plan's; a row that sees a key which no row of its tile
+ * saw when the plan was made, and a region that has become shorter than what the plan's rows saw, set status bit 4, and the result is
+ * void.  fp32
  * queries and the probabilities go through the tensor cores as bf16 pairs, bf16 queries are taken as they are.  K and V outside
  * the span of keys that the rows of a query tile see -- from the first to the last -- may hold anything; inside it
  * they must be finite, since the rows that do not see a key multiply its value by zero. A query row that holds a NaN or an

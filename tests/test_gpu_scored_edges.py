@@ -138,3 +138,18 @@ def test_visible_infinities(b, heads, hd, pool, parts):
     assert (torch.isnan(seen) if parts else seen == float("inf")).all()
     out[0, :, 9] = 0
     assert torch.isfinite(out).all()
+
+
+def test_plan_for_a_region_that_has_become_shorter_is_reported(b):
+    """Blocks behind the shorter region may hold anything by now, and the plan has them multiplied by zero."""
+    import torch
+    w = Wave(b, torch, [(300, 0, 200, 0), (300, 0, 60, 1)], 2, 2, seed=5)
+    ws, out = b.Workspace(64), torch.empty(w.total, 256, device="cuda")
+    hi = torch.full((w.total,), 50, dtype=torch.int32, device="cuda")
+    for score, lens, want in ((b.Score(), 299, b.STATUS_BAD_SLOT), (b.Score(), 100, b.STATUS_BAD_SLOT), (b.Score(d_hi=hi), 49, b.STATUS_BAD_SLOT),
+                              (b.Score(d_hi=hi), 50, 0), (b.Score(d_hi=hi), 200, 0)):
+        w.d_prefill.fill_(300)
+        b.prefill_plan_scored_tc(score, w.tiles, w.d_prefill, 16, ws)
+        w.d_prefill.fill_(lens)
+        b.prefill_attention_scored_tc(w.layer, *w.text, w.text_blocks, score, w.q, w.d_prefill, w.tiles, 16, 2, out, ws, reuse_plan=True)
+        assert ws.status() == want, (lens, want)

@@ -794,9 +794,11 @@ rswa_prefill_tc_kernel(const PrefillParams p, const __grid_constant__ PrefillMap
             if constexpr (Mode::kScored) {
                 if (live) {
                     // The plan fixed the keys that the tile's rows may see; ranges and prefix lengths are those of now.  A row that has
-                    // come to see others would lose them: it is reported.
-                    tc_row_range(p, t, r, max(__ldg(p.d_prefill_len + t.slot), 0), plo, phi);
-                    if (plo < phi && (plo < cur.fixed_lo || phi > cur.fixed_hi)) atomicOr(p.status, kStatusBadSlot);
+                    // come to see others would lose them, and a region that has become shorter than the plan's keys leaves whatever its
+                    // blocks hold now to be multiplied by zero: both are reported.
+                    const int pfx = max(__ldg(p.d_prefill_len + t.slot), 0);
+                    tc_row_range(p, t, r, pfx, plo, phi);
+                    if ((plo < phi && (plo < cur.fixed_lo || phi > cur.fixed_hi)) || cur.fixed_hi > pfx) atomicOr(p.status, kStatusBadSlot);
                 }
                 fixed_span = tc_span(live, plo, phi);
                 if (t.kind == 1) text_span = tc_span(live, tlo, thi);
