@@ -198,3 +198,20 @@ def test_one_row_in_place_from_two_views(b):
     m.rope_rows(b.rope, wide[1:2, :HD], None, wide[1, :HD][None], None, ints(1), 1, 0, HD, stream=b.stream)
     rows = m.QkvRows.from_buffer_copy(b.reached[0][1][1])
     assert rows.q == rows.q_out and rows.q_stride == rows.q_out_stride == HD
+
+
+def test_a_call_that_fails_after_planning(b, monkeypatch):
+    """The library may have made the new plan before it refused the call: what is reused next has to hold the rows of either."""
+    call(b, "prefill_plan_scored_tc")
+    many = b.m.make_prefill_tiles([(0, 2 * N, 0, 0, 0, 0)])
+    big = torch.zeros(2 * N, HEADS * HD)
+    fine = b.m.check
+    monkeypatch.setattr(b.m, "check", lambda status: (_ for _ in ()).throw(b.m.Error(1, "refused")))
+    for name, change in (("prefill_attention_scored_tc", dict(tiles=many, q=big, out=big, score=b.m.Score())), ("prefill_plan_scored_tc", dict(tiles=many, score=b.m.Score()))):
+        b.ws.plan_rows = N
+        with pytest.raises(b.m.Error):
+            call(b, name, **change)
+        with pytest.raises(ValueError):
+            call(b, "prefill_attention_scored_tc", reuse_plan=True)
+    monkeypatch.setattr(b.m, "check", fine)
+    call(b, "prefill_attention_scored_tc", reuse_plan=True, q=big, out=big, score=b.m.Score())

@@ -780,6 +780,7 @@ def prefill_plan_scored_tc(score, tiles, d_prefill, window, ws, stream=None):
     t, rows = _tiles(tiles)
     if (score.rows is not None and rows > score.rows) or (score.device is not None and score.device != dev):
         raise ArgumentError(f"the score's tensors are for {score.rows} rows on device {score.device}, the tiles reach {rows} on cuda:{dev}")
+    ws.plan_rows = max(rows, ws.plan_rows or 0)  # until the call has succeeded: the library may hold the old plan or the new one
     check(lib().uocr_b200_rswa_prefill_plan_scored_tc(score.desc, t.ctypes.data, t.shape[0], _slot_ints(d_prefill, dev, "d_prefill"), window, ws.h,
                                                       stream_handle(stream, dev)))
     ws.plan_rows = rows
@@ -791,6 +792,8 @@ def prefill_attention_scored_tc(layer, text_k, text_v, text_blocks, score, q, d_
     t, rows = (tiles, ws.plan_rows) if reuse_plan and ws.plan_rows is not None else _tiles(tiles)  # the rows of a reused plan are the plan's
     q, dt, out = _scored(layer, score, q, rows, heads, out, ws, dev)
     text_k, text_v = _text_pools(layer, text_k, text_v, text_blocks, dev)
+    if not reuse_plan:
+        ws.plan_rows = max(rows, ws.plan_rows or 0)
     check(lib().uocr_b200_rswa_prefill_attention_scored_tc(
         layer.desc, text_k, text_v, text_blocks, score.desc, q, dt, _slot_ints(d_prefill, dev, "d_prefill"), None if reuse_plan else t.ctypes.data, len(t),
         window, heads, out, ws.h, stream_handle(stream, dev)))
