@@ -511,7 +511,8 @@ UOCR_B200_API int uocr_b200_rswa_rope_append_decode_batch_paged(
  * both directions, a document up to the row itself -- cut to the region; an empty range hides it.
  * Ring and text-window tokens are all visible, as in the plain calls.  Keys and values a row does not
  * see are never multiplied: they may hold anything, NaN included (the tensor-core call below states its
- * own rule).  Everything is computed in fp32; `out` is fp32 or bf16 as the workspace says.  What a row does see is taken as it is,
+ * own rule).  Everything is computed in fp32 (a bias of b costs a score 2^-24 b, which
+ * matters where all that a row sees is far away); `out` is fp32 or bf16 as the workspace says.  What a row does see is taken as it is,
  * NaN and infinities included, and a row whose scores are all -infinity is NaN, as 0/0 is.  One exception: where a multiple of four query
  * heads shares a bf16 KV head of 64 or 128 dims the products take their operands in bf16 parts, and an infinity in a query, or
  * in a key or value that the row sees, gives NaN.  None of these calls records the event pair of uocr_b200_workspace_set_timing.
